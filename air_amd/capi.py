@@ -44,6 +44,13 @@ EPILOGUE_SWIGLU = 2
 EPILOGUE_RESIDUAL_LOAD = 3
 EPILOGUE_RESIDUAL_PREFILL = 4
 
+KV8_I8 = 1
+KV8_E4M3 = 2
+KV8_BLOCK_TOKENS = 16
+KV8_WEIGHTS_NONE = 0
+KV8_WEIGHTS_ADD = 1
+KV8_WEIGHTS_SET = 2
+
 LINEAR_AUTO = 0
 LINEAR_DECODE = 1
 LINEAR_PREFILL = 2
@@ -92,6 +99,22 @@ class KvLayout(ctypes.Structure):
         ("pool_pages", ctypes.c_uint32),
         ("chunks", ctypes.c_void_p),       # device chunk table (null: one pool)
         ("chunk_shift", ctypes.c_uint32),
+    ]
+
+
+class Kv8Layout(ctypes.Structure):
+    """air_hip_kv8_layout: the paged 8-bit KV cache."""
+    _fields_ = [
+        ("pool", ctypes.c_void_p),
+        ("page_tokens", ctypes.c_uint32),
+        ("kv_heads", ctypes.c_uint32),
+        ("head_dim", ctypes.c_uint32),
+        ("layers", ctypes.c_uint32),
+        ("max_pages", ctypes.c_uint32),
+        ("pool_pages", ctypes.c_uint32),
+        ("chunks", ctypes.c_void_p),       # device chunk table (null: one pool)
+        ("chunk_shift", ctypes.c_uint32),
+        ("type", ctypes.c_int32),          # KV8_I8 or KV8_E4M3
     ]
 
 
@@ -148,6 +171,11 @@ SIGNATURES = {
     "air_hip_add_rms_norm": (_I, [_P, _P, _P, _P, _P, _U32, _U64, ctypes.c_double]),
     "air_hip_attention_make_tiles": (_I, [_P, _U32, _U32, _U32, _P, _U32, _P]),
     "air_hip_attention_online": (_I, [_P, _P, _P, _U64, _U32, _P, _P, _U32, _U32, _U32, _U32, _P, _U32, _U64, _P]),
+    "air_hip_kv8_page_bytes": (_U64, [_P]),
+    "air_hip_kv8_append": (_I, [_P, _P, _P, _U64, _U64, _U32, _P, _P, _U32]),
+    "air_hip_kv8_read": (_I, [_P, _P, _U32, _P, _P, _P, _U32, _U32, _U64, _P, _P, _P]),
+    "air_hip_kv8_attention": (_I, [_P, _P, _P, _U64, _U32, _P, _P, _U32, _U32, _P, _U32, _U64, _I, _P]),
+    "air_hip_kv8_evict": (_I, [_P, _P, _U32, _P, _P, _P, _U32, _U32, _U32, _U32, _U32, _U64, _P]),
     "air_hip_silu_mul": (_I, [_P, _P, _P, _U32, _U64]),
     "air_hip_silu_mul_prefill": (_I, [_P, _P, _P, _U32, _U64]),
     "air_hip_rms_norm_prefill": (_I, [_P, _P, _P, _P, _P, _U32, _U64, ctypes.c_double]),
@@ -216,6 +244,11 @@ def ptr(obj) -> int:
 
 def canonical_bytes(type_id: int, k: int, n: int) -> int:
     return int(lib().air_hip_canonical_bytes(type_id, k, n))
+
+
+def kv8_page_bytes(layout: "Kv8Layout") -> int:
+    """Bytes of a page of an 8-bit KV cache (0: the layout is not valid)."""
+    return int(lib().air_hip_kv8_page_bytes(ctypes.byref(layout)))
 
 
 def device_count() -> int:

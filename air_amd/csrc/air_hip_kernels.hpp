@@ -384,6 +384,60 @@ hipError_t launch_attention_tiles(const KvLayout& kv, const float* qkv, std::uin
                                   std::uint32_t q_heads, std::uint32_t kv_heads, std::uint32_t head_dim,
                                   const AttentionTile* tiles, std::uint32_t tile_count, std::uint32_t splits,
                                   float* partials, float* out, hipStream_t stream);
+// ---- the paged 8-bit KV cache (kv8.hip, attention_kv8.hip) --------------------
+
+constexpr unsigned kKv8Block = 16;   // tokens that share a scale
+constexpr int kKv8I8 = 1, kKv8E4M3 = 2;
+
+struct Kv8Geometry {
+    unsigned char* pool;              // contiguous pool, or null when chunks is set
+    unsigned char* const* chunks;     // pool_pages >> chunk_shift chunk bases (null: not allocated)
+    std::uint64_t page_bytes;
+    std::uint32_t record_bytes;       // of a block: 128 + 32 * head_dim
+    std::uint32_t page_blocks;        // blocks per page
+    std::uint32_t page_magic;         // block / page_blocks = umulhi(block, magic); 0: one block a page
+    std::uint32_t max_pages;          // page-table row length
+    std::uint32_t pool_pages;         // page ids accepted: [0, pool_pages)
+    std::uint32_t chunk_shift;
+    std::uint32_t layers;
+    std::uint32_t kv_heads;
+    std::uint32_t head_dim;           // 64 or 128
+    int type;                         // kKv8I8 or kKv8E4M3
+};
+
+hipError_t launch_kv8_append(const Kv8Geometry& g, const float* qkv, std::uint64_t stride, std::uint64_t q_width,
+                             std::uint32_t m, const std::int32_t* positions, const std::int32_t* tables,
+                             std::uint32_t layer, hipStream_t stream);
+// starts, k, v and weights may be null.
+hipError_t launch_kv8_read(const Kv8Geometry& g, std::uint32_t seqs, const std::int32_t* starts,
+                           const std::int32_t* lengths, const std::int32_t* tables, std::uint32_t layer,
+                           std::uint32_t layers, std::uint64_t max_tokens, float* k, float* v, float* weights,
+                           hipStream_t stream);
+hipError_t launch_kv8_evict(const Kv8Geometry& g, std::uint32_t seqs, const std::int32_t* lengths,
+                            const std::int32_t* tables, const std::int32_t* new_tables, std::uint32_t layer,
+                            std::uint32_t layers, std::uint32_t keep_first, std::uint32_t keep_last,
+                            std::uint32_t budget, std::uint64_t max_tokens, std::int32_t* kept, hipStream_t stream);
+
+// How a call's attention is cut: `splits` workgroups of split_chunks 64-token
+// chunks over a tile's keys.
+struct Kv8Shape {
+    std::uint32_t tiles;          // grid x
+    std::uint32_t tile_heads;     // grid y
+    std::uint32_t splits;         // grid z
+    std::uint32_t split_chunks;
+};
+Kv8Shape kv8_attention_shape(std::uint32_t m, std::uint32_t q_heads, std::uint32_t kv_heads, std::uint64_t max_tokens);
+// Bytes of scratch: the splits' partials and, with weights, the rows' softmax
+// statistics.
+std::uint64_t kv8_attention_scratch(const Kv8Shape& shape, std::uint32_t m, std::uint32_t q_heads,
+                                    std::uint32_t head_dim, bool weights);
+// weights: 0 none, 1 add, 2 set.  run_starts may be null (every row its own run).
+hipError_t launch_kv8_attention(const Kv8Geometry& g, const float* qkv, std::uint64_t stride, std::uint32_t m,
+                                const std::int32_t* positions, const std::int32_t* tables, std::uint32_t layer,
+                                std::uint32_t q_heads, const std::int32_t* run_starts, std::uint32_t runs,
+                                std::uint64_t max_tokens, int weights, const Kv8Shape& shape, void* scratch, float* out,
+                                hipStream_t stream);
+
 hipError_t launch_silu_mul(const float* gate_up, float* out, std::uint32_t m, std::uint64_t ffn, hipStream_t stream);
 // The RMSNorm (with the residual add first when y is given) and the SwiGLU,
 // each also writing its output as the next prefill linear's operand

@@ -1,0 +1,542 @@
+// attention_kv8.hip -- attention over the paged 8-bit KV cache, and the
+// attention weights it gathers.
+//
+//   s_t = (q . k_t) / sqrt(D),  p_t = e^(s_t - m) / sum e^(s - m),
+//   out = sum_t p_t v_t,        weight_t (+)= sum over rows and q heads of p_t
+//
+// Codes are exact in f16, and an f32 operand is the sum of two f16 values to
+// 22 bits (its rounding and the rounding of what that leaves), so both
+// products run on v_mfma_f32_16x16x32_f16 with two instructions where one
+// f16 operand would take one: q = hi + lo against K codes, p = hi + lo
+// against V codes, summed in f32.  The result differs from a float64
+// attention over the same codes by ~5e-7 relative, as an f32 computation
+// does; a single f16 p would leave 2e-4.
+//
+// A wave walks chunks of 64 tokens (four blocks) of one KV head for 16 query
+// vectors, with nothing staged in LDS:
+//
+//   S^T = K Q^T   row i of tile b is token 4 b + i % 4 of block i / 4, so
+//                 lane (vector, g) ends with all 16 tokens of block g, in
+//                 order: one scale of K and of V a lane, and p lies as
+//   O^T += V^T P^T  wants it, 8 tokens of block g in lane group g a step.
+//
+// So the record's K and V codes go from memory into operand registers, a
+// vector's statistics stay in its lanes (lane % 16), and an output lane holds
+// four consecutive dims of one vector.
+//
+// Running references are integers, in powers of two: M >= every s log2(e) so
+// far (for the denominator) and M2 >= every s log2(e) + log2(scale of V) (for
+// the numerators, whose p carries V's scale: a block of large values does not
+// take the low bits of the others).  Rescaling by a power of two is exact.
+#include "air_hip_device.hpp"
+#include "air_hip_kernels.hpp"
+#include "air_hip_kv8.hpp"
+
+namespace air_hip {
+namespace {
+
+constexpr unsigned kWaves = 4;
+constexpr unsigned kThreads = 64 * kWaves;
+constexpr unsigned kVectors = 16;          // query vectors of a tile
+constexpr unsigned kChunkBlocks = 4;       // blocks of a chunk, one per lane group
+constexpr unsigned kChunkTokens = kChunkBlocks * kKv8Block;
+constexpr int kNone = -(1 << 30);          // a reference that no score has set
+constexpr int kPBits = 15;                 // p' < 2^15 in f16: the largest p' keeps 2^-38 of itself
+constexpr unsigned kStat = 4;              // floats before a partial's D sums
+
+// Codes of blocks without a page: any finite value will do under a mask.
+__device__ __align__(16) unsigned char g_no_record[kKv8Codes + 2 * kKv8Block * 128];
+
+// 16 code bytes as two f16 operands of eight.
+template <int TYPE>
+__device__ __forceinline__ void codes_to_half(const u32x4& c, half8v& a, half8v& b) {
+    half2v h[8];
+#pragma unroll
+    for (unsigned i = 0; i < 4u; ++i) {
+        if constexpr (TYPE == kKv8I8) {
+            q8_dword_to_half(c[i], h[2u * i], h[2u * i + 1u]);
+        } else {
+            h[2u * i] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c[i], 1.0f, false);
+            h[2u * i + 1u] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c[i], 1.0f, true);
+        }
+    }
+#pragma unroll
+    for (unsigned i = 0; i < 4u; ++i) {
+        a[2u * i] = h[i][0];
+        a[2u * i + 1u] = h[i][1];
+        b[2u * i] = h[4u + i][0];
+        b[2u * i + 1u] = h[4u + i][1];
+    }
+}
+
+// x = hi + lo to 22 bits.
+__device__ __forceinline__ void split_f16(float x, _Float16& hi, _Float16& lo) {
+    hi = static_cast<_Float16>(x);
+    lo = static_cast<_Float16>(x - static_cast<float>(hi));
+}
+
+// The B operands of the products with K of one query vector (lane % 16), and
+// the factor that undoes their power-of-two scale: the vector's largest
+// magnitude lies in [2^8, 2^9), so that hi and lo are normal f16 down to
+// 2^-31 of it.
+template <unsigned D>
+struct QueryFragments {
+    half8v hi[D / 32], lo[D / 32];
+    float undo;
+};
+
+template <unsigned D>
+__device__ __forceinline__ void load_query(const float* q, unsigned grp, QueryFragments<D>& f) {
+    float x[D / 4];
+    float top = 0.0f;
+#pragma unroll
+    for (unsigned s = 0; s < D / 64u; ++s) {
+#pragma unroll
+        for (unsigned i = 0; i < 4u; ++i) {
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (q) v = *reinterpret_cast<const float4*>(q + 64u * s + 16u * grp + 4u * i);
+            x[16u * s + 4u * i] = v.x;
+            x[16u * s + 4u * i + 1u] = v.y;
+            x[16u * s + 4u * i + 2u] = v.z;
+            x[16u * s + 4u * i + 3u] = v.w;
+        }
+    }
+#pragma unroll
+    for (unsigned i = 0; i < D / 4u; ++i) top = fmaxf(top, fabsf(x[i]));
+    top = fmaxf(top, __shfl_xor(top, 16));
+    top = fmaxf(top, __shfl_xor(top, 32));
+    int e = static_cast<int>(__float_as_uint(top) >> 23) - 127;   // -127: zero or subnormal; 128: not finite
+    e = e < -110 ? -110 : e > 120 ? 120 : e;
+    const float scale = __uint_as_float(static_cast<std::uint32_t>(127 + 8 - e) << 23);
+    f.undo = __uint_as_float(static_cast<std::uint32_t>(127 - 8 + e) << 23);
+#pragma unroll
+    for (unsigned i = 0; i < D / 32u; ++i) {
+#pragma unroll
+        for (unsigned j = 0; j < 8u; ++j) {
+            _Float16 hi, lo;
+            split_f16(x[8u * i + j] * scale, hi, lo);
+            f.hi[i][j] = hi;
+            f.lo[i][j] = lo;
+        }
+    }
+}
+
+// A lane's codes of the chunk's K: tile b, 64-dim step s.
+template <unsigned D>
+struct KeyCodes {
+    u32x4 c[4][D / 64];
+};
+
+template <unsigned D>
+__device__ __forceinline__ void load_keys(const unsigned char* rec, unsigned lane, KeyCodes<D>& k) {
+    const unsigned char* const at = rec + kKv8Codes + (lane >> 4) * 64u + (lane & 3u) * 16u;
+#pragma unroll
+    for (unsigned b = 0; b < 4u; ++b) {
+#pragma unroll
+        for (unsigned s = 0; s < D / 64u; ++s) {
+            k.c[b][s] = *reinterpret_cast<const u32x4*>(at + b * (D * 4u) + s * 256u);
+        }
+    }
+}
+
+// S^T of the chunk: score[b][r] is token 4 b + r of this lane's block for
+// vector lane % 16, times the fragments' scale.
+template <int TYPE, unsigned D>
+__device__ __forceinline__ void chunk_scores(const KeyCodes<D>& k, const QueryFragments<D>& q, float4v score[4]) {
+#pragma unroll
+    for (unsigned b = 0; b < 4u; ++b) {
+        score[b] = float4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (unsigned s = 0; s < D / 64u; ++s) {
+            half8v a0, a1;
+            codes_to_half<TYPE>(k.c[b][s], a0, a1);
+            score[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, q.hi[2u * s], score[b], 0, 0, 0);
+            score[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, q.lo[2u * s], score[b], 0, 0, 0);
+            score[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, q.hi[2u * s + 1u], score[b], 0, 0, 0);
+            score[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, q.lo[2u * s + 1u], score[b], 0, 0, 0);
+        }
+    }
+}
+
+// One row's heads (or up to 16 of them) of one KV head per workgroup; its
+// waves take the chunks of split blockIdx.z in turn.
+template <int TYPE, unsigned D>
+__global__ __launch_bounds__(kThreads) void kv8_attention_kernel(
+    Kv8Geometry g, const float* __restrict__ qkv, std::uint64_t stride, const std::int32_t* __restrict__ positions,
+    const std::int32_t* __restrict__ tables, std::uint32_t layer, std::uint32_t q_heads, std::uint64_t max_tokens,
+    std::uint32_t split_chunks, float score_scale, float* __restrict__ partials, float2* __restrict__ stats,
+    float* __restrict__ out) {
+    constexpr unsigned LD = D + 4;
+    __shared__ float sums[kWaves][kVectors][LD];
+    __shared__ int wave_m[kWaves][kVectors], wave_m2[kWaves][kVectors];
+    __shared__ float wave_l[kWaves][kVectors];
+    const unsigned tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, grp = lane >> 4, col = lane & 15u;
+    const std::uint32_t row = blockIdx.x, split = blockIdx.z;
+    const std::uint32_t group = q_heads / g.kv_heads, parts = (group + kVectors - 1u) / kVectors;
+    const std::uint32_t kvh = blockIdx.y / parts, part = blockIdx.y % parts;
+    const std::uint32_t head0 = kvh * group + part * kVectors;
+    const std::uint32_t nq = group - part * kVectors < kVectors ? group - part * kVectors : kVectors;
+    std::int64_t last = positions[row];
+    if (last >= static_cast<std::int64_t>(max_tokens)) last = static_cast<std::int64_t>(max_tokens) - 1;
+    const std::uint32_t chunks = last < 0 ? 0u : static_cast<std::uint32_t>(last / kChunkTokens) + 1u;
+    const std::uint32_t live = chunks == 0u ? 1u : (chunks + split_chunks - 1u) / split_chunks;
+    if (split >= live) return;
+    const std::int32_t* const table = tables + static_cast<std::uint64_t>(row) * g.max_pages;
+    const std::uint32_t end = chunks < (split + 1u) * split_chunks ? chunks : (split + 1u) * split_chunks;
+
+    QueryFragments<D> q;
+    load_query<D>(col < nq ? qkv + static_cast<std::uint64_t>(row) * stride + static_cast<std::uint64_t>(head0 + col) * D
+                           : nullptr,
+                  grp, q);
+    const float lane_scale = q.undo * score_scale;
+
+    int m = kNone, m2 = kNone;
+    float l = 0.0f;
+    float4v o[D / 16];
+#pragma unroll
+    for (unsigned t = 0; t < D / 16u; ++t) o[t] = float4v{0.f, 0.f, 0.f, 0.f};
+
+    for (std::uint32_t c = split * split_chunks + wave; c < end; c += kWaves) {
+        const unsigned char* const krec0 = kv8_record(g, table, layer, kvh, c * kChunkBlocks + (col >> 2));
+        const unsigned char* const vrec0 = kv8_record(g, table, layer, kvh, c * kChunkBlocks + grp);
+        const unsigned char* const krec = krec0 ? krec0 : g_no_record;
+        const unsigned char* const vrec = vrec0 ? vrec0 : g_no_record;
+        KeyCodes<D> keys;
+        load_keys<D>(krec, lane, keys);
+        const float2 scales = *reinterpret_cast<const float2*>(vrec);
+        u32x4 vals[D / 16];
+#pragma unroll
+        for (unsigned t = 0; t < D / 16u; ++t) {
+            vals[t] = *reinterpret_cast<const u32x4*>(vrec + kKv8Codes + kKv8Block * D + (16u * t + col) * 16u);
+        }
+        float4v s[4];
+        chunk_scores<TYPE, D>(keys, q, s);
+        // Tokens of this lane's block that the row attends to.
+        const std::int64_t first = (static_cast<std::int64_t>(c) * kChunkBlocks + grp) * kKv8Block;
+        const int limit = vrec0 == nullptr || last < first ? -1 : last - first > 15 ? 15 : static_cast<int>(last - first);
+        const float factor = lane_scale * scales.x;
+        float top = -__builtin_huge_valf();
+#pragma unroll
+        for (unsigned b = 0; b < 4u; ++b) {
+#pragma unroll
+            for (unsigned r = 0; r < 4u; ++r) {
+                const float x = s[b][r] * factor;
+                s[b][r] = static_cast<int>(4u * b + r) <= limit ? x : -__builtin_huge_valf();
+                top = fmaxf(top, s[b][r]);
+            }
+        }
+        // References: the block's own, then the vector's over the four blocks.
+        const float bound = fminf(fmaxf(ceilf(top), -0x1p28f), 0x1p28f);   // differences stay in 32 bits
+        const int block_m = top == -__builtin_huge_valf() ? kNone : static_cast<int>(bound);
+        const int exponent = __builtin_amdgcn_frexp_expf(scales.y);   // scale < 2^exponent
+        const int block_m2 = block_m == kNone || scales.y == 0.0f ? kNone : block_m + exponent;
+        int m_new = block_m > m ? block_m : m, m2_new = block_m2 > m2 ? block_m2 : m2;
+#pragma unroll
+        for (int off = 16; off <= 32; off <<= 1) {
+            const int a = __shfl_xor(m_new, off), a2 = __shfl_xor(m2_new, off);
+            m_new = a > m_new ? a : m_new;
+            m2_new = a2 > m2_new ? a2 : m2_new;
+        }
+        // p' = 2^(s - base) * share, at most 2^kPBits; a scale of V far below
+        // the others' (or zero) keeps base near M, so the same powers also
+        // sum up the denominator.
+        int e = m2_new - kPBits - m_new - 40;
+        e = scales.y == 0.0f || exponent < e ? e : exponent;
+        const int base = m2_new - e - kPBits;
+        const float share = __builtin_amdgcn_ldexpf(scales.y, -e);
+        const float fbase = static_cast<float>(base);
+        float sum = 0.0f;
+        half8v p_hi[2], p_lo[2];
+#pragma unroll
+        for (unsigned b = 0; b < 4u; ++b) {
+#pragma unroll
+            for (unsigned r = 0; r < 4u; ++r) {
+                const float x = __builtin_amdgcn_exp2f(s[b][r] - fbase);
+                sum += x;
+                _Float16 hi, lo;
+                split_f16(x * share, hi, lo);
+                p_hi[b >> 1][4u * (b & 1u) + r] = hi;
+                p_lo[b >> 1][4u * (b & 1u) + r] = lo;
+            }
+        }
+        l = __builtin_amdgcn_ldexpf(l, m - m_new) + __builtin_amdgcn_ldexpf(sum, base - m_new);
+        const int down = m2 - m2_new;
+        if (__any(down != 0)) {
+#pragma unroll
+            for (unsigned t = 0; t < D / 16u; ++t) {
+#pragma unroll
+                for (unsigned r = 0; r < 4u; ++r) o[t][r] = __builtin_amdgcn_ldexpf(o[t][r], down);
+            }
+        }
+        m = m_new;
+        m2 = m2_new;
+        if constexpr (TYPE == kKv8E4M3) {
+            // Slots behind the row's last token may hold NaN codes, which a
+            // zero p does not silence.
+            if (__any(limit < 15)) {
+                const int n = limit + 1;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    const int bytes = n - 4 * w;
+                    const std::uint32_t mask = bytes >= 4 ? 0xffffffffu : bytes <= 0 ? 0u : (1u << (8 * bytes)) - 1u;
+#pragma unroll
+                    for (unsigned t = 0; t < D / 16u; ++t) vals[t][w] &= mask;
+                }
+            }
+        }
+#pragma unroll
+        for (unsigned t = 0; t < D / 16u; ++t) {
+            half8v a0, a1;
+            codes_to_half<TYPE>(vals[t], a0, a1);
+            o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, p_hi[0], o[t], 0, 0, 0);
+            o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, p_lo[0], o[t], 0, 0, 0);
+            o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, p_hi[1], o[t], 0, 0, 0);
+            o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, p_lo[1], o[t], 0, 0, 0);
+        }
+    }
+
+    // The waves meet: sums in units of 2^(M2 - kPBits), l of 2^M.
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    if (grp == 0u) {
+        wave_m[wave][col] = m;
+        wave_m2[wave][col] = m2;
+        wave_l[wave][col] = l;
+    }
+#pragma unroll
+    for (unsigned t = 0; t < D / 16u; ++t) *reinterpret_cast<float4v*>(&sums[wave][col][16u * t + 4u * grp]) = o[t];
+    __syncthreads();
+    for (unsigned idx = tid; idx < nq * (D / 4u); idx += kThreads) {
+        const unsigned v = idx / (D / 4u), d4 = idx % (D / 4u);
+        int mm = kNone, mm2 = kNone;
+#pragma unroll
+        for (unsigned w = 0; w < kWaves; ++w) {
+            mm = wave_m[w][v] > mm ? wave_m[w][v] : mm;
+            mm2 = wave_m2[w][v] > mm2 ? wave_m2[w][v] : mm2;
+        }
+        float total = 0.0f;
+        float4v acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (unsigned w = 0; w < kWaves; ++w) {
+            total += __builtin_amdgcn_ldexpf(wave_l[w][v], wave_m[w][v] - mm);
+            const float4v a = *reinterpret_cast<const float4v*>(&sums[w][v][4u * d4]);
+#pragma unroll
+            for (unsigned r = 0; r < 4u; ++r) acc[r] += __builtin_amdgcn_ldexpf(a[r], wave_m2[w][v] - mm2);
+        }
+        const std::uint64_t vector = static_cast<std::uint64_t>(row) * q_heads + head0 + v;
+        if (live == 1u) {
+            float4v y;
+#pragma unroll
+            for (unsigned r = 0; r < 4u; ++r) {
+                y[r] = total == 0.0f ? 0.0f : __builtin_amdgcn_ldexpf(acc[r] / total, mm2 - kPBits - mm);
+            }
+            *reinterpret_cast<float4v*>(out + vector * D + 4u * d4) = y;
+            if (stats && d4 == 0u) stats[vector] = make_float2(static_cast<float>(mm), total == 0.0f ? 0.0f : 1.0f / total);
+        } else {
+            float* const p = partials + (vector * gridDim.z + split) * (D + kStat);
+            if (d4 == 0u) {
+                *reinterpret_cast<float4v*>(p) = float4v{__int_as_float(mm), __int_as_float(mm2), total, 0.0f};
+            }
+            *reinterpret_cast<float4v*>(p + kStat + 4u * d4) = acc;
+        }
+    }
+}
+
+// Joins the splits of a row's vectors.
+template <unsigned D>
+__global__ __launch_bounds__(kThreads) void kv8_merge_kernel(const std::int32_t* __restrict__ positions,
+                                                             std::uint32_t q_heads, std::uint64_t max_tokens,
+                                                             std::uint32_t split_chunks, std::uint32_t splits,
+                                                             const float* __restrict__ partials,
+                                                             float2* __restrict__ stats, float* __restrict__ out) {
+    const std::uint32_t row = blockIdx.x;
+    const unsigned idx = blockIdx.y * kThreads + threadIdx.x;
+    if (idx >= q_heads * (D / 4u)) return;
+    std::int64_t last = positions[row];
+    if (last >= static_cast<std::int64_t>(max_tokens)) last = static_cast<std::int64_t>(max_tokens) - 1;
+    const std::uint32_t chunks = last < 0 ? 0u : static_cast<std::uint32_t>(last / kChunkTokens) + 1u;
+    const std::uint32_t live = (chunks + split_chunks - 1u) / split_chunks;
+    if (live <= 1u) return;   // the attention kernel wrote this row
+    const unsigned v = idx / (D / 4u), d4 = idx % (D / 4u);
+    const std::uint64_t vector = static_cast<std::uint64_t>(row) * q_heads + v;
+    const float* const base = partials + vector * splits * (D + kStat);
+    int m = kNone, m2 = kNone;
+    float total = 0.0f;
+    float4v acc = {0.f, 0.f, 0.f, 0.f};
+    for (std::uint32_t s = 0; s < live; ++s) {
+        const float4v head = *reinterpret_cast<const float4v*>(base + s * (D + kStat));
+        const float4v a = *reinterpret_cast<const float4v*>(base + s * (D + kStat) + kStat + 4u * d4);
+        const int pm = __float_as_int(head[0]), pm2 = __float_as_int(head[1]);
+        const int nm = pm > m ? pm : m, nm2 = pm2 > m2 ? pm2 : m2;
+        total = __builtin_amdgcn_ldexpf(total, m - nm) + __builtin_amdgcn_ldexpf(head[2], pm - nm);
+#pragma unroll
+        for (unsigned r = 0; r < 4u; ++r) {
+            acc[r] = __builtin_amdgcn_ldexpf(acc[r], m2 - nm2) + __builtin_amdgcn_ldexpf(a[r], pm2 - nm2);
+        }
+        m = nm;
+        m2 = nm2;
+    }
+    float4v y;
+#pragma unroll
+    for (unsigned r = 0; r < 4u; ++r) {
+        y[r] = total == 0.0f ? 0.0f : __builtin_amdgcn_ldexpf(acc[r] / total, m2 - kPBits - m);
+    }
+    *reinterpret_cast<float4v*>(out + vector * D + 4u * d4) = y;
+    if (stats && d4 == 0u) stats[vector] = make_float2(static_cast<float>(m), total == 0.0f ? 0.0f : 1.0f / total);
+}
+
+// The weights a run's rows give one chunk of tokens: the scores again, by the
+// same instructions as in the attention, and p from the rows' statistics.
+// A chunk of a (run, KV head) has one wave, which adds its sums with one
+// atomic a token: a page that two runs share loses nothing, and elsewhere the
+// single addition leaves one order.
+template <int TYPE, unsigned D>
+__global__ __launch_bounds__(kThreads) void kv8_weights_kernel(
+    Kv8Geometry g, const float* __restrict__ qkv, std::uint64_t stride, std::uint32_t m,
+    const std::int32_t* __restrict__ positions, const std::int32_t* __restrict__ tables, std::uint32_t layer,
+    std::uint32_t q_heads, const std::int32_t* __restrict__ run_starts, std::uint64_t max_tokens, float score_scale,
+    const float2* __restrict__ stats, bool add) {
+    const unsigned tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, grp = lane >> 4, col = lane & 15u;
+    const std::uint32_t kvh = blockIdx.y, run = blockIdx.z;
+    std::int64_t begin = run, end = static_cast<std::int64_t>(run) + 1;
+    if (run_starts) {
+        begin = run_starts[run];
+        end = run_starts[run + 1u];
+    }
+    begin = begin < 0 ? 0 : begin;
+    end = end > static_cast<std::int64_t>(m) ? static_cast<std::int64_t>(m) : end;
+    if (begin >= end) return;
+    const std::uint32_t chunk = blockIdx.x * kWaves + wave;
+    const std::int64_t token0 = static_cast<std::int64_t>(chunk) * kChunkTokens;
+    const std::int32_t* const table = tables + static_cast<std::uint64_t>(begin) * g.max_pages;
+    const std::uint32_t group = q_heads / g.kv_heads;
+    // Tokens past the run's last position (or max_tokens) are not held.
+    std::int64_t last = -1;
+    for (std::int64_t r = begin + lane; r < end; r += 64) last = positions[r] > last ? positions[r] : last;
+    for (int off = 32; off > 0; off >>= 1) {
+        const std::int64_t o = __shfl_xor(static_cast<int>(last), off);
+        last = o > last ? o : last;
+    }
+    if (last >= static_cast<std::int64_t>(max_tokens)) last = static_cast<std::int64_t>(max_tokens) - 1;
+    if (token0 > last) return;
+    const unsigned char* const krec0 = kv8_record(g, table, layer, kvh, chunk * kChunkBlocks + (col >> 2));
+    unsigned char* const vrec0 = kv8_record(g, table, layer, kvh, chunk * kChunkBlocks + grp);
+    KeyCodes<D> keys;
+    load_keys<D>(krec0 ? krec0 : g_no_record, lane, keys);
+    const float k_scale = *reinterpret_cast<const float*>(vrec0 ? vrec0 : g_no_record);
+    const std::int64_t first = token0 + grp * kKv8Block;
+    float sum[4][4] = {};
+    const std::int64_t vectors = (end - begin) * group;
+    for (std::int64_t v0 = 0; v0 < vectors; v0 += kVectors) {
+        const std::int64_t v = v0 + col;
+        const bool active = v < vectors;
+        const std::int64_t r = begin + (active ? v / group : 0);
+        const std::uint64_t head = static_cast<std::uint64_t>(kvh) * group + (active ? v % group : 0);
+        std::int64_t upto = active ? positions[r] : -1;
+        if (upto >= static_cast<std::int64_t>(max_tokens)) upto = static_cast<std::int64_t>(max_tokens) - 1;
+        if (!__any(upto >= token0)) continue;
+        QueryFragments<D> q;
+        load_query<D>(active ? qkv + static_cast<std::uint64_t>(r) * stride + head * D : nullptr, grp, q);
+        const float2 st = active ? stats[static_cast<std::uint64_t>(r) * q_heads + head] : make_float2(0.f, 0.f);
+        float4v s[4];
+        chunk_scores<TYPE, D>(keys, q, s);
+        const float factor = q.undo * score_scale * k_scale;
+        const int limit = vrec0 == nullptr || upto < first ? -1 : upto - first > 15 ? 15 : static_cast<int>(upto - first);
+#pragma unroll
+        for (unsigned b = 0; b < 4u; ++b) {
+#pragma unroll
+            for (unsigned i = 0; i < 4u; ++i) {
+                const float p = __builtin_amdgcn_exp2f(s[b][i] * factor - st.x) * st.y;
+                sum[b][i] += static_cast<int>(4u * b + i) <= limit ? p : 0.0f;
+            }
+        }
+    }
+#pragma unroll
+    for (unsigned b = 0; b < 4u; ++b) {
+#pragma unroll
+        for (unsigned i = 0; i < 4u; ++i) {
+#pragma unroll
+            for (int off = 1; off < 16; off <<= 1) sum[b][i] += __shfl_xor(sum[b][i], off);
+        }
+    }
+    if (vrec0 == nullptr) return;
+    float mine = 0.0f;   // lane (col, grp): token col of block grp
+#pragma unroll
+    for (unsigned t = 0; t < 16u; ++t) mine = col == t ? sum[t >> 2][t & 3u] : mine;
+    if (first + col > last) return;
+    float* const at = reinterpret_cast<float*>(vrec0 + kKv8Weights) + col;
+    if (add) {
+        atomicAdd(at, mine);
+    } else {
+        *at = mine;
+    }
+}
+
+} // namespace
+
+Kv8Shape kv8_attention_shape(std::uint32_t m, std::uint32_t q_heads, std::uint32_t kv_heads, std::uint64_t max_tokens) {
+    const std::uint32_t group = q_heads / kv_heads, parts = (group + kVectors - 1u) / kVectors;
+    const std::uint32_t chunks = static_cast<std::uint32_t>((max_tokens + kChunkTokens - 1u) / kChunkTokens);
+    // Splits of equal length, so that rows of unequal lengths make workgroups
+    // of equal work: at least two chunks a wave, and at most about four
+    // workgroups a CU if every row were max_tokens long.
+    const std::uint64_t tiles = static_cast<std::uint64_t>(m) * kv_heads * parts;
+    std::uint64_t per = (tiles * chunks + 1023u) / 1024u;
+    per = (per + kWaves - 1u) / kWaves * kWaves;
+    if (per < 2u * kWaves) per = 2u * kWaves;
+    if (per > chunks) per = chunks;
+    const std::uint32_t splits = static_cast<std::uint32_t>((chunks + per - 1u) / per);
+    return Kv8Shape{m, kv_heads * parts, splits, static_cast<std::uint32_t>(per)};
+}
+
+std::uint64_t kv8_attention_scratch(const Kv8Shape& shape, std::uint32_t m, std::uint32_t q_heads,
+                                    std::uint32_t head_dim, bool weights) {
+    const std::uint64_t vectors = static_cast<std::uint64_t>(m) * q_heads;
+    const std::uint64_t stats = weights ? (vectors * sizeof(float2) + 255u) / 256u * 256u : 0u;
+    return stats + (shape.splits > 1u ? vectors * shape.splits * (head_dim + kStat) * sizeof(float) : 0u);
+}
+
+hipError_t launch_kv8_attention(const Kv8Geometry& g, const float* qkv, std::uint64_t stride, std::uint32_t m,
+                                const std::int32_t* positions, const std::int32_t* tables, std::uint32_t layer,
+                                std::uint32_t q_heads, const std::int32_t* run_starts, std::uint32_t runs,
+                                std::uint64_t max_tokens, int weights, const Kv8Shape& shape, void* scratch, float* out,
+                                hipStream_t stream) {
+    const std::uint64_t vectors = static_cast<std::uint64_t>(m) * q_heads;
+    float2* const stats = weights ? static_cast<float2*>(scratch) : nullptr;
+    float* const partials = reinterpret_cast<float*>(
+        static_cast<unsigned char*>(scratch) + (weights ? (vectors * sizeof(float2) + 255u) / 256u * 256u : 0u));
+    // Scores in powers of two: s log2(e) = (q . k) * log2(e) / sqrt(D).
+    const float scale = static_cast<float>(1.4426950408889634 / __builtin_sqrt(static_cast<double>(g.head_dim)));
+    const dim3 grid(shape.tiles, shape.tile_heads, shape.splits);
+    const std::uint64_t chunks = (max_tokens + kChunkTokens - 1u) / kChunkTokens;
+    const dim3 weight_grid(static_cast<unsigned>((chunks + kWaves - 1u) / kWaves), g.kv_heads, runs);
+#define AIR_KV8_ATTENTION(T, D)                                                                                     \
+    hipLaunchKernelGGL((kv8_attention_kernel<T, D>), grid, dim3(kThreads), 0, stream, g, qkv, stride, positions, tables, \
+                       layer, q_heads, max_tokens, shape.split_chunks, scale, partials, stats, out);                \
+    if (shape.splits > 1u) {                                                                                        \
+        hipLaunchKernelGGL(kv8_merge_kernel<D>, dim3(m, (q_heads * (D / 4u) + kThreads - 1u) / kThreads),           \
+                           dim3(kThreads), 0, stream, positions, q_heads, max_tokens, shape.split_chunks, shape.splits, \
+                           partials, stats, out);                                                                   \
+    }                                                                                                               \
+    if (weights) {                                                                                                  \
+        hipLaunchKernelGGL((kv8_weights_kernel<T, D>), weight_grid, dim3(kThreads), 0, stream, g, qkv, stride, m,   \
+                           positions, tables, layer, q_heads, run_starts, max_tokens, scale, stats, weights == 1);  \
+    }
+    if (g.type == kKv8I8) {
+        if (g.head_dim == 128u) {
+            AIR_KV8_ATTENTION(kKv8I8, 128)
+        } else {
+            AIR_KV8_ATTENTION(kKv8I8, 64)
+        }
+    } else {
+        if (g.head_dim == 128u) {
+            AIR_KV8_ATTENTION(kKv8E4M3, 128)
+        } else {
+            AIR_KV8_ATTENTION(kKv8E4M3, 64)
+        }
+    }
+#undef AIR_KV8_ATTENTION
+    return hipGetLastError();
+}
+
+} // namespace air_hip

@@ -2189,3 +2189,210 @@ int air_hip_argmax(air_hip_context* ctx, const float* logits, uint32_t m, uint64
 }
 
 } // extern "C"
+
+// ---- the paged 8-bit KV cache ------------------------------------------------
+
+namespace {
+static_assert(AIR_HIP_KV8_I8 == kKv8I8 && AIR_HIP_KV8_E4M3 == kKv8E4M3, "cache types agree");
+static_assert(AIR_HIP_KV8_BLOCK_TOKENS == kKv8Block, "block lengths agree");
+
+// Rows of one append launch: its workgroups look for rows of their block
+// among all of them.
+constexpr std::uint32_t kKv8AppendRows = 2048;
+
+std::uint64_t kv8_record_bytes(const air_hip_kv8_layout* kv) { return 128u + 32ull * kv->head_dim; }
+
+// Shape of the layout; the pool is checked by the calls that touch it.
+int check_kv8_shape(const air_hip_kv8_layout* kv) {
+    if (!kv) return fail(AIR_HIP_INVALID_ARGUMENT, "8-bit KV layout must not be null");
+    if (kv->type != AIR_HIP_KV8_I8 && kv->type != AIR_HIP_KV8_E4M3) {
+        return fail(AIR_HIP_INVALID_ARGUMENT, "8-bit KV type %d is neither i8 nor e4m3", static_cast<int>(kv->type));
+    }
+    if (kv->page_tokens == 0 || kv->kv_heads == 0 || kv->head_dim == 0 || kv->layers == 0 || kv->max_pages == 0 ||
+        kv->pool_pages == 0) {
+        return fail(AIR_HIP_INVALID_ARGUMENT, "8-bit KV layout has a zero dimension");
+    }
+    if (kv->head_dim != 64u && kv->head_dim != 128u) {
+        return fail(AIR_HIP_UNSUPPORTED, "the 8-bit KV cache supports head widths 64 and 128, not %u", kv->head_dim);
+    }
+    if (kv->page_tokens % AIR_HIP_KV8_BLOCK_TOKENS != 0u) {
+        return fail(AIR_HIP_INVALID_ARGUMENT, "8-bit KV pages hold whole blocks of %u tokens, not %u tokens",
+                    AIR_HIP_KV8_BLOCK_TOKENS, kv->page_tokens);
+    }
+    // A page is found as block * magic >> 32, exact while blocks * blocks per
+    // page fit 32 bits; tokens are int32.
+    const uint64_t per = kv->page_tokens / AIR_HIP_KV8_BLOCK_TOKENS;
+    if (kv->page_tokens > 65536u || kv->kv_heads > 65535u || kv->layers > 65535u ||
+        static_cast<uint64_t>(kv->max_pages) * kv->page_tokens > static_cast<uint64_t>(INT32_MAX) ||
+        (kv->max_pages + 4ull) * per * per > 0xffffffffull) {
+        return fail(AIR_HIP_UNSUPPORTED, "8-bit KV tables of %u pages of %u tokens are too long", kv->max_pages,
+                    kv->page_tokens);
+    }
+    if (kv->pool_pages > static_cast<uint32_t>(INT32_MAX)) {
+        return fail(AIR_HIP_INVALID_ARGUMENT, "8-bit KV pool pages must fit int32 page ids");
+    }
+    if (kv->chunks && (kv->chunk_shift > 30u || kv->pool_pages % (1u << kv->chunk_shift) != 0u)) {
+        return fail(AIR_HIP_INVALID_ARGUMENT,
+                    "chunked 8-bit KV pool: pool_pages must be a whole number of 2^chunk_shift chunks");
+    }
+    return AIR_HIP_OK;
+}
+int check_kv8(const air_hip_kv8_layout* kv) {
+    if (int rc = check_kv8_shape(kv); rc != AIR_HIP_OK) return rc;
+    if (!kv->pool && !kv->chunks) {
+        return fail(AIR_HIP_INVALID_ARGUMENT, "8-bit KV layout needs its pool or its chunk table");
+    }
+    if (!kv->chunks && reinterpret_cast<std::uintptr_t>(kv->pool) % 16u != 0) {
+        return fail(AIR_HIP_INVALID_ARGUMENT, "the 8-bit KV pool must be 16-byte aligned");
+    }
+    return AIR_HIP_OK;
+}
+uint64_t kv8_page_bytes(const air_hip_kv8_layout* kv) {
+    return static_cast<uint64_t>(kv->layers) * kv->kv_heads * (kv->page_tokens / AIR_HIP_KV8_BLOCK_TOKENS) *
+           kv8_record_bytes(kv);
+}
+Kv8Geometry kv8_geometry_of(const air_hip_kv8_layout* kv) {
+    Kv8Geometry g{};
+    g.pool = kv->chunks ? nullptr : static_cast<unsigned char*>(kv->pool);
+    g.chunks = reinterpret_cast<unsigned char* const*>(kv->chunks);
+    g.page_bytes = kv8_page_bytes(kv);
+    g.record_bytes = static_cast<std::uint32_t>(kv8_record_bytes(kv));
+    g.page_blocks = kv->page_tokens / AIR_HIP_KV8_BLOCK_TOKENS;
+    g.page_magic = g.page_blocks == 1u ? 0u : static_cast<std::uint32_t>((1ull << 32) / g.page_blocks + 1u);
+    g.max_pages = kv->max_pages;
+    g.pool_pages = kv->pool_pages;
+    g.chunk_shift = kv->chunks ? kv->chunk_shift : 0u;
+    g.layers = kv->layers;
+    g.kv_heads = kv->kv_heads;
+    g.head_dim = kv->head_dim;
+    g.type = kv->type;
+    return g;
+}
+int check_kv8_tokens(const air_hip_kv8_layout* kv, uint64_t max_tokens) {
+    if (max_tokens == 0 || max_tokens > static_cast<uint64_t>(kv->max_pages) * kv->page_tokens) {
+        return fail(AIR_HIP_INVALID_ARGUMENT, "max_tokens must be in [1, max_pages * page_tokens]");
+    }
+    return AIR_HIP_OK;
+}
+int check_kv8_layers(const air_hip_kv8_layout* kv, uint32_t layer, uint32_t layers) {
+    if (layers == 0 || layer >= kv->layers || layers > kv->layers - layer) {
+        return fail(AIR_HIP_INVALID_ARGUMENT, "layers %u..%llu are out of range", layer,
+                    static_cast<unsigned long long>(layer) + layers);
+    }
+    return AIR_HIP_OK;
+}
+} // namespace
+
+extern "C" {
+
+uint64_t air_hip_kv8_page_bytes(const air_hip_kv8_layout* kv) {
+    return check_kv8_shape(kv) == AIR_HIP_OK ? kv8_page_bytes(kv) : 0u;
+}
+
+int air_hip_kv8_append(air_hip_context* ctx, const air_hip_kv8_layout* kv, const float* qkv, uint64_t row_stride,
+                       uint64_t q_width, uint32_t m, const int32_t* positions, const int32_t* page_tables,
+                       uint32_t layer) {
+    if (!ctx || !qkv || !positions || !page_tables) return fail(AIR_HIP_INVALID_ARGUMENT, "arguments must not be null");
+    forget_loaded_source(ctx);
+    if (int rc = check_kv8(kv); rc != AIR_HIP_OK) return rc;
+    if (layer >= kv->layers) return fail(AIR_HIP_INVALID_ARGUMENT, "layer %u is out of range", layer);
+    if (row_stride < q_width + 2u * static_cast<uint64_t>(kv->kv_heads) * kv->head_dim) {
+        return fail(AIR_HIP_INVALID_ARGUMENT, "row stride is shorter than q|k|v");
+    }
+    if (m == 0) return AIR_HIP_OK;
+    DeviceScope scope(ctx->device);
+    if (scope.status() != hipSuccess) return hip_fail(scope.status(), "hipSetDevice");
+    for (uint32_t r = 0; r < m; r += kKv8AppendRows) {
+        const uint32_t rows = std::min(m - r, kKv8AppendRows);
+        const hipError_t err =
+            launch_kv8_append(kv8_geometry_of(kv), qkv + static_cast<uint64_t>(r) * row_stride, row_stride, q_width, rows,
+                              positions + r, page_tables + static_cast<uint64_t>(r) * kv->max_pages, layer, ctx->stream);
+        if (err != hipSuccess) return hip_fail(err, "kv8_append_kernel");
+    }
+    return AIR_HIP_OK;
+}
+
+int air_hip_kv8_read(air_hip_context* ctx, const air_hip_kv8_layout* kv, uint32_t sequences, const int32_t* starts,
+                     const int32_t* lengths, const int32_t* page_tables, uint32_t layer, uint32_t layers,
+                     uint64_t max_tokens, float* k, float* v, float* weights) {
+    if (!ctx || !lengths || !page_tables) return fail(AIR_HIP_INVALID_ARGUMENT, "arguments must not be null");
+    forget_loaded_source(ctx);
+    if (int rc = check_kv8(kv); rc != AIR_HIP_OK) return rc;
+    if (int rc = check_kv8_layers(kv, layer, layers); rc != AIR_HIP_OK) return rc;
+    if (int rc = check_kv8_tokens(kv, max_tokens); rc != AIR_HIP_OK) return rc;
+    if (sequences == 0 || (!k && !v && !weights)) return AIR_HIP_OK;
+    if (static_cast<uint64_t>(sequences) * layers > 65535u) {
+        return fail(AIR_HIP_UNSUPPORTED, "at most 65535 (sequence, layer) pairs per call");
+    }
+    DeviceScope scope(ctx->device);
+    if (scope.status() != hipSuccess) return hip_fail(scope.status(), "hipSetDevice");
+    const hipError_t err = launch_kv8_read(kv8_geometry_of(kv), sequences, starts, lengths, page_tables, layer, layers,
+                                           max_tokens, k, v, weights, ctx->stream);
+    return err == hipSuccess ? AIR_HIP_OK : hip_fail(err, "kv8_read_kernel");
+}
+
+int air_hip_kv8_attention(air_hip_context* ctx, const air_hip_kv8_layout* kv, const float* qkv, uint64_t row_stride,
+                          uint32_t m, const int32_t* positions, const int32_t* page_tables, uint32_t layer,
+                          uint32_t q_heads, const int32_t* run_starts, uint32_t runs, uint64_t max_tokens, int weights,
+                          float* out) {
+    if (!ctx || !qkv || !positions || !page_tables || !out) {
+        return fail(AIR_HIP_INVALID_ARGUMENT, "arguments must not be null");
+    }
+    forget_loaded_source(ctx);
+    if (int rc = check_kv8(kv); rc != AIR_HIP_OK) return rc;
+    if (layer >= kv->layers) return fail(AIR_HIP_INVALID_ARGUMENT, "layer %u is out of range", layer);
+    if (q_heads == 0 || q_heads % kv->kv_heads != 0) {
+        return fail(AIR_HIP_INVALID_ARGUMENT, "q heads must be a non-zero multiple of the KV heads");
+    }
+    if (int rc = check_kv8_tokens(kv, max_tokens); rc != AIR_HIP_OK) return rc;
+    if (weights != AIR_HIP_KV8_WEIGHTS_NONE && weights != AIR_HIP_KV8_WEIGHTS_ADD && weights != AIR_HIP_KV8_WEIGHTS_SET) {
+        return fail(AIR_HIP_INVALID_ARGUMENT, "weights must be NONE, ADD or SET, not %d", weights);
+    }
+    if (!run_starts && runs != 0) return fail(AIR_HIP_INVALID_ARGUMENT, "%u runs need run_starts", runs);
+    if (row_stride < static_cast<uint64_t>(q_heads) * kv->head_dim || row_stride % 4u != 0 ||
+        reinterpret_cast<std::uintptr_t>(qkv) % 16u != 0 || reinterpret_cast<std::uintptr_t>(out) % 16u != 0) {
+        return fail(AIR_HIP_INVALID_ARGUMENT, "q|k|v rows and output must be 16-byte aligned, stride >= the q heads");
+    }
+    if (m == 0) return AIR_HIP_OK;
+    if (m > 65535u || q_heads > 65535u || runs > 65535u) {
+        return fail(AIR_HIP_UNSUPPORTED, "at most 65535 rows, runs and q heads per call");
+    }
+    DeviceScope scope(ctx->device);
+    if (scope.status() != hipSuccess) return hip_fail(scope.status(), "hipSetDevice");
+    const Kv8Shape shape = kv8_attention_shape(m, q_heads, kv->kv_heads, max_tokens);
+    if (int rc = ensure_attention_scratch(ctx, kv8_attention_scratch(shape, m, q_heads, kv->head_dim, weights != 0));
+        rc != AIR_HIP_OK) {
+        return rc;
+    }
+    const hipError_t err =
+        launch_kv8_attention(kv8_geometry_of(kv), qkv, row_stride, m, positions, page_tables, layer, q_heads, run_starts,
+                             run_starts ? runs : m, max_tokens, weights, shape, ctx->attention_scratch, out, ctx->stream);
+    return err == hipSuccess ? AIR_HIP_OK : hip_fail(err, "kv8_attention_kernel");
+}
+
+int air_hip_kv8_evict(air_hip_context* ctx, const air_hip_kv8_layout* kv, uint32_t sequences, const int32_t* lengths,
+                      const int32_t* page_tables, const int32_t* new_page_tables, uint32_t layer, uint32_t layers,
+                      uint32_t keep_first, uint32_t keep_last, uint32_t budget, uint64_t max_tokens, int32_t* kept) {
+    if (!ctx || !lengths || !page_tables || !new_page_tables || !kept) {
+        return fail(AIR_HIP_INVALID_ARGUMENT, "arguments must not be null");
+    }
+    forget_loaded_source(ctx);
+    if (int rc = check_kv8(kv); rc != AIR_HIP_OK) return rc;
+    if (int rc = check_kv8_layers(kv, layer, layers); rc != AIR_HIP_OK) return rc;
+    if (int rc = check_kv8_tokens(kv, max_tokens); rc != AIR_HIP_OK) return rc;
+    if (budget == 0 || budget > static_cast<uint32_t>(INT32_MAX) ||
+        static_cast<uint64_t>(keep_first) + keep_last > budget) {
+        return fail(AIR_HIP_INVALID_ARGUMENT, "the budget must be positive and hold keep_first + keep_last tokens");
+    }
+    if (sequences == 0) return AIR_HIP_OK;
+    if (sequences > 65535u || static_cast<uint64_t>(kv->kv_heads) * layers > 65535u) {
+        return fail(AIR_HIP_UNSUPPORTED, "at most 65535 sequences and (layer, KV head) pairs per call");
+    }
+    DeviceScope scope(ctx->device);
+    if (scope.status() != hipSuccess) return hip_fail(scope.status(), "hipSetDevice");
+    const hipError_t err = launch_kv8_evict(kv8_geometry_of(kv), sequences, lengths, page_tables, new_page_tables, layer,
+                                            layers, keep_first, keep_last, budget, max_tokens, kept, ctx->stream);
+    return err == hipSuccess ? AIR_HIP_OK : hip_fail(err, "kv8_evict kernels");
+}
+
+} // extern "C"

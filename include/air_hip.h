@@ -596,6 +596,130 @@ int air_hip_attention_online(air_hip_context* ctx, const air_hip_kv_layout* kv, 
                              const air_hip_attention_tile* tiles, uint32_t tile_count, uint64_t max_tokens,
                              float* out);
 
+/* ---- the 8-bit KV cache ----------------------------------------------------- */
+/* A paged KV cache of 8-bit codes with one f32 scale for the K and one for the
+ * V of each block of 16 tokens, layer and KV head: a quarter of the fp32
+ * pool's bytes (1.03 per element at head width 128), so four times the
+ * tokens and a quarter of a decode step's reads.  Besides the codes a block
+ * keeps the attention weight that its tokens gathered, by which a sequence
+ * that outgrew its budget is shortened.  No counterpart in the reference,
+ * whose cache is fp32 (src/cuda/cuda_backend.cu:1186-1300).
+ *
+ * Positions are slots of the cache.  They are a sequence's token positions
+ * until it is shortened by air_hip_kv8_evict; from then on its next slot is
+ * its new length, while RoPE (air_hip_rope, before the append) goes on with
+ * the token position.
+ *
+ * Values: scale = A / qmax in f32 for values of largest magnitude A (qmax 127
+ * or 448), code = the nearest to the f32 quotient x / scale (ties to even),
+ * value = code * scale.  A non-finite value makes its block's scale NaN: the
+ * block reads as NaN, and so does what attends to it, until it is begun anew
+ * at its first slot. */
+enum {
+    AIR_HIP_KV8_I8 = 1,      /* codes -127..127 */
+    AIR_HIP_KV8_E4M3 = 2     /* OCP e4m3: 4 exponent, 3 mantissa bits, +-448 */
+};
+#define AIR_HIP_KV8_BLOCK_TOKENS 16u
+
+/* Page p holds [layer][KV head][page_tokens / 16] records of 128 + 32 *
+ * head_dim bytes: f32 scale of K, f32 scale of V, 56 unused bytes, 16 f32
+ * weights, K codes [token / 4][dim / 16][token % 4][dim % 16], V codes
+ * [dim][token]; i8 codes are stored as code + 128.  The pool is one
+ * allocation or a chunk table, as in air_hip_kv_layout; it and the chunks are
+ * 16-byte aligned (128 keeps a record's lines its own).  Entries of a page
+ * table outside [0, pool_pages), and pages of unallocated chunks, hold no
+ * tokens. */
+typedef struct air_hip_kv8_layout {
+    void* pool;
+    uint32_t page_tokens;    /* a multiple of 16 */
+    uint32_t kv_heads;
+    uint32_t head_dim;       /* 64 or 128 */
+    uint32_t layers;
+    uint32_t max_pages;      /* entries of a page-table row */
+    uint32_t pool_pages;
+    void* const* chunks;     /* device chunk table, or null for a single pool */
+    uint32_t chunk_shift;    /* log2 of the pages per chunk (<= 30) */
+    int32_t type;            /* AIR_HIP_KV8_* */
+} air_hip_kv8_layout;
+
+/* Bytes of a page of this layout (its pool, chunks and page counts are not
+ * looked at beyond being valid numbers); 0 if the layout is not valid. */
+uint64_t air_hip_kv8_page_bytes(const air_hip_kv8_layout* kv);
+
+/* Quantises each row's k and v (the q|k|v row after RoPE, as
+ * air_hip_kv_append takes it) into the slot positions[r] of its sequence.
+ * Per block that rows of the call name: a block whose lowest such slot is its
+ * first is begun anew, with the scale of the new values; otherwise the slots
+ * below are held, the scale is the larger of the held and the new one, and if
+ * it grows the held codes are rounded again under it (code * (old / new), f32).
+ * Slots behind the new ones hold nothing afterwards.  New tokens have weight 0.
+ * Rows may come in any order and from any sequences; of rows that name one
+ * slot the last is stored.  Rows with a negative position or without a page
+ * are skipped.  More than 2048 rows are stored as successive calls of 2048. */
+int air_hip_kv8_append(air_hip_context* ctx, const air_hip_kv8_layout* kv, const float* qkv, uint64_t row_stride,
+                       uint64_t q_width, uint32_t m, const int32_t* positions, const int32_t* page_tables,
+                       uint32_t layer);
+
+/* Tokens starts[i] .. starts[i] + lengths[i] - 1 (starts null: from 0; at
+ * most max_tokens) of `sequences` sequences (page_tables: int32
+ * [sequences][max_pages]) in layers [layer, layer + layers) as f32 values:
+ *   k, v     [layers][sequences][max_tokens][kv_heads * head_dim]
+ *   weights  [layers][sequences][max_tokens][kv_heads]
+ * any of them null.  What lies behind a sequence's tokens, and tokens without
+ * a page, are left as they were. */
+int air_hip_kv8_read(air_hip_context* ctx, const air_hip_kv8_layout* kv, uint32_t sequences, const int32_t* starts,
+                     const int32_t* lengths, const int32_t* page_tables, uint32_t layer, uint32_t layers,
+                     uint64_t max_tokens, float* k, float* v, float* weights);
+
+/* Attention of every row's q heads over slots 0..positions[r] of its sequence
+ * (below max_tokens, which bounds the work and sizes the context's scratch):
+ * out [m][q_heads * head_dim], f32 accurate over the stored values (both
+ * products carry their f32 operand as two f16 parts, sums in f32).  Tokens
+ * without a page take no part; a row that attends to nothing (a negative
+ * position) gets zeros.
+ *   run_starts  int32 [runs + 1], device, ascending: run i is rows
+ *               run_starts[i] .. run_starts[i + 1] - 1, all of one sequence
+ *               (their page tables name the same pages up to the run's last
+ *               position); every row of the call lies in a run.  Null with
+ *               runs 0: every row is a run of its own.  Rows of a run share
+ *               what they read.
+ *   weights     what the rows' probabilities do to the weights of the tokens
+ *               they attend to: AIR_HIP_KV8_WEIGHTS_NONE nothing; _ADD adds
+ *               sum over the run's rows and the KV head's q heads of p to
+ *               the weight of every slot 0..the run's last position; _SET
+ *               stores that sum.  Deterministic where no page belongs to two
+ *               runs of the call.
+ * q|k|v rows and out 16-byte aligned, row_stride a multiple of 4. */
+enum {
+    AIR_HIP_KV8_WEIGHTS_NONE = 0,
+    AIR_HIP_KV8_WEIGHTS_ADD = 1,
+    AIR_HIP_KV8_WEIGHTS_SET = 2
+};
+int air_hip_kv8_attention(air_hip_context* ctx, const air_hip_kv8_layout* kv, const float* qkv, uint64_t row_stride,
+                          uint32_t m, const int32_t* positions, const int32_t* page_tables, uint32_t layer,
+                          uint32_t q_heads, const int32_t* run_starts, uint32_t runs, uint64_t max_tokens, int weights,
+                          float* out);
+
+/* Shortens every sequence longer than `budget` (lengths[i], counted up to
+ * max_tokens) to `budget` tokens, for each layer of [layer, layer + layers)
+ * and KV head on its own: the first keep_first, the last keep_last, and of
+ * those between the ones of largest weight (equal weights: the lowest slots;
+ * NaN ranks lowest), in their order, in slots 0..budget - 1 of the pages of
+ * new_page_tables, with their weights.  Shorter sequences keep every token.
+ * The caller's new length is min(lengths[i], budget).  A new block's scale is
+ * the largest of its tokens' scales; codes are rounded again where it differs
+ * (code * (old / new), f32).
+ *   new_page_tables  int32 [sequences][max_pages]: either page_tables itself
+ *                    (the same pointer), which shortens in place, or tables
+ *                    whose pages no page_tables of the call names; pages of
+ *                    the budget's tokens must be there.
+ *   kept             int32 [sequences][layers][kv_heads][budget], written:
+ *                    the slots kept, ascending, then -1.
+ * A page that another sequence names too must not be shortened in place. */
+int air_hip_kv8_evict(air_hip_context* ctx, const air_hip_kv8_layout* kv, uint32_t sequences, const int32_t* lengths,
+                      const int32_t* page_tables, const int32_t* new_page_tables, uint32_t layer, uint32_t layers,
+                      uint32_t keep_first, uint32_t keep_last, uint32_t budget, uint64_t max_tokens, int32_t* kept);
+
 /* out[r][i] = silu(gate_up[r][i]) * gate_up[r][ffn + i] over fused gate|up
  * rows (reference_executor.cpp:33-35, 400). */
 int air_hip_silu_mul(air_hip_context* ctx, const float* gate_up, float* out, uint32_t m, uint64_t ffn);
