@@ -69,16 +69,23 @@ __device__ __forceinline__ void codes_to_half(const u32x4& c, half8v& a, half8v&
     }
 }
 
-// x = hi + lo to 22 bits.
+// x = hi + lo to 22 bits.  The empty asm makes x one f32 value: a product
+// passed in could otherwise be rounded straight to f16 for hi and by way of
+// f32 for lo, and the two hi differ next to a tie (seen as single weights off
+// by 2^-11).
 __device__ __forceinline__ void split_f16(float x, _Float16& hi, _Float16& lo) {
+    asm("" : "+v"(x));
     hi = static_cast<_Float16>(x);
     lo = static_cast<_Float16>(x - static_cast<float>(hi));
 }
 
 // The B operands of the products with K of one query vector (lane % 16), and
-// the factor that undoes their power-of-two scale: the vector's largest
-// magnitude lies in [2^8, 2^9), so that hi and lo are normal f16 down to
-// 2^-31 of it.
+// the factor that undoes their power-of-two scale.  An MFMA adds its 32
+// products in a window of 24 bits below the largest and drops what lies under
+// it (the sum then meets the accumulator with one rounding), so hi is whole:
+// with the vector's largest magnitude in [2^10, 2^11), hi times a code is a
+// multiple of the code's last place and 32 of them fit the window.  lo is the
+// f16 nearest to the rest, to 2^-24 of the largest magnitude.
 template <unsigned D>
 struct QueryFragments {
     half8v hi[D / 32], lo[D / 32];
@@ -107,16 +114,15 @@ __device__ __forceinline__ void load_query(const float* q, unsigned grp, QueryFr
     top = fmaxf(top, __shfl_xor(top, 32));
     int e = static_cast<int>(__float_as_uint(top) >> 23) - 127;   // -127: zero or subnormal; 128: not finite
     e = e < -110 ? -110 : e > 120 ? 120 : e;
-    const float scale = __uint_as_float(static_cast<std::uint32_t>(127 + 8 - e) << 23);
-    f.undo = __uint_as_float(static_cast<std::uint32_t>(127 - 8 + e) << 23);
+    const float scale = __uint_as_float(static_cast<std::uint32_t>(127 + 10 - e) << 23);
+    f.undo = __uint_as_float(static_cast<std::uint32_t>(127 - 10 + e) << 23);
 #pragma unroll
     for (unsigned i = 0; i < D / 32u; ++i) {
 #pragma unroll
         for (unsigned j = 0; j < 8u; ++j) {
-            _Float16 hi, lo;
-            split_f16(x[8u * i + j] * scale, hi, lo);
-            f.hi[i][j] = hi;
-            f.lo[i][j] = lo;
+            const float y = x[8u * i + j] * scale, whole = rintf(y);
+            f.hi[i][j] = static_cast<_Float16>(whole);
+            f.lo[i][j] = static_cast<_Float16>(y - whole);
         }
     }
 }
@@ -139,21 +145,39 @@ __device__ __forceinline__ void load_keys(const unsigned char* rec, unsigned lan
     }
 }
 
+// c = a b to twice the precision: what a block's scores are multiplied by (to
+// one f32 a block's scores would all be off by up to 2^-24 of themselves).
+struct Factor {
+    float hi, lo;
+};
+__device__ __forceinline__ Factor score_factor(float undo, float2 score_scale, float k_scale) {
+    const float a = undo * score_scale.x;          // undo is a power of two
+    const float hi = a * k_scale;
+    return Factor{hi, __builtin_fmaf(undo * score_scale.y, k_scale, __builtin_fmaf(a, k_scale, -hi))};
+}
+// 2^(score * factor - base)
+__device__ __forceinline__ float score_power(float score, const Factor& f, float base) {
+    return __builtin_amdgcn_exp2f(__builtin_fmaf(score, f.hi, __builtin_fmaf(score, f.lo, -base)));
+}
+
 // S^T of the chunk: score[b][r] is token 4 b + r of this lane's block for
 // vector lane % 16, times the fragments' scale.
 template <int TYPE, unsigned D>
 __device__ __forceinline__ void chunk_scores(const KeyCodes<D>& k, const QueryFragments<D>& q, float4v score[4]) {
 #pragma unroll
     for (unsigned b = 0; b < 4u; ++b) {
+        half8v a[D / 32];
+#pragma unroll
+        for (unsigned s = 0; s < D / 64u; ++s) codes_to_half<TYPE>(k.c[b][s], a[2u * s], a[2u * s + 1u]);
+        // The low parts first: their roundings are those of a small sum.
         score[b] = float4v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (unsigned s = 0; s < D / 64u; ++s) {
-            half8v a0, a1;
-            codes_to_half<TYPE>(k.c[b][s], a0, a1);
-            score[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, q.hi[2u * s], score[b], 0, 0, 0);
-            score[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, q.lo[2u * s], score[b], 0, 0, 0);
-            score[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, q.hi[2u * s + 1u], score[b], 0, 0, 0);
-            score[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, q.lo[2u * s + 1u], score[b], 0, 0, 0);
+        for (unsigned i = 0; i < D / 32u; ++i) {
+            score[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i], q.lo[i], score[b], 0, 0, 0);
+        }
+#pragma unroll
+        for (unsigned i = 0; i < D / 32u; ++i) {
+            score[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i], q.hi[i], score[b], 0, 0, 0);
         }
     }
 }
@@ -164,7 +188,7 @@ template <int TYPE, unsigned D>
 __global__ __launch_bounds__(kThreads) void kv8_attention_kernel(
     Kv8Geometry g, const float* __restrict__ qkv, std::uint64_t stride, const std::int32_t* __restrict__ positions,
     const std::int32_t* __restrict__ tables, std::uint32_t layer, std::uint32_t q_heads, std::uint64_t max_tokens,
-    std::uint32_t split_chunks, float score_scale, float* __restrict__ partials, float2* __restrict__ stats,
+    std::uint32_t split_chunks, float2 score_scale, float* __restrict__ partials, float2* __restrict__ stats,
     float* __restrict__ out) {
     constexpr unsigned LD = D + 4;
     __shared__ float sums[kWaves][kVectors][LD];
@@ -188,7 +212,6 @@ __global__ __launch_bounds__(kThreads) void kv8_attention_kernel(
     load_query<D>(col < nq ? qkv + static_cast<std::uint64_t>(row) * stride + static_cast<std::uint64_t>(head0 + col) * D
                            : nullptr,
                   grp, q);
-    const float lane_scale = q.undo * score_scale;
 
     int m = kNone, m2 = kNone;
     float l = 0.0f;
@@ -214,15 +237,13 @@ __global__ __launch_bounds__(kThreads) void kv8_attention_kernel(
         // Tokens of this lane's block that the row attends to.
         const std::int64_t first = (static_cast<std::int64_t>(c) * kChunkBlocks + grp) * kKv8Block;
         const int limit = vrec0 == nullptr || last < first ? -1 : last - first > 15 ? 15 : static_cast<int>(last - first);
-        const float factor = lane_scale * scales.x;
+        const Factor factor = score_factor(q.undo, score_scale, scales.x);
         float top = -__builtin_huge_valf();
 #pragma unroll
         for (unsigned b = 0; b < 4u; ++b) {
 #pragma unroll
             for (unsigned r = 0; r < 4u; ++r) {
-                const float x = s[b][r] * factor;
-                s[b][r] = static_cast<int>(4u * b + r) <= limit ? x : -__builtin_huge_valf();
-                top = fmaxf(top, s[b][r]);
+                if (static_cast<int>(4u * b + r) <= limit) top = fmaxf(top, s[b][r] * factor.hi);
             }
         }
         // References: the block's own, then the vector's over the four blocks.
@@ -237,13 +258,14 @@ __global__ __launch_bounds__(kThreads) void kv8_attention_kernel(
             m_new = a > m_new ? a : m_new;
             m2_new = a2 > m2_new ? a2 : m2_new;
         }
-        // p' = 2^(s - base) * share, at most 2^kPBits; a scale of V far below
+        // p' = 2^(s - base) * share, below 2^kPBits; a scale of V far below
         // the others' (or zero) keeps base near M, so the same powers also
-        // sum up the denominator.
-        int e = m2_new - kPBits - m_new - 40;
+        // sum up the denominator.  s - base is small where p is large, and
+        // rounded once.
+        int e = m2_new - m_new - 40;
         e = scales.y == 0.0f || exponent < e ? e : exponent;
-        const int base = m2_new - e - kPBits;
-        const float share = __builtin_amdgcn_ldexpf(scales.y, -e);
+        const int base = m2_new - e;
+        const float share = __builtin_amdgcn_ldexpf(scales.y, kPBits - e);
         const float fbase = static_cast<float>(base);
         float sum = 0.0f;
         half8v p_hi[2], p_lo[2];
@@ -251,7 +273,8 @@ __global__ __launch_bounds__(kThreads) void kv8_attention_kernel(
         for (unsigned b = 0; b < 4u; ++b) {
 #pragma unroll
             for (unsigned r = 0; r < 4u; ++r) {
-                const float x = __builtin_amdgcn_exp2f(s[b][r] - fbase);
+                float x = score_power(s[b][r], factor, fbase);
+                x = static_cast<int>(4u * b + r) <= limit ? x : 0.0f;
                 sum += x;
                 _Float16 hi, lo;
                 split_f16(x * share, hi, lo);
@@ -394,7 +417,7 @@ template <int TYPE, unsigned D>
 __global__ __launch_bounds__(kThreads) void kv8_weights_kernel(
     Kv8Geometry g, const float* __restrict__ qkv, std::uint64_t stride, std::uint32_t m,
     const std::int32_t* __restrict__ positions, const std::int32_t* __restrict__ tables, std::uint32_t layer,
-    std::uint32_t q_heads, const std::int32_t* __restrict__ run_starts, std::uint64_t max_tokens, float score_scale,
+    std::uint32_t q_heads, const std::int32_t* __restrict__ run_starts, std::uint64_t max_tokens, float2 score_scale,
     const float2* __restrict__ stats, bool add) {
     const unsigned tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, grp = lane >> 4, col = lane & 15u;
     const std::uint32_t kvh = blockIdx.y, run = blockIdx.z;
@@ -440,13 +463,13 @@ __global__ __launch_bounds__(kThreads) void kv8_weights_kernel(
         const float2 st = active ? stats[static_cast<std::uint64_t>(r) * q_heads + head] : make_float2(0.f, 0.f);
         float4v s[4];
         chunk_scores<TYPE, D>(keys, q, s);
-        const float factor = q.undo * score_scale * k_scale;
+        const Factor factor = score_factor(q.undo, score_scale, k_scale);
         const int limit = vrec0 == nullptr || upto < first ? -1 : upto - first > 15 ? 15 : static_cast<int>(upto - first);
 #pragma unroll
         for (unsigned b = 0; b < 4u; ++b) {
 #pragma unroll
             for (unsigned i = 0; i < 4u; ++i) {
-                const float p = __builtin_amdgcn_exp2f(s[b][i] * factor - st.x) * st.y;
+                const float p = score_power(s[b][i], factor, st.x) * st.y;
                 sum[b][i] += static_cast<int>(4u * b + i) <= limit ? p : 0.0f;
             }
         }
@@ -506,7 +529,8 @@ hipError_t launch_kv8_attention(const Kv8Geometry& g, const float* qkv, std::uin
     float* const partials = reinterpret_cast<float*>(
         static_cast<unsigned char*>(scratch) + (weights ? (vectors * sizeof(float2) + 255u) / 256u * 256u : 0u));
     // Scores in powers of two: s log2(e) = (q . k) * log2(e) / sqrt(D).
-    const float scale = static_cast<float>(1.4426950408889634 / __builtin_sqrt(static_cast<double>(g.head_dim)));
+    const double exact = 1.4426950408889634 / __builtin_sqrt(static_cast<double>(g.head_dim));
+    const float2 scale = make_float2(static_cast<float>(exact), static_cast<float>(exact - static_cast<float>(exact)));
     const dim3 grid(shape.tiles, shape.tile_heads, shape.splits);
     const std::uint64_t chunks = (max_tokens + kChunkTokens - 1u) / kChunkTokens;
     const dim3 weight_grid(static_cast<unsigned>((chunks + kWaves - 1u) / kWaves), g.kv_heads, runs);

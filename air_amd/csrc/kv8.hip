@@ -2,8 +2,8 @@
 //
 // A block (16 tokens of one layer and KV head) holds its K and its V codes
 // under one f32 scale each; a value is code * scale.  The scale of values
-// with largest magnitude A is A / qmax (127 for i8, 448 for e4m3) in f32, a
-// code the nearest to x / scale (f32 quotient, ties to even).  A block that
+// with largest magnitude A is A times the f32 nearest to 1 / qmax (127 for i8,
+// 448 for e4m3), a code the nearest to x / scale (f32 quotient, ties to even).  A block that
 // takes a non-finite value gets a NaN scale and reads as NaN until it is
 // begun anew, so a broken model shows in its logits as it does over the f32
 // pool instead of turning into large finite keys.
@@ -14,7 +14,7 @@
 namespace air_hip {
 namespace {
 
-__device__ __forceinline__ float kv8_qmax(int type) { return type == kKv8I8 ? 127.0f : 448.0f; }
+__device__ __forceinline__ constexpr float kv8_unit(int type) { return type == kKv8I8 ? 1.0f / 127.0f : 1.0f / 448.0f; }
 
 // Code of x in a block of scale s: zero where the scale holds nothing (zero:
 // all values are zero; NaN: the block is poisoned).
@@ -108,7 +108,7 @@ __global__ __launch_bounds__(2 * D) void kv8_append_kernel(Kv8Geometry g, const 
         const std::uint32_t t = wave_top[(value ? D / 64u : 0u) + w];
         top = t > top ? t : top;
     }
-    const float need = top >= 0x7f800000u ? nan_f32() : __uint_as_float(top) / kv8_qmax(TYPE);
+    const float need = top >= 0x7f800000u ? nan_f32() : __uint_as_float(top) * kv8_unit(TYPE);
     const bool held = first > 0u;
     // !(need <= old): a NaN need replaces the scale, a NaN scale stays.
     const bool grows = held && old_scale == old_scale && !(need <= old_scale);

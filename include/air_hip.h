@@ -610,8 +610,8 @@ int air_hip_attention_online(air_hip_context* ctx, const air_hip_kv_layout* kv, 
  * its new length, while RoPE (air_hip_rope, before the append) goes on with
  * the token position.
  *
- * Values: scale = A / qmax in f32 for values of largest magnitude A (qmax 127
- * or 448), code = the nearest to the f32 quotient x / scale (ties to even),
+ * Values: scale = A * (1 / qmax) in f32 for values of largest magnitude A
+ * (qmax 127 or 448, 1 / qmax rounded to f32), code = the nearest to the f32 quotient x / scale (ties to even),
  * value = code * scale.  A non-finite value makes its block's scale NaN: the
  * block reads as NaN, and so does what attends to it, until it is begun anew
  * at its first slot. */

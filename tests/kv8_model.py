@@ -12,7 +12,7 @@ import numpy as np
 
 from air_amd import capi
 
-QMAX = {capi.KV8_I8: 127.0, capi.KV8_E4M3: 448.0}
+UNIT = {capi.KV8_I8: np.float32(1) / np.float32(127), capi.KV8_E4M3: np.float32(1) / np.float32(448)}
 BLOCK = 16
 
 
@@ -110,7 +110,7 @@ class Cache:
                     lo = q_width + which * width + head * self.d
                     x = {t: qkv[r, lo:lo + self.d].astype(np.float32) for t, r in rows.items()}
                     top = np.float32(max(np.abs(v).max() if np.isfinite(v).all() else math.inf for v in x.values()))
-                    need = top / np.float32(QMAX[self.kind]) if np.isfinite(top) else np.float32(math.nan)
+                    need = top * UNIT[self.kind] if np.isfinite(top) else np.float32(math.nan)
                     old = f[which].copy()
                     scale = need
                     if first > 0:

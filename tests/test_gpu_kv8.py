@@ -417,6 +417,61 @@ def test_attention_over_a_long_cache(torch_cuda, hip_ctx, kind):
 
 @pytest.mark.gpu
 @KINDS
+def test_attention_errors_are_those_of_f32(torch_cuda, hip_ctx, kind):
+    """Over 448 vectors and 3500 tokens the errors against float64 are, in the
+    root mean square, at most 16 half steps of f32 (2^-24 each): a score of up
+    to 30 is right to about 2^-24 of itself, which e^s turns into a relative
+    error of some half steps of p, and the sums add one or two more.  A single
+    weight in a thousand held to one f16 (2^-12) would be above it."""
+    torch = torch_cuda
+    gen = torch.Generator(device="cuda:0")
+    gen.manual_seed(61 + kind)
+    q_heads, kvh, d, n, m = 28, 4, 128, 3500, 16
+    cache = Cache(kind, kvh, d, 1, 16, 224, 224)
+    dev = Device(torch, hip_ctx, cache)
+    table = torch.randperm(224, device="cuda:0", generator=gen).to(torch.int32).repeat(2048, 1)
+    width = 2 * kvh * d
+    for a in range(0, n, 2048):
+        b = min(n, a + 2048)
+        x = torch.randn((b - a, width), device="cuda:0", generator=gen)
+        pos = torch.arange(a, b, dtype=torch.int32, device="cuda:0")
+        capi.check(dev.lib.air_hip_kv8_append(hip_ctx.handle, ctypes.byref(dev.kv), x.data_ptr(), width, 0, b - a,
+                                              pos.data_ptr(), table.data_ptr(), 0))
+    k, v, _ = dev.read(None, [n], table[:1].cpu().numpy(), 0, 1, n, 0.0)
+    cache.pool[...] = dev.pool()
+    x = torch.randn((m, q_heads * d), device="cuda:0", generator=gen)
+    x *= torch.exp(0.6 * torch.randn((m, 1), device="cuda:0", generator=gen))
+    x = x.cpu().numpy()
+    pos = [n - 1 - 7 * r for r in range(m)]
+    tab = table[:m].cpu().numpy()
+    got = dev.attention(x, pos, tab, 0, q_heads, n).reshape(m, kvh, -1, d)
+    got_run = dev.attention(x, pos, tab, 0, q_heads, n, [(0, m)]).reshape(m, kvh, -1, d)
+    # Values from codes and scales in 64 bits: read() has rounded their product.
+    t = np.arange(n)
+    page = tab[0, t // 16]
+    f = Cache.floats(cache.pool)[page, 0, :, 0]                      # [tokens][kv heads][floats]
+    rec = cache.pool[page, 0, :, 0]
+    at_k = np.stack([cache.k_at(i) for i in range(16)])[t % 16][:, None]
+    at_v = np.stack([cache.v_at(i) for i in range(16)])[t % 16][:, None]
+    k64 = kv8_model.value(np.take_along_axis(rec, at_k, 2), kind) * f[..., 0:1].astype(np.float64)
+    v64 = kv8_model.value(np.take_along_axis(rec, at_v, 2), kind) * f[..., 1:2].astype(np.float64)
+    assert np.abs(k64.reshape(1, 1, n, -1) - k).max() <= 2.0 ** -24 * np.abs(k64).max()
+    assert np.abs(v64.reshape(1, 1, n, -1) - v).max() <= 2.0 ** -24 * np.abs(v64).max()
+    q = x.astype(np.float64).reshape(m, kvh, -1, d)
+    want = np.empty(got.shape)
+    for g in range(kvh):
+        s = np.einsum("mhd,td->mht", q[:, g], k64[:, g]) / np.sqrt(d)
+        s = np.where(np.arange(n)[None, None, :] > np.array(pos)[:, None, None], -np.inf, s)
+        p = np.exp(s - s.max(axis=-1, keepdims=True))
+        want[:, g] = np.einsum("mht,td->mhd", p / p.sum(axis=-1, keepdims=True), v64[:, g])
+    for side in (got, got_run):
+        err = np.linalg.norm(side - want) / np.linalg.norm(want)
+        print("rms error in half steps of f32", err * 2 ** 24, flush=True)
+        assert err <= 16 * 2.0 ** -24
+
+
+@pytest.mark.gpu
+@KINDS
 def test_agrees_with_the_online_attention_over_read_values(torch_cuda, hip_ctx, kind):
     """The values read into an fp32 pool and attended to by
     air_hip_attention_online give the same rows."""
