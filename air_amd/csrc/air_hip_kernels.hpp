@@ -421,12 +421,14 @@ hipError_t launch_kv8_evict(const Kv8Geometry& g, std::uint32_t seqs, const std:
 // How a call's attention is cut: `splits` workgroups of split_chunks 64-token
 // chunks over a tile's keys.
 struct Kv8Shape {
-    std::uint32_t tiles;          // grid x
-    std::uint32_t tile_heads;     // grid y
+    std::uint32_t tiles;          // grid y
+    std::uint32_t tile_heads;     // grid x
     std::uint32_t splits;         // grid z
     std::uint32_t split_chunks;
+    std::uint32_t tile_rows;      // rows of one run a tile holds; 0: a tile is a row
 };
-Kv8Shape kv8_attention_shape(std::uint32_t m, std::uint32_t q_heads, std::uint32_t kv_heads, std::uint64_t max_tokens);
+Kv8Shape kv8_attention_shape(std::uint32_t m, std::uint32_t q_heads, std::uint32_t kv_heads, std::uint32_t runs,
+                             std::uint64_t max_tokens);
 // Bytes of scratch: the splits' partials and, with weights, the rows' softmax
 // statistics.
 std::uint64_t kv8_attention_scratch(const Kv8Shape& shape, std::uint32_t m, std::uint32_t q_heads,

@@ -37,7 +37,8 @@ namespace {
 
 constexpr unsigned kWaves = 4;
 constexpr unsigned kThreads = 64 * kWaves;
-constexpr unsigned kVectors = 16;          // query vectors of a tile
+constexpr unsigned kVectors = 16;          // query vectors of an MFMA tile
+constexpr unsigned kPromptTiles = 2;       // MFMA tiles of a workgroup where runs have several rows
 constexpr unsigned kChunkBlocks = 4;       // blocks of a chunk, one per lane group
 constexpr unsigned kChunkTokens = kChunkBlocks * kKv8Block;
 constexpr int kNone = -(1 << 30);          // a reference that no score has set
@@ -69,14 +70,17 @@ __device__ __forceinline__ void codes_to_half(const u32x4& c, half8v& a, half8v&
     }
 }
 
-// x = hi + lo to 22 bits.  The empty asm makes x one f32 value: a product
-// passed in could otherwise be rounded straight to f16 for hi and by way of
-// f32 for lo, and the two hi differ next to a tie (seen as single weights off
-// by 2^-11).
-__device__ __forceinline__ void split_f16(float x, _Float16& hi, _Float16& lo) {
-    asm("" : "+v"(x));
-    hi = static_cast<_Float16>(x);
-    lo = static_cast<_Float16>(x - static_cast<float>(hi));
+// x share = hi + lo to 22 bits, for two x.  hi passes an empty asm so that
+// both halves go by one rounding of it: left to itself the compiler may round
+// the product straight to f16 in one place and by way of f32 in the other,
+// and next to a tie these differ (seen as single weights off by 2^-11).
+__device__ __forceinline__ void split_products(float x0, float x1, float share, half2v& hi, half2v& lo) {
+    typedef float float2v __attribute__((ext_vector_type(2)));
+    std::uint32_t bits = __builtin_bit_cast(std::uint32_t, __builtin_convertvector(float2v{x0 * share, x1 * share}, half2v));
+    asm("" : "+v"(bits));
+    hi = __builtin_bit_cast(half2v, bits);
+    lo[0] = static_cast<_Float16>(__builtin_fmaf(x0, share, -static_cast<float>(hi[0])));
+    lo[1] = static_cast<_Float16>(__builtin_fmaf(x1, share, -static_cast<float>(hi[1])));
 }
 
 // The B operands of the products with K of one query vector (lane % 16), and
@@ -182,42 +186,145 @@ __device__ __forceinline__ void chunk_scores(const KeyCodes<D>& k, const QueryFr
     }
 }
 
-// One row's heads (or up to 16 of them) of one KV head per workgroup; its
-// waves take the chunks of split blockIdx.z in turn.
-template <int TYPE, unsigned D>
-__global__ __launch_bounds__(kThreads) void kv8_attention_kernel(
-    Kv8Geometry g, const float* __restrict__ qkv, std::uint64_t stride, const std::int32_t* __restrict__ positions,
-    const std::int32_t* __restrict__ tables, std::uint32_t layer, std::uint32_t q_heads, std::uint64_t max_tokens,
-    std::uint32_t split_chunks, float2 score_scale, float* __restrict__ partials, float2* __restrict__ stats,
-    float* __restrict__ out) {
+// max over the four lane groups of a vector, in every lane of it.
+__device__ __forceinline__ int groups_max(int x) {
+    const auto h = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    const int a = static_cast<int>(h[0]), b = static_cast<int>(h[1]);
+    const int m = a > b ? a : b;
+    const auto q = __builtin_amdgcn_permlane16_swap(m, m, false, false);
+    const int c = static_cast<int>(q[0]), d = static_cast<int>(q[1]);
+    return c > d ? c : d;
+}
+
+// The rows of a tile: with RUNS up to kRows rows of one run (kRows whole
+// groups of q heads fit its 16 NV vectors, at least one row), otherwise one
+// row.  A group of more than 16 NV q heads is cut into parts (grid x).
+struct Tile {
+    std::uint32_t row, rows;       // first row, rows (0: no tile)
+    std::uint32_t head, heads;     // q heads of each row
+};
+
+__device__ __forceinline__ Tile find_tile(std::uint32_t index, const std::int32_t* __restrict__ run_starts,
+                                          std::uint32_t runs, std::uint32_t m, std::uint32_t tile_rows) {
+    // Run i owns tiles run_starts[i] / tile_rows + i and on: at least as many
+    // as its rows need, and the count over all runs needs no prefix sum.  The
+    // wave looks 64 runs up at a time.
+    const unsigned lane = threadIdx.x & 63u;
+    std::uint32_t lo = 0u, hi = runs;              // the run is in [lo, hi)
+    const auto first_tile = [&](std::uint32_t i) __attribute__((always_inline)) {
+        const std::int32_t s = run_starts[i];
+        return (s > 0 ? static_cast<std::uint32_t>(s) / tile_rows : 0u) + i;
+    };
+    while (hi - lo > 1u) {
+        const std::uint32_t step = (hi - lo + 63u) / 64u;
+        const std::uint32_t i = lo + lane * step;
+        const bool below = i < hi && first_tile(i) <= index;
+        const std::uint64_t mask = __ballot(below);
+        if (mask == 0u) return Tile{0u, 0u, 0u, 0u};
+        const std::uint32_t last = 63u - static_cast<std::uint32_t>(__builtin_clzll(mask));
+        lo += last * step;
+        hi = lo + step < hi ? lo + step : hi;
+    }
+    const std::int64_t begin = run_starts[lo], end = run_starts[lo + 1u];
+    if (begin < 0 || end > static_cast<std::int64_t>(m) || first_tile(lo) > index) return Tile{0u, 0u, 0u, 0u};
+    const std::int64_t row = begin + static_cast<std::int64_t>(index - first_tile(lo)) * tile_rows;
+    if (row >= end) return Tile{0u, 0u, 0u, 0u};
+    const std::int64_t left = end - row;
+    return Tile{static_cast<std::uint32_t>(row), static_cast<std::uint32_t>(left < tile_rows ? left : tile_rows), 0u, 0u};
+}
+
+// A tile of up to 16 NV query vectors of one KV head per workgroup; its waves
+// take the chunks of split blockIdx.z in turn, every wave for all vectors.
+// With NV > 1 the vectors' operands lie in LDS, and a chunk's codes are turned
+// into f16 once for all of them.
+template <int TYPE, unsigned D, unsigned NV, bool RUNS>
+__global__ __launch_bounds__(kThreads, 2) void kv8_attention_kernel(
+    Kv8Geometry g, const float* __restrict__ qkv, std::uint64_t stride, std::uint32_t m,
+    const std::int32_t* __restrict__ positions, const std::int32_t* __restrict__ tables, std::uint32_t layer,
+    std::uint32_t q_heads, const std::int32_t* __restrict__ run_starts, std::uint32_t runs, std::uint32_t tile_rows,
+    std::uint64_t max_tokens, std::uint32_t split_chunks, float2 score_scale, float* __restrict__ partials,
+    float2* __restrict__ stats, float* __restrict__ out) {
     constexpr unsigned LD = D + 4;
-    __shared__ float sums[kWaves][kVectors][LD];
-    __shared__ int wave_m[kWaves][kVectors], wave_m2[kWaves][kVectors];
-    __shared__ float wave_l[kWaves][kVectors];
+    constexpr unsigned kTile = kVectors * NV;
+    constexpr unsigned kFrags = D / 32;            // k steps of a score
+    union Shared {
+        half8v query[NV > 1u ? NV : 1u][kFrags][2][64];
+        float sums[kWaves][kTile][LD];
+    };
+    __shared__ Shared sh;
+    __shared__ float undo_of[kTile];
+    __shared__ int wave_m[kWaves][kTile], wave_m2[kWaves][kTile];
+    __shared__ float wave_l[kWaves][kTile];
     const unsigned tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, grp = lane >> 4, col = lane & 15u;
-    const std::uint32_t row = blockIdx.x, split = blockIdx.z;
-    const std::uint32_t group = q_heads / g.kv_heads, parts = (group + kVectors - 1u) / kVectors;
-    const std::uint32_t kvh = blockIdx.y / parts, part = blockIdx.y % parts;
-    const std::uint32_t head0 = kvh * group + part * kVectors;
-    const std::uint32_t nq = group - part * kVectors < kVectors ? group - part * kVectors : kVectors;
-    std::int64_t last = positions[row];
-    if (last >= static_cast<std::int64_t>(max_tokens)) last = static_cast<std::int64_t>(max_tokens) - 1;
-    const std::uint32_t chunks = last < 0 ? 0u : static_cast<std::uint32_t>(last / kChunkTokens) + 1u;
+    const std::uint32_t split = blockIdx.z;
+    const std::uint32_t group = q_heads / g.kv_heads, parts = (group + kTile - 1u) / kTile;
+    const std::uint32_t kvh = blockIdx.x / parts, part = blockIdx.x % parts;
+    // The last rows of a run reach furthest: they start first.
+    const std::uint32_t index = gridDim.y - 1u - blockIdx.y;
+    Tile tile{index, 1u, 0u, 0u};
+    if constexpr (RUNS) tile = find_tile(index, run_starts, runs, m, tile_rows);
+    if (tile.rows == 0u) return;
+    tile.head = kvh * group + part * kTile;
+    tile.heads = group - part * kTile < kTile ? group - part * kTile : kTile;
+    const unsigned nq = tile.rows * tile.heads;
+
+    // The furthest position of the tile, and those of this lane's vectors
+    // (places without a vector go along with the furthest).
+    const int most = static_cast<int>(max_tokens) - 1;
+    int reach = -1;
+    for (unsigned r = 0; r < tile.rows; ++r) {
+        const int p = positions[tile.row + r];
+        reach = p > reach ? p : reach;
+    }
+    reach = reach < most ? reach : most;
+    int pos[NV];
+#pragma unroll
+    for (unsigned n = 0; n < NV; ++n) {
+        const unsigned v = n * kVectors + col;
+        pos[n] = v < nq ? positions[tile.row + v / tile.heads] : reach;
+        pos[n] = pos[n] < reach ? pos[n] : reach;
+    }
+    const std::uint32_t chunks = reach < 0 ? 0u : static_cast<std::uint32_t>(reach) / kChunkTokens + 1u;
     const std::uint32_t live = chunks == 0u ? 1u : (chunks + split_chunks - 1u) / split_chunks;
     if (split >= live) return;
-    const std::int32_t* const table = tables + static_cast<std::uint64_t>(row) * g.max_pages;
+    const std::int32_t* const table = tables + static_cast<std::uint64_t>(tile.row) * g.max_pages;
     const std::uint32_t end = chunks < (split + 1u) * split_chunks ? chunks : (split + 1u) * split_chunks;
 
+    const auto vector_at = [&](unsigned v) __attribute__((always_inline)) -> const float* {
+        if (v >= nq) return nullptr;
+        return qkv + static_cast<std::uint64_t>(tile.row + v / tile.heads) * stride +
+               static_cast<std::uint64_t>(tile.head + v % tile.heads) * D;
+    };
     QueryFragments<D> q;
-    load_query<D>(col < nq ? qkv + static_cast<std::uint64_t>(row) * stride + static_cast<std::uint64_t>(head0 + col) * D
-                           : nullptr,
-                  grp, q);
-
-    int m = kNone, m2 = kNone;
-    float l = 0.0f;
-    float4v o[D / 16];
+    float undo[NV];
+    if constexpr (NV == 1u) {
+        load_query<D>(vector_at(col), grp, q);
+        undo[0] = q.undo;
+    } else {
+        for (unsigned n = wave; n < NV; n += kWaves) {
+            load_query<D>(vector_at(n * kVectors + col), grp, q);
 #pragma unroll
-    for (unsigned t = 0; t < D / 16u; ++t) o[t] = float4v{0.f, 0.f, 0.f, 0.f};
+            for (unsigned i = 0; i < kFrags; ++i) {
+                sh.query[n][i][0][lane] = q.lo[i];
+                sh.query[n][i][1][lane] = q.hi[i];
+            }
+            if (grp == 0u) undo_of[n * kVectors + col] = q.undo;
+        }
+        __syncthreads();
+#pragma unroll
+        for (unsigned n = 0; n < NV; ++n) undo[n] = undo_of[n * kVectors + col];
+    }
+
+    int ref[NV], ref2[NV];                         // M and M2
+    float l[NV];
+    float4v o[NV][D / 16];
+#pragma unroll
+    for (unsigned n = 0; n < NV; ++n) {
+        ref[n] = ref2[n] = kNone;
+        l[n] = 0.0f;
+#pragma unroll
+        for (unsigned t = 0; t < D / 16u; ++t) o[n][t] = float4v{0.f, 0.f, 0.f, 0.f};
+    }
 
     for (std::uint32_t c = split * split_chunks + wave; c < end; c += kWaves) {
         const unsigned char* const krec0 = kv8_record(g, table, layer, kvh, c * kChunkBlocks + (col >> 2));
@@ -232,72 +339,110 @@ __global__ __launch_bounds__(kThreads) void kv8_attention_kernel(
         for (unsigned t = 0; t < D / 16u; ++t) {
             vals[t] = *reinterpret_cast<const u32x4*>(vrec + kKv8Codes + kKv8Block * D + (16u * t + col) * 16u);
         }
-        float4v s[4];
-        chunk_scores<TYPE, D>(keys, q, s);
-        // Tokens of this lane's block that the row attends to.
+        float4v s[NV][4];
+        if constexpr (NV == 1u) {
+            chunk_scores<TYPE, D>(keys, q, s[0]);
+        } else {
+#pragma unroll
+            for (unsigned b = 0; b < 4u; ++b) {
+                half8v a[kFrags];
+#pragma unroll
+                for (unsigned i = 0; i < kFrags / 2u; ++i) codes_to_half<TYPE>(keys.c[b][i], a[2u * i], a[2u * i + 1u]);
+#pragma unroll
+                for (unsigned n = 0; n < NV; ++n) {
+                    s[n][b] = float4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (unsigned h = 0; h < 2u; ++h) {   // low parts first
+#pragma unroll
+                        for (unsigned i = 0; i < kFrags; ++i) {
+                            s[n][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i], sh.query[n][i][h][lane], s[n][b], 0, 0, 0);
+                        }
+                    }
+                }
+            }
+        }
+        // Tokens of this lane's block that its vectors may attend to.
         const std::int64_t first = (static_cast<std::int64_t>(c) * kChunkBlocks + grp) * kKv8Block;
-        const int limit = vrec0 == nullptr || last < first ? -1 : last - first > 15 ? 15 : static_cast<int>(last - first);
-        const Factor factor = score_factor(q.undo, score_scale, scales.x);
-        float top = -__builtin_huge_valf();
+        const int exponent = __builtin_amdgcn_frexp_expf(scales.y);   // scale of V < 2^exponent
+        half8v p_hi[NV][2], p_lo[NV][2];
 #pragma unroll
-        for (unsigned b = 0; b < 4u; ++b) {
+        for (unsigned n = 0; n < NV; ++n) {
+            const Factor factor = score_factor(undo[n], score_scale, scales.x);
+            const std::int64_t ahead = pos[n] - first;
+            const int limit = vrec0 == nullptr || ahead < 0 ? -1 : ahead > 15 ? 15 : static_cast<int>(ahead);
+            const bool whole = __all(limit == 15);
+            float top = -__builtin_huge_valf();
+            if (whole) {
 #pragma unroll
-            for (unsigned r = 0; r < 4u; ++r) {
-                if (static_cast<int>(4u * b + r) <= limit) top = fmaxf(top, s[b][r] * factor.hi);
+                for (unsigned b = 0; b < 4u; ++b) {
+#pragma unroll
+                    for (unsigned r = 0; r < 4u; ++r) top = fmaxf(top, s[n][b][r]);
+                }
+            } else {
+#pragma unroll
+                for (unsigned b = 0; b < 4u; ++b) {
+#pragma unroll
+                    for (unsigned r = 0; r < 4u; ++r) {
+                        top = fmaxf(top, static_cast<int>(4u * b + r) <= limit ? s[n][b][r] : -__builtin_huge_valf());
+                    }
+                }
             }
-        }
-        // References: the block's own, then the vector's over the four blocks.
-        const float bound = fminf(fmaxf(ceilf(top), -0x1p28f), 0x1p28f);   // differences stay in 32 bits
-        const int block_m = top == -__builtin_huge_valf() ? kNone : static_cast<int>(bound);
-        const int exponent = __builtin_amdgcn_frexp_expf(scales.y);   // scale < 2^exponent
-        const int block_m2 = block_m == kNone || scales.y == 0.0f ? kNone : block_m + exponent;
-        int m_new = block_m > m ? block_m : m, m2_new = block_m2 > m2 ? block_m2 : m2;
+            // The block's own references; the vector's only move when one of
+            // its blocks passes them.
+            const float bound = fminf(fmaxf(ceilf(top * factor.hi), -0x1p28f), 0x1p28f);   // differences stay in 32 bits
+            const int block_m = limit < 0 ? kNone : static_cast<int>(bound);
+            const int block_m2 = limit < 0 || scales.y == 0.0f ? kNone : block_m + exponent;
+            if (__any(block_m > ref[n] || block_m2 > ref2[n])) {
+                const int next = groups_max(block_m > ref[n] ? block_m : ref[n]);
+                const int next2 = groups_max(block_m2 > ref2[n] ? block_m2 : ref2[n]);
+                l[n] = __builtin_amdgcn_ldexpf(l[n], ref[n] - next);
+                const int down = ref2[n] - next2;
 #pragma unroll
-        for (int off = 16; off <= 32; off <<= 1) {
-            const int a = __shfl_xor(m_new, off), a2 = __shfl_xor(m2_new, off);
-            m_new = a > m_new ? a : m_new;
-            m2_new = a2 > m2_new ? a2 : m2_new;
-        }
-        // p' = 2^(s - base) * share, below 2^kPBits; a scale of V far below
-        // the others' (or zero) keeps base near M, so the same powers also
-        // sum up the denominator.  s - base is small where p is large, and
-        // rounded once.
-        int e = m2_new - m_new - 40;
-        e = scales.y == 0.0f || exponent < e ? e : exponent;
-        const int base = m2_new - e;
-        const float share = __builtin_amdgcn_ldexpf(scales.y, kPBits - e);
-        const float fbase = static_cast<float>(base);
-        float sum = 0.0f;
-        half8v p_hi[2], p_lo[2];
+                for (unsigned t = 0; t < D / 16u; ++t) {
 #pragma unroll
-        for (unsigned b = 0; b < 4u; ++b) {
-#pragma unroll
-            for (unsigned r = 0; r < 4u; ++r) {
-                float x = score_power(s[b][r], factor, fbase);
-                x = static_cast<int>(4u * b + r) <= limit ? x : 0.0f;
-                sum += x;
-                _Float16 hi, lo;
-                split_f16(x * share, hi, lo);
-                p_hi[b >> 1][4u * (b & 1u) + r] = hi;
-                p_lo[b >> 1][4u * (b & 1u) + r] = lo;
+                    for (unsigned r = 0; r < 4u; ++r) o[n][t][r] = __builtin_amdgcn_ldexpf(o[n][t][r], down);
+                }
+                ref[n] = next;
+                ref2[n] = next2;
             }
-        }
-        l = __builtin_amdgcn_ldexpf(l, m - m_new) + __builtin_amdgcn_ldexpf(sum, base - m_new);
-        const int down = m2 - m2_new;
-        if (__any(down != 0)) {
+            // p' = 2^(s - base) * share, below 2^kPBits; a scale of V far below
+            // the others' (or zero) keeps base near M, so the same powers also
+            // sum up the denominator.  s - base is small where p is large, and
+            // rounded once.
+            int e = ref2[n] - ref[n] - 40;
+            e = scales.y == 0.0f || exponent < e ? e : exponent;
+            const int base = ref2[n] - e;
+            const float share = __builtin_amdgcn_ldexpf(scales.y, kPBits - e);
+            const float fbase = static_cast<float>(base);
+            float sum = 0.0f;
 #pragma unroll
-            for (unsigned t = 0; t < D / 16u; ++t) {
+            for (unsigned b = 0; b < 4u; ++b) {
 #pragma unroll
-                for (unsigned r = 0; r < 4u; ++r) o[t][r] = __builtin_amdgcn_ldexpf(o[t][r], down);
+                for (unsigned r = 0; r < 4u; r += 2u) {
+                    float x0 = score_power(s[n][b][r], factor, fbase);
+                    float x1 = score_power(s[n][b][r + 1u], factor, fbase);
+                    if (!whole) {
+                        x0 = static_cast<int>(4u * b + r) <= limit ? x0 : 0.0f;
+                        x1 = static_cast<int>(4u * b + r + 1u) <= limit ? x1 : 0.0f;
+                    }
+                    sum += x0;
+                    sum += x1;
+                    half2v hi, lo;
+                    split_products(x0, x1, share, hi, lo);
+                    p_hi[n][b >> 1][4u * (b & 1u) + r] = hi[0];
+                    p_hi[n][b >> 1][4u * (b & 1u) + r + 1u] = hi[1];
+                    p_lo[n][b >> 1][4u * (b & 1u) + r] = lo[0];
+                    p_lo[n][b >> 1][4u * (b & 1u) + r + 1u] = lo[1];
+                }
             }
+            l[n] += __builtin_amdgcn_ldexpf(sum, base - ref[n]);
         }
-        m = m_new;
-        m2 = m2_new;
         if constexpr (TYPE == kKv8E4M3) {
-            // Slots behind the row's last token may hold NaN codes, which a
+            // Slots behind the tile's last token may hold NaN codes, which a
             // zero p does not silence.
-            if (__any(limit < 15)) {
-                const int n = limit + 1;
+            const std::int64_t ahead = reach - first;
+            if (__any(vrec0 == nullptr || ahead < 15)) {
+                const int n = vrec0 == nullptr || ahead < 0 ? 0 : ahead > 15 ? 16 : static_cast<int>(ahead) + 1;
 #pragma unroll
                 for (int w = 0; w < 4; ++w) {
                     const int bytes = n - 4 * w;
@@ -311,23 +456,31 @@ __global__ __launch_bounds__(kThreads) void kv8_attention_kernel(
         for (unsigned t = 0; t < D / 16u; ++t) {
             half8v a0, a1;
             codes_to_half<TYPE>(vals[t], a0, a1);
-            o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, p_hi[0], o[t], 0, 0, 0);
-            o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, p_lo[0], o[t], 0, 0, 0);
-            o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, p_hi[1], o[t], 0, 0, 0);
-            o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, p_lo[1], o[t], 0, 0, 0);
+#pragma unroll
+            for (unsigned n = 0; n < NV; ++n) {
+                o[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, p_hi[n][0], o[n][t], 0, 0, 0);
+                o[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, p_lo[n][0], o[n][t], 0, 0, 0);
+                o[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, p_hi[n][1], o[n][t], 0, 0, 0);
+                o[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, p_lo[n][1], o[n][t], 0, 0, 0);
+            }
         }
     }
 
     // The waves meet: sums in units of 2^(M2 - kPBits), l of 2^M.
-    l += __shfl_xor(l, 16);
-    l += __shfl_xor(l, 32);
-    if (grp == 0u) {
-        wave_m[wave][col] = m;
-        wave_m2[wave][col] = m2;
-        wave_l[wave][col] = l;
-    }
+    if constexpr (NV > 1u) __syncthreads();        // the query operands make room
 #pragma unroll
-    for (unsigned t = 0; t < D / 16u; ++t) *reinterpret_cast<float4v*>(&sums[wave][col][16u * t + 4u * grp]) = o[t];
+    for (unsigned n = 0; n < NV; ++n) {
+        const unsigned v = n * kVectors + col;
+        l[n] += __shfl_xor(l[n], 16);
+        l[n] += __shfl_xor(l[n], 32);
+        if (grp == 0u) {
+            wave_m[wave][v] = ref[n];
+            wave_m2[wave][v] = ref2[n];
+            wave_l[wave][v] = l[n];
+        }
+#pragma unroll
+        for (unsigned t = 0; t < D / 16u; ++t) *reinterpret_cast<float4v*>(&sh.sums[wave][v][16u * t + 4u * grp]) = o[n][t];
+    }
     __syncthreads();
     for (unsigned idx = tid; idx < nq * (D / 4u); idx += kThreads) {
         const unsigned v = idx / (D / 4u), d4 = idx % (D / 4u);
@@ -342,11 +495,12 @@ __global__ __launch_bounds__(kThreads) void kv8_attention_kernel(
 #pragma unroll
         for (unsigned w = 0; w < kWaves; ++w) {
             total += __builtin_amdgcn_ldexpf(wave_l[w][v], wave_m[w][v] - mm);
-            const float4v a = *reinterpret_cast<const float4v*>(&sums[w][v][4u * d4]);
+            const float4v a = *reinterpret_cast<const float4v*>(&sh.sums[w][v][4u * d4]);
 #pragma unroll
             for (unsigned r = 0; r < 4u; ++r) acc[r] += __builtin_amdgcn_ldexpf(a[r], wave_m2[w][v] - mm2);
         }
-        const std::uint64_t vector = static_cast<std::uint64_t>(row) * q_heads + head0 + v;
+        const std::uint64_t vector =
+            static_cast<std::uint64_t>(tile.row + v / tile.heads) * q_heads + tile.head + v % tile.heads;
         if (live == 1u) {
             float4v y;
 #pragma unroll
@@ -357,57 +511,78 @@ __global__ __launch_bounds__(kThreads) void kv8_attention_kernel(
             if (stats && d4 == 0u) stats[vector] = make_float2(static_cast<float>(mm), total == 0.0f ? 0.0f : 1.0f / total);
         } else {
             float* const p = partials + (vector * gridDim.z + split) * (D + kStat);
-            if (d4 == 0u) {
-                *reinterpret_cast<float4v*>(p) = float4v{__int_as_float(mm), __int_as_float(mm2), total, 0.0f};
-            }
+            if (d4 == 0u) *reinterpret_cast<float4v*>(p) = float4v{__int_as_float(mm), __int_as_float(mm2), total, 0.0f};
             *reinterpret_cast<float4v*>(p + kStat + 4u * d4) = acc;
         }
     }
 }
 
-// Joins the splits of a row's vectors.
-template <unsigned D>
-__global__ __launch_bounds__(kThreads) void kv8_merge_kernel(const std::int32_t* __restrict__ positions,
-                                                             std::uint32_t q_heads, std::uint64_t max_tokens,
-                                                             std::uint32_t split_chunks, std::uint32_t splits,
-                                                             const float* __restrict__ partials,
-                                                             float2* __restrict__ stats, float* __restrict__ out) {
-    const std::uint32_t row = blockIdx.x;
-    const unsigned idx = blockIdx.y * kThreads + threadIdx.x;
-    if (idx >= q_heads * (D / 4u)) return;
-    std::int64_t last = positions[row];
-    if (last >= static_cast<std::int64_t>(max_tokens)) last = static_cast<std::int64_t>(max_tokens) - 1;
-    const std::uint32_t chunks = last < 0 ? 0u : static_cast<std::uint32_t>(last / kChunkTokens) + 1u;
+// Joins the splits of a tile's vectors (as many as its furthest position made
+// workgroups of), eight loads in flight.
+template <unsigned D, unsigned NV, bool RUNS>
+__global__ __launch_bounds__(kThreads) void kv8_merge_kernel(
+    const std::int32_t* __restrict__ positions, std::uint32_t m, std::uint32_t q_heads, std::uint32_t kv_heads,
+    const std::int32_t* __restrict__ run_starts, std::uint32_t runs, std::uint32_t tile_rows, std::uint64_t max_tokens,
+    std::uint32_t split_chunks, std::uint32_t splits, const float* __restrict__ partials, float2* __restrict__ stats,
+    float* __restrict__ out) {
+    constexpr unsigned kTile = kVectors * NV;
+    constexpr unsigned kBatch = 8;
+    const std::uint32_t group = q_heads / kv_heads, parts = (group + kTile - 1u) / kTile;
+    const std::uint32_t kvh = blockIdx.x / parts, part = blockIdx.x % parts;
+    Tile tile{blockIdx.y, 1u, 0u, 0u};
+    if constexpr (RUNS) tile = find_tile(blockIdx.y, run_starts, runs, m, tile_rows);
+    if (tile.rows == 0u) return;
+    tile.head = kvh * group + part * kTile;
+    tile.heads = group - part * kTile < kTile ? group - part * kTile : kTile;
+    int reach = -1;
+    for (unsigned r = 0; r < tile.rows; ++r) {
+        const int p = positions[tile.row + r];
+        reach = p > reach ? p : reach;
+    }
+    const int most = static_cast<int>(max_tokens) - 1;
+    reach = reach < most ? reach : most;
+    const std::uint32_t chunks = reach < 0 ? 0u : static_cast<std::uint32_t>(reach) / kChunkTokens + 1u;
     const std::uint32_t live = (chunks + split_chunks - 1u) / split_chunks;
-    if (live <= 1u) return;   // the attention kernel wrote this row
-    const unsigned v = idx / (D / 4u), d4 = idx % (D / 4u);
-    const std::uint64_t vector = static_cast<std::uint64_t>(row) * q_heads + v;
-    const float* const base = partials + vector * splits * (D + kStat);
-    int m = kNone, m2 = kNone;
-    float total = 0.0f;
-    float4v acc = {0.f, 0.f, 0.f, 0.f};
-    for (std::uint32_t s = 0; s < live; ++s) {
-        const float4v head = *reinterpret_cast<const float4v*>(base + s * (D + kStat));
-        const float4v a = *reinterpret_cast<const float4v*>(base + s * (D + kStat) + kStat + 4u * d4);
-        const int pm = __float_as_int(head[0]), pm2 = __float_as_int(head[1]);
-        const int nm = pm > m ? pm : m, nm2 = pm2 > m2 ? pm2 : m2;
-        total = __builtin_amdgcn_ldexpf(total, m - nm) + __builtin_amdgcn_ldexpf(head[2], pm - nm);
+    if (live <= 1u) return;   // the attention kernel wrote this tile
+    for (unsigned idx = threadIdx.x; idx < tile.rows * tile.heads * (D / 4u); idx += kThreads) {
+        const unsigned v = idx / (D / 4u), d4 = idx % (D / 4u);
+        const std::uint64_t vector =
+            static_cast<std::uint64_t>(tile.row + v / tile.heads) * q_heads + tile.head + v % tile.heads;
+        const float* const base = partials + vector * splits * (D + kStat);
+        int ref = kNone, ref2 = kNone;
+        float total = 0.0f;
+        float4v acc = {0.f, 0.f, 0.f, 0.f};
+        for (std::uint32_t s0 = 0; s0 < live; s0 += kBatch) {
+            float4v head[kBatch], part_sum[kBatch];
+#pragma unroll
+            for (unsigned j = 0; j < kBatch; ++j) {
+                const std::uint32_t at = (s0 + j < live ? s0 + j : live - 1u) * (D + kStat);
+                head[j] = *reinterpret_cast<const float4v*>(base + at);
+                part_sum[j] = *reinterpret_cast<const float4v*>(base + at + kStat + 4u * d4);
+            }
+#pragma unroll
+            for (unsigned j = 0; j < kBatch; ++j) {
+                if (s0 + j >= live) continue;
+                const int a = __float_as_int(head[j][0]), a2 = __float_as_int(head[j][1]);
+                const int next = a > ref ? a : ref, next2 = a2 > ref2 ? a2 : ref2;
+                total = __builtin_amdgcn_ldexpf(total, ref - next) + __builtin_amdgcn_ldexpf(head[j][2], a - next);
+#pragma unroll
+                for (unsigned r = 0; r < 4u; ++r) {
+                    acc[r] = __builtin_amdgcn_ldexpf(acc[r], ref2 - next2) + __builtin_amdgcn_ldexpf(part_sum[j][r], a2 - next2);
+                }
+                ref = next;
+                ref2 = next2;
+            }
+        }
+        float4v y;
 #pragma unroll
         for (unsigned r = 0; r < 4u; ++r) {
-            acc[r] = __builtin_amdgcn_ldexpf(acc[r], m2 - nm2) + __builtin_amdgcn_ldexpf(a[r], pm2 - nm2);
+            y[r] = total == 0.0f ? 0.0f : __builtin_amdgcn_ldexpf(acc[r] / total, ref2 - kPBits - ref);
         }
-        m = nm;
-        m2 = nm2;
+        *reinterpret_cast<float4v*>(out + vector * D + 4u * d4) = y;
+        if (stats && d4 == 0u) stats[vector] = make_float2(static_cast<float>(ref), total == 0.0f ? 0.0f : 1.0f / total);
     }
-    float4v y;
-#pragma unroll
-    for (unsigned r = 0; r < 4u; ++r) {
-        y[r] = total == 0.0f ? 0.0f : __builtin_amdgcn_ldexpf(acc[r] / total, m2 - kPBits - m);
-    }
-    *reinterpret_cast<float4v*>(out + vector * D + 4u * d4) = y;
-    if (stats && d4 == 0u) stats[vector] = make_float2(static_cast<float>(m), total == 0.0f ? 0.0f : 1.0f / total);
 }
-
 // The weights a run's rows give one chunk of tokens: the scores again, by the
 // same instructions as in the attention, and p from the rows' statistics.
 // A chunk of a (run, KV head) has one wave, which adds its sums with one
@@ -497,19 +672,26 @@ __global__ __launch_bounds__(kThreads) void kv8_weights_kernel(
 
 } // namespace
 
-Kv8Shape kv8_attention_shape(std::uint32_t m, std::uint32_t q_heads, std::uint32_t kv_heads, std::uint64_t max_tokens) {
-    const std::uint32_t group = q_heads / kv_heads, parts = (group + kVectors - 1u) / kVectors;
+Kv8Shape kv8_attention_shape(std::uint32_t m, std::uint32_t q_heads, std::uint32_t kv_heads, std::uint32_t runs,
+                             std::uint64_t max_tokens) {
+    const std::uint32_t group = q_heads / kv_heads;
+    // Two rows a run on average share their keys; below that a tile is a row.
+    const bool by_run = runs != 0u && m >= 2u * runs;
+    const std::uint32_t tile = kVectors * (by_run ? kPromptTiles : 1u);
+    const std::uint32_t parts = (group + tile - 1u) / tile;
+    const std::uint32_t tile_rows = by_run && group < tile ? tile / group : 1u;
+    const std::uint32_t tiles = by_run ? m / tile_rows + runs : m;
     const std::uint32_t chunks = static_cast<std::uint32_t>((max_tokens + kChunkTokens - 1u) / kChunkTokens);
     // Splits of equal length, so that rows of unequal lengths make workgroups
     // of equal work: at least two chunks a wave, and at most about four
     // workgroups a CU if every row were max_tokens long.
-    const std::uint64_t tiles = static_cast<std::uint64_t>(m) * kv_heads * parts;
-    std::uint64_t per = (tiles * chunks + 1023u) / 1024u;
+    const std::uint64_t groups = static_cast<std::uint64_t>(by_run ? m / tile_rows + 1u : m) * kv_heads * parts;
+    std::uint64_t per = (groups * chunks + 1023u) / 1024u;
     per = (per + kWaves - 1u) / kWaves * kWaves;
     if (per < 2u * kWaves) per = 2u * kWaves;
     if (per > chunks) per = chunks;
     const std::uint32_t splits = static_cast<std::uint32_t>((chunks + per - 1u) / per);
-    return Kv8Shape{m, kv_heads * parts, splits, static_cast<std::uint32_t>(per)};
+    return Kv8Shape{tiles, kv_heads * parts, splits, static_cast<std::uint32_t>(per), by_run ? tile_rows : 0u};
 }
 
 std::uint64_t kv8_attention_scratch(const Kv8Shape& shape, std::uint32_t m, std::uint32_t q_heads,
@@ -518,6 +700,48 @@ std::uint64_t kv8_attention_scratch(const Kv8Shape& shape, std::uint32_t m, std:
     const std::uint64_t stats = weights ? (vectors * sizeof(float2) + 255u) / 256u * 256u : 0u;
     return stats + (shape.splits > 1u ? vectors * shape.splits * (head_dim + kStat) * sizeof(float) : 0u);
 }
+
+namespace {
+
+template <int TYPE, unsigned D, unsigned NV, bool RUNS>
+void launch_tiles(const Kv8Geometry& g, const float* qkv, std::uint64_t stride, std::uint32_t m,
+                  const std::int32_t* positions, const std::int32_t* tables, std::uint32_t layer, std::uint32_t q_heads,
+                  const std::int32_t* run_starts, std::uint32_t runs, std::uint64_t max_tokens, const Kv8Shape& shape,
+                  float2 scale, float* partials, float2* stats, float* out, hipStream_t stream) {
+    hipLaunchKernelGGL((kv8_attention_kernel<TYPE, D, NV, RUNS>), dim3(shape.tile_heads, shape.tiles, shape.splits),
+                       dim3(kThreads), 0, stream, g, qkv, stride, m, positions, tables, layer, q_heads, run_starts, runs,
+                       shape.tile_rows, max_tokens, shape.split_chunks, scale, partials, stats, out);
+    if (shape.splits > 1u) {
+        hipLaunchKernelGGL((kv8_merge_kernel<D, NV, RUNS>), dim3(shape.tile_heads, shape.tiles), dim3(kThreads), 0,
+                           stream, positions, m, q_heads, g.kv_heads, run_starts, runs, shape.tile_rows, max_tokens,
+                           shape.split_chunks, shape.splits, partials, stats, out);
+    }
+}
+
+template <int TYPE, unsigned D>
+void launch_typed(const Kv8Geometry& g, const float* qkv, std::uint64_t stride, std::uint32_t m,
+                  const std::int32_t* positions, const std::int32_t* tables, std::uint32_t layer, std::uint32_t q_heads,
+                  const std::int32_t* run_starts, std::uint32_t runs, std::uint64_t max_tokens, int weights,
+                  const Kv8Shape& shape, float* partials, float2* stats, float* out, hipStream_t stream) {
+    // Scores in powers of two: s log2(e) = (q . k) * log2(e) / sqrt(D).
+    const double exact = 1.4426950408889634 / __builtin_sqrt(static_cast<double>(D));
+    const float2 scale = make_float2(static_cast<float>(exact), static_cast<float>(exact - static_cast<float>(exact)));
+    if (shape.tile_rows != 0u) {
+        launch_tiles<TYPE, D, kPromptTiles, true>(g, qkv, stride, m, positions, tables, layer, q_heads, run_starts, runs,
+                                                  max_tokens, shape, scale, partials, stats, out, stream);
+    } else {
+        launch_tiles<TYPE, D, 1u, false>(g, qkv, stride, m, positions, tables, layer, q_heads, nullptr, 0u, max_tokens,
+                                         shape, scale, partials, stats, out, stream);
+    }
+    if (weights) {
+        const std::uint64_t chunks = (max_tokens + kChunkTokens - 1u) / kChunkTokens;
+        const dim3 grid(static_cast<unsigned>((chunks + kWaves - 1u) / kWaves), g.kv_heads, run_starts ? runs : m);
+        hipLaunchKernelGGL((kv8_weights_kernel<TYPE, D>), grid, dim3(kThreads), 0, stream, g, qkv, stride, m, positions,
+                           tables, layer, q_heads, run_starts, max_tokens, scale, stats, weights == 1);
+    }
+}
+
+} // namespace
 
 hipError_t launch_kv8_attention(const Kv8Geometry& g, const float* qkv, std::uint64_t stride, std::uint32_t m,
                                 const std::int32_t* positions, const std::int32_t* tables, std::uint32_t layer,
@@ -528,38 +752,10 @@ hipError_t launch_kv8_attention(const Kv8Geometry& g, const float* qkv, std::uin
     float2* const stats = weights ? static_cast<float2*>(scratch) : nullptr;
     float* const partials = reinterpret_cast<float*>(
         static_cast<unsigned char*>(scratch) + (weights ? (vectors * sizeof(float2) + 255u) / 256u * 256u : 0u));
-    // Scores in powers of two: s log2(e) = (q . k) * log2(e) / sqrt(D).
-    const double exact = 1.4426950408889634 / __builtin_sqrt(static_cast<double>(g.head_dim));
-    const float2 scale = make_float2(static_cast<float>(exact), static_cast<float>(exact - static_cast<float>(exact)));
-    const dim3 grid(shape.tiles, shape.tile_heads, shape.splits);
-    const std::uint64_t chunks = (max_tokens + kChunkTokens - 1u) / kChunkTokens;
-    const dim3 weight_grid(static_cast<unsigned>((chunks + kWaves - 1u) / kWaves), g.kv_heads, runs);
-#define AIR_KV8_ATTENTION(T, D)                                                                                     \
-    hipLaunchKernelGGL((kv8_attention_kernel<T, D>), grid, dim3(kThreads), 0, stream, g, qkv, stride, positions, tables, \
-                       layer, q_heads, max_tokens, shape.split_chunks, scale, partials, stats, out);                \
-    if (shape.splits > 1u) {                                                                                        \
-        hipLaunchKernelGGL(kv8_merge_kernel<D>, dim3(m, (q_heads * (D / 4u) + kThreads - 1u) / kThreads),           \
-                           dim3(kThreads), 0, stream, positions, q_heads, max_tokens, shape.split_chunks, shape.splits, \
-                           partials, stats, out);                                                                   \
-    }                                                                                                               \
-    if (weights) {                                                                                                  \
-        hipLaunchKernelGGL((kv8_weights_kernel<T, D>), weight_grid, dim3(kThreads), 0, stream, g, qkv, stride, m,   \
-                           positions, tables, layer, q_heads, run_starts, max_tokens, scale, stats, weights == 1);  \
-    }
-    if (g.type == kKv8I8) {
-        if (g.head_dim == 128u) {
-            AIR_KV8_ATTENTION(kKv8I8, 128)
-        } else {
-            AIR_KV8_ATTENTION(kKv8I8, 64)
-        }
-    } else {
-        if (g.head_dim == 128u) {
-            AIR_KV8_ATTENTION(kKv8E4M3, 128)
-        } else {
-            AIR_KV8_ATTENTION(kKv8E4M3, 64)
-        }
-    }
-#undef AIR_KV8_ATTENTION
+    const auto launch = g.type == kKv8I8 ? (g.head_dim == 128u ? launch_typed<kKv8I8, 128> : launch_typed<kKv8I8, 64>)
+                                         : (g.head_dim == 128u ? launch_typed<kKv8E4M3, 128> : launch_typed<kKv8E4M3, 64>);
+    launch(g, qkv, stride, m, positions, tables, layer, q_heads, run_starts, runs, max_tokens, weights, shape, partials,
+           stats, out, stream);
     return hipGetLastError();
 }
 

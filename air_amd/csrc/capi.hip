@@ -2348,25 +2348,27 @@ int air_hip_kv8_attention(air_hip_context* ctx, const air_hip_kv8_layout* kv, co
     if (weights != AIR_HIP_KV8_WEIGHTS_NONE && weights != AIR_HIP_KV8_WEIGHTS_ADD && weights != AIR_HIP_KV8_WEIGHTS_SET) {
         return fail(AIR_HIP_INVALID_ARGUMENT, "weights must be NONE, ADD or SET, not %d", weights);
     }
-    if (!run_starts && runs != 0) return fail(AIR_HIP_INVALID_ARGUMENT, "%u runs need run_starts", runs);
+    if ((run_starts == nullptr) != (runs == 0)) {
+        return fail(AIR_HIP_INVALID_ARGUMENT, "run_starts and a number of runs go together (%u given)", runs);
+    }
     if (row_stride < static_cast<uint64_t>(q_heads) * kv->head_dim || row_stride % 4u != 0 ||
         reinterpret_cast<std::uintptr_t>(qkv) % 16u != 0 || reinterpret_cast<std::uintptr_t>(out) % 16u != 0) {
         return fail(AIR_HIP_INVALID_ARGUMENT, "q|k|v rows and output must be 16-byte aligned, stride >= the q heads");
     }
     if (m == 0) return AIR_HIP_OK;
-    if (m > 65535u || q_heads > 65535u || runs > 65535u) {
-        return fail(AIR_HIP_UNSUPPORTED, "at most 65535 rows, runs and q heads per call");
+    if (static_cast<uint64_t>(m) + runs > 65535u || q_heads > 65535u) {
+        return fail(AIR_HIP_UNSUPPORTED, "at most 65535 rows and runs together, and q heads, per call");
     }
     DeviceScope scope(ctx->device);
     if (scope.status() != hipSuccess) return hip_fail(scope.status(), "hipSetDevice");
-    const Kv8Shape shape = kv8_attention_shape(m, q_heads, kv->kv_heads, max_tokens);
+    const Kv8Shape shape = kv8_attention_shape(m, q_heads, kv->kv_heads, runs, max_tokens);
     if (int rc = ensure_attention_scratch(ctx, kv8_attention_scratch(shape, m, q_heads, kv->head_dim, weights != 0));
         rc != AIR_HIP_OK) {
         return rc;
     }
     const hipError_t err =
         launch_kv8_attention(kv8_geometry_of(kv), qkv, row_stride, m, positions, page_tables, layer, q_heads, run_starts,
-                             run_starts ? runs : m, max_tokens, weights, shape, ctx->attention_scratch, out, ctx->stream);
+                             runs, max_tokens, weights, shape, ctx->attention_scratch, out, ctx->stream);
     return err == hipSuccess ? AIR_HIP_OK : hip_fail(err, "kv8_attention_kernel");
 }
 

@@ -711,7 +711,7 @@ def test_refusals(torch_cuda, hip_ctx):
         assert read(**over) == 1, over
     assert read(seqs=65536) == 6
     for over in [dict(x=None), dict(pos=None), dict(out=None), dict(layer=2), dict(heads=0), dict(heads=3),
-                 dict(top=0), dict(top=65), dict(mode=3), dict(mode=-1), dict(runs=1), dict(stride=255),
+                 dict(top=0), dict(top=65), dict(mode=3), dict(mode=-1), dict(runs=1), dict(starts=i), dict(stride=255),
                  dict(stride=510), dict(x=p + 4), dict(out=p + 4)]:
         assert attend(**over) == 1, over
     for over in [dict(m=65536), dict(starts=i, runs=65536)]:
