@@ -28,13 +28,18 @@ namespace air_hip {
 constexpr unsigned kKv8Weights = 64;    // byte offset of the weights
 constexpr unsigned kKv8Codes = 128;     // byte offset of the K codes
 
-// Record of block `block` of the sequence with this page table, or null when
-// the table does not name a page of the pool.
-__device__ __forceinline__ unsigned char* kv8_record(const Kv8Geometry& g, const std::int32_t* table,
-                                                     std::uint32_t layer, std::uint32_t head, std::uint32_t block) {
-    const std::uint32_t slot = g.page_magic == 0u ? block : __umulhi(block, g.page_magic);
-    if (slot >= g.max_pages) return nullptr;
-    const std::int32_t page = table[slot];
+// A record in global memory: its address as the loads take it.
+typedef __attribute__((address_space(1))) unsigned char Kv8Byte;
+
+// Entry of a page table that names block `block`'s page.
+__device__ __forceinline__ std::uint32_t kv8_slot(const Kv8Geometry& g, std::uint32_t block) {
+    return g.page_magic == 0u ? block : __umulhi(block, g.page_magic);
+}
+
+// Record of block `block` in the page that entry `slot` of its table names;
+// null when the pool holds no such page.
+__device__ __forceinline__ Kv8Byte* kv8_record_in(const Kv8Geometry& g, std::int32_t page, std::uint32_t slot,
+                                                  std::uint32_t layer, std::uint32_t head, std::uint32_t block) {
     if (page < 0 || static_cast<std::uint32_t>(page) >= g.pool_pages) return nullptr;
     std::uint32_t p = static_cast<std::uint32_t>(page);
     unsigned char* base = g.pool;
@@ -45,7 +50,16 @@ __device__ __forceinline__ unsigned char* kv8_record(const Kv8Geometry& g, const
     }
     const std::uint64_t index = (static_cast<std::uint64_t>(layer) * g.kv_heads + head) * g.page_blocks +
                                 (block - slot * g.page_blocks);
-    return base + p * g.page_bytes + index * g.record_bytes;
+    return (Kv8Byte*)(base + p * g.page_bytes + index * g.record_bytes);
+}
+
+// Record of block `block` of the sequence with this page table, or null when
+// the table does not name a page of the pool.
+__device__ __forceinline__ unsigned char* kv8_record(const Kv8Geometry& g, const std::int32_t* table,
+                                                     std::uint32_t layer, std::uint32_t head, std::uint32_t block) {
+    const std::uint32_t slot = kv8_slot(g, block);
+    if (slot >= g.max_pages) return nullptr;
+    return (unsigned char*)kv8_record_in(g, table[slot], slot, layer, head, block);
 }
 
 // Offset of (token, dim) in a record's K and V codes.

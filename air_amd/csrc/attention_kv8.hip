@@ -138,50 +138,57 @@ struct KeyCodes {
 };
 
 template <unsigned D>
-__device__ __forceinline__ void load_keys(const unsigned char* rec, unsigned lane, KeyCodes<D>& k) {
-    const unsigned char* const at = rec + kKv8Codes + (lane >> 4) * 64u + (lane & 3u) * 16u;
+__device__ __forceinline__ void load_keys(const Kv8Byte* rec, unsigned lane, KeyCodes<D>& k) {
+    const Kv8Byte* const at = rec + kKv8Codes + (lane >> 4) * 64u + (lane & 3u) * 16u;
 #pragma unroll
     for (unsigned b = 0; b < 4u; ++b) {
 #pragma unroll
         for (unsigned s = 0; s < D / 64u; ++s) {
-            k.c[b][s] = *reinterpret_cast<const u32x4*>(at + b * (D * 4u) + s * 256u);
+            k.c[b][s] = *(const __attribute__((address_space(1))) u32x4*)(at + b * (D * 4u) + s * 256u);
         }
     }
 }
 
-// c = a b to twice the precision: what a block's scores are multiplied by (to
-// one f32 a block's scores would all be off by up to 2^-24 of themselves).
-struct Factor {
-    float hi, lo;
-};
-__device__ __forceinline__ Factor score_factor(float undo, float2 score_scale, float k_scale) {
-    const float a = undo * score_scale.x;          // undo is a power of two
-    const float hi = a * k_scale;
-    return Factor{hi, __builtin_fmaf(undo * score_scale.y, k_scale, __builtin_fmaf(a, k_scale, -hi))};
+// What a block's scores are multiplied by.  A block without a scale has codes
+// of zero; any factor will do, and one makes its masked scores -inf.
+__device__ __forceinline__ float score_factor(float undo, float score_scale, float k_scale) {
+    const float f = undo * score_scale * k_scale;      // undo is a power of two
+    return f == 0.0f ? 1.0f : f;
 }
-// 2^(score * factor - base)
-__device__ __forceinline__ float score_power(float score, const Factor& f, float base) {
-    return __builtin_amdgcn_exp2f(__builtin_fmaf(score, f.hi, __builtin_fmaf(score, f.lo, -base)));
+// 2^(score * factor - base), one rounding
+__device__ __forceinline__ float score_power(float score, float factor, float base) {
+    return __builtin_amdgcn_exp2f(__builtin_fmaf(score, factor, -base));
+}
+
+// A lane's codes of the chunk's V: dim 16 t + lane % 16 of block lane / 16.
+template <unsigned D>
+__device__ __forceinline__ void load_values(const Kv8Byte* rec, unsigned lane, u32x4 (&v)[D / 16]) {
+    const Kv8Byte* const at = rec + kKv8Codes + kKv8Block * D + (lane & 15u) * 16u;
+#pragma unroll
+    for (unsigned t = 0; t < D / 16u; ++t) v[t] = *(const __attribute__((address_space(1))) u32x4*)(at + t * 256u);
+}
+
+// The two scales of a record.
+__device__ __forceinline__ float2 load_scales(const Kv8Byte* rec) {
+    const u32x2 v = *(const __attribute__((address_space(1))) u32x2*)rec;
+    return make_float2(__uint_as_float(v.x), __uint_as_float(v.y));
 }
 
 // S^T of the chunk: score[b][r] is token 4 b + r of this lane's block for
 // vector lane % 16, times the fragments' scale.
+// The low parts come first: their roundings are those of a small sum.
 template <int TYPE, unsigned D>
-__device__ __forceinline__ void chunk_scores(const KeyCodes<D>& k, const QueryFragments<D>& q, float4v score[4]) {
+__device__ __forceinline__ void chunk_scores(const KeyCodes<D>& k, const QueryFragments<D>& q, float4v (&score)[4]) {
 #pragma unroll
     for (unsigned b = 0; b < 4u; ++b) {
         half8v a[D / 32];
-#pragma unroll
-        for (unsigned s = 0; s < D / 64u; ++s) codes_to_half<TYPE>(k.c[b][s], a[2u * s], a[2u * s + 1u]);
-        // The low parts first: their roundings are those of a small sum.
         score[b] = float4v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (unsigned i = 0; i < D / 32u; ++i) {
-            score[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i], q.lo[i], score[b], 0, 0, 0);
-        }
+        for (unsigned s = 0; s < D / 64u; ++s) codes_to_half<TYPE>(k.c[b][s], a[2u * s], a[2u * s + 1u]);
 #pragma unroll
-        for (unsigned i = 0; i < D / 32u; ++i) {
-            score[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i], q.hi[i], score[b], 0, 0, 0);
+        for (unsigned i = 0; i < D / 16u; ++i) {
+            const half8v f = i < D / 32u ? q.lo[i] : q.hi[i - D / 32u];
+            score[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i % (D / 32u)], f, score[b], 0, 0, 0);
         }
     }
 }
@@ -238,11 +245,11 @@ __device__ __forceinline__ Tile find_tile(std::uint32_t index, const std::int32_
 // With NV > 1 the vectors' operands lie in LDS, and a chunk's codes are turned
 // into f16 once for all of them.
 template <int TYPE, unsigned D, unsigned NV, bool RUNS>
-__global__ __launch_bounds__(kThreads, 2) void kv8_attention_kernel(
+__global__ __launch_bounds__(kThreads, NV == 1u ? 3 : 2) void kv8_attention_kernel(
     Kv8Geometry g, const float* __restrict__ qkv, std::uint64_t stride, std::uint32_t m,
     const std::int32_t* __restrict__ positions, const std::int32_t* __restrict__ tables, std::uint32_t layer,
     std::uint32_t q_heads, const std::int32_t* __restrict__ run_starts, std::uint32_t runs, std::uint32_t tile_rows,
-    std::uint64_t max_tokens, std::uint32_t split_chunks, float2 score_scale, float* __restrict__ partials,
+    std::uint64_t max_tokens, std::uint32_t split_chunks, float score_scale, float* __restrict__ partials,
     float2* __restrict__ stats, float* __restrict__ out) {
     constexpr unsigned LD = D + 4;
     constexpr unsigned kTile = kVectors * NV;
@@ -326,35 +333,48 @@ __global__ __launch_bounds__(kThreads, 2) void kv8_attention_kernel(
         for (unsigned t = 0; t < D / 16u; ++t) o[n][t] = float4v{0.f, 0.f, 0.f, 0.f};
     }
 
-    for (std::uint32_t c = split * split_chunks + wave; c < end; c += kWaves) {
-        const unsigned char* const krec0 = kv8_record(g, table, layer, kvh, c * kChunkBlocks + (col >> 2));
-        const unsigned char* const vrec0 = kv8_record(g, table, layer, kvh, c * kChunkBlocks + grp);
-        const unsigned char* const krec = krec0 ? krec0 : g_no_record;
-        const unsigned char* const vrec = vrec0 ? vrec0 : g_no_record;
+    // Page ids are read a chunk ahead, before this chunk's codes: loads return
+    // in order, so what waits for the ids does not wait for the codes.
+    const Kv8Byte* const none = (const Kv8Byte*)g_no_record;
+    const std::uint32_t from = split * split_chunks + wave;
+    const auto page_of = [&](std::uint32_t block, std::uint32_t& slot) __attribute__((always_inline)) -> std::int32_t {
+        slot = kv8_slot(g, block);
+        return slot < g.max_pages ? table[slot] : -1;
+    };
+    // Pages of the blocks whose K and V this lane loads.
+    std::uint32_t k_block = from * kChunkBlocks + (col >> 2), v_block = from * kChunkBlocks + grp, k_slot, v_slot;
+    std::int32_t k_page = page_of(k_block, k_slot), v_page = page_of(v_block, v_slot);
+    for (std::uint32_t c = from; c < end; c += kWaves) {
+        const Kv8Byte* const krec = kv8_record_in(g, k_page, k_slot, layer, kvh, k_block);
+        const Kv8Byte* const vrec = kv8_record_in(g, v_page, v_slot, layer, kvh, v_block);
+        const bool here = vrec != nullptr;
+        k_block += kWaves * kChunkBlocks;
+        v_block += kWaves * kChunkBlocks;
+        k_page = page_of(k_block, k_slot);
+        v_page = page_of(v_block, v_slot);
         KeyCodes<D> keys;
-        load_keys<D>(krec, lane, keys);
-        const float2 scales = *reinterpret_cast<const float2*>(vrec);
         u32x4 vals[D / 16];
-#pragma unroll
-        for (unsigned t = 0; t < D / 16u; ++t) {
-            vals[t] = *reinterpret_cast<const u32x4*>(vrec + kKv8Codes + kKv8Block * D + (16u * t + col) * 16u);
-        }
+        load_keys<D>(krec ? krec : none, lane, keys);
+        const float2 now = load_scales(vrec ? vrec : none);
+        load_values<D>(vrec ? vrec : none, lane, vals);
         float4v s[NV][4];
         if constexpr (NV == 1u) {
             chunk_scores<TYPE, D>(keys, q, s[0]);
         } else {
+            asm volatile("" ::: "memory");         // the query operands are read again, not kept in registers
 #pragma unroll
             for (unsigned b = 0; b < 4u; ++b) {
                 half8v a[kFrags];
 #pragma unroll
                 for (unsigned i = 0; i < kFrags / 2u; ++i) codes_to_half<TYPE>(keys.c[b][i], a[2u * i], a[2u * i + 1u]);
 #pragma unroll
-                for (unsigned n = 0; n < NV; ++n) {
-                    s[n][b] = float4v{0.f, 0.f, 0.f, 0.f};
+                for (unsigned n = 0; n < NV; ++n) s[n][b] = float4v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (unsigned h = 0; h < 2u; ++h) {   // low parts first
+                for (unsigned h = 0; h < 2u; ++h) {       // low parts first
 #pragma unroll
-                        for (unsigned i = 0; i < kFrags; ++i) {
+                    for (unsigned i = 0; i < kFrags; ++i) {
+#pragma unroll
+                        for (unsigned n = 0; n < NV; ++n) {
                             s[n][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i], sh.query[n][i][h][lane], s[n][b], 0, 0, 0);
                         }
                     }
@@ -362,36 +382,39 @@ __global__ __launch_bounds__(kThreads, 2) void kv8_attention_kernel(
             }
         }
         // Tokens of this lane's block that its vectors may attend to.
-        const std::int64_t first = (static_cast<std::int64_t>(c) * kChunkBlocks + grp) * kKv8Block;
-        const int exponent = __builtin_amdgcn_frexp_expf(scales.y);   // scale of V < 2^exponent
+        const int first = static_cast<int>((c * kChunkBlocks + grp) * kKv8Block);
+        const int exponent = __builtin_amdgcn_frexp_expf(now.y);   // scale of V < 2^exponent
         half8v p_hi[NV][2], p_lo[NV][2];
 #pragma unroll
         for (unsigned n = 0; n < NV; ++n) {
-            const Factor factor = score_factor(undo[n], score_scale, scales.x);
-            const std::int64_t ahead = pos[n] - first;
-            const int limit = vrec0 == nullptr || ahead < 0 ? -1 : ahead > 15 ? 15 : static_cast<int>(ahead);
-            const bool whole = __all(limit == 15);
-            float top = -__builtin_huge_valf();
-            if (whole) {
-#pragma unroll
-                for (unsigned b = 0; b < 4u; ++b) {
-#pragma unroll
-                    for (unsigned r = 0; r < 4u; ++r) top = fmaxf(top, s[n][b][r]);
-                }
-            } else {
+            float factor = score_factor(undo[n], score_scale, now.x);
+            float v_scale = now.y;
+            const int ahead = pos[n] - first;
+            if (!__all(here && ahead >= 15)) {
+                // What a vector does not see scores -inf; a block that it sees
+                // nothing of has no scales either (they may be NaN).
+                const int limit = here ? ahead : -1;
+                factor = limit < 0 ? 1.0f : factor;
+                v_scale = limit < 0 ? 0.0f : v_scale;
 #pragma unroll
                 for (unsigned b = 0; b < 4u; ++b) {
 #pragma unroll
                     for (unsigned r = 0; r < 4u; ++r) {
-                        top = fmaxf(top, static_cast<int>(4u * b + r) <= limit ? s[n][b][r] : -__builtin_huge_valf());
+                        s[n][b][r] = static_cast<int>(4u * b + r) <= limit ? s[n][b][r] : -__builtin_huge_valf();
                     }
                 }
             }
+            float top = s[n][0][0];
+#pragma unroll
+            for (unsigned b = 0; b < 4u; ++b) {
+#pragma unroll
+                for (unsigned r = 0; r < 4u; ++r) top = fmaxf(top, s[n][b][r]);
+            }
             // The block's own references; the vector's only move when one of
             // its blocks passes them.
-            const float bound = fminf(fmaxf(ceilf(top * factor.hi), -0x1p28f), 0x1p28f);   // differences stay in 32 bits
-            const int block_m = limit < 0 ? kNone : static_cast<int>(bound);
-            const int block_m2 = limit < 0 || scales.y == 0.0f ? kNone : block_m + exponent;
+            const float bound = fminf(ceilf(top * factor), 0x1p28f);
+            const int block_m = bound < -0x1p28f ? kNone : static_cast<int>(bound);   // differences stay in 32 bits
+            const int block_m2 = block_m == kNone || v_scale == 0.0f ? kNone : block_m + exponent;
             if (__any(block_m > ref[n] || block_m2 > ref2[n])) {
                 const int next = groups_max(block_m > ref[n] ? block_m : ref[n]);
                 const int next2 = groups_max(block_m2 > ref2[n] ? block_m2 : ref2[n]);
@@ -410,21 +433,17 @@ __global__ __launch_bounds__(kThreads, 2) void kv8_attention_kernel(
             // sum up the denominator.  s - base is small where p is large, and
             // rounded once.
             int e = ref2[n] - ref[n] - 40;
-            e = scales.y == 0.0f || exponent < e ? e : exponent;
+            e = v_scale == 0.0f || exponent < e ? e : exponent;
             const int base = ref2[n] - e;
-            const float share = __builtin_amdgcn_ldexpf(scales.y, kPBits - e);
+            const float share = __builtin_amdgcn_ldexpf(v_scale, kPBits - e);
             const float fbase = static_cast<float>(base);
             float sum = 0.0f;
 #pragma unroll
             for (unsigned b = 0; b < 4u; ++b) {
 #pragma unroll
                 for (unsigned r = 0; r < 4u; r += 2u) {
-                    float x0 = score_power(s[n][b][r], factor, fbase);
-                    float x1 = score_power(s[n][b][r + 1u], factor, fbase);
-                    if (!whole) {
-                        x0 = static_cast<int>(4u * b + r) <= limit ? x0 : 0.0f;
-                        x1 = static_cast<int>(4u * b + r + 1u) <= limit ? x1 : 0.0f;
-                    }
+                    const float x0 = score_power(s[n][b][r], factor, fbase);
+                    const float x1 = score_power(s[n][b][r + 1u], factor, fbase);
                     sum += x0;
                     sum += x1;
                     half2v hi, lo;
@@ -440,12 +459,11 @@ __global__ __launch_bounds__(kThreads, 2) void kv8_attention_kernel(
         if constexpr (TYPE == kKv8E4M3) {
             // Slots behind the tile's last token may hold NaN codes, which a
             // zero p does not silence.
-            const std::int64_t ahead = reach - first;
-            if (__any(vrec0 == nullptr || ahead < 15)) {
-                const int n = vrec0 == nullptr || ahead < 0 ? 0 : ahead > 15 ? 16 : static_cast<int>(ahead) + 1;
+            const int ahead = here ? reach - first : -1;
+            if (__any(ahead < 15)) {
 #pragma unroll
                 for (int w = 0; w < 4; ++w) {
-                    const int bytes = n - 4 * w;
+                    const int bytes = ahead + 1 - 4 * w;
                     const std::uint32_t mask = bytes >= 4 ? 0xffffffffu : bytes <= 0 ? 0u : (1u << (8 * bytes)) - 1u;
 #pragma unroll
                     for (unsigned t = 0; t < D / 16u; ++t) vals[t][w] &= mask;
@@ -454,14 +472,15 @@ __global__ __launch_bounds__(kThreads, 2) void kv8_attention_kernel(
         }
 #pragma unroll
         for (unsigned t = 0; t < D / 16u; ++t) {
-            half8v a0, a1;
-            codes_to_half<TYPE>(vals[t], a0, a1);
+            half8v a[2];
+            codes_to_half<TYPE>(vals[t], a[0], a[1]);
 #pragma unroll
-            for (unsigned n = 0; n < NV; ++n) {
-                o[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, p_hi[n][0], o[n][t], 0, 0, 0);
-                o[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, p_lo[n][0], o[n][t], 0, 0, 0);
-                o[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, p_hi[n][1], o[n][t], 0, 0, 0);
-                o[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, p_lo[n][1], o[n][t], 0, 0, 0);
+            for (unsigned i = 0; i < 4u; ++i) {
+#pragma unroll
+                for (unsigned n = 0; n < NV; ++n) {
+                    const half8v f = i < 2u ? p_lo[n][i] : p_hi[n][i - 2u];
+                    o[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i & 1u], f, o[n][t], 0, 0, 0);
+                }
             }
         }
     }
@@ -517,8 +536,54 @@ __global__ __launch_bounds__(kThreads, 2) void kv8_attention_kernel(
     }
 }
 
-// Joins the splits of a tile's vectors (as many as its furthest position made
-// workgroups of), eight loads in flight.
+// Splits that a tile reaching to `reach` was cut into.
+__device__ __forceinline__ std::uint32_t live_splits(int reach, std::uint64_t max_tokens, std::uint32_t split_chunks) {
+    const int most = static_cast<int>(max_tokens) - 1;
+    reach = reach < most ? reach : most;
+    const std::uint32_t chunks = reach < 0 ? 0u : static_cast<std::uint32_t>(reach) / kChunkTokens + 1u;
+    return (chunks + split_chunks - 1u) / split_chunks;
+}
+
+// Dims 4 d4 .. + 3 of a vector from its splits' partials, eight loads in flight.
+template <unsigned D>
+__device__ __forceinline__ float4v join_splits(const float* __restrict__ base, std::uint32_t live, unsigned d4, int& ref,
+                                               float& total) {
+    constexpr unsigned kBatch = 8;
+    ref = kNone;
+    total = 0.0f;
+    int ref2 = kNone;
+    float4v acc = {0.f, 0.f, 0.f, 0.f};
+    for (std::uint32_t s0 = 0; s0 < live; s0 += kBatch) {
+        float4v head[kBatch], sums[kBatch];
+#pragma unroll
+        for (unsigned j = 0; j < kBatch; ++j) {
+            const std::uint32_t at = (s0 + j < live ? s0 + j : live - 1u) * (D + kStat);
+            head[j] = *reinterpret_cast<const float4v*>(base + at);
+            sums[j] = *reinterpret_cast<const float4v*>(base + at + kStat + 4u * d4);
+        }
+#pragma unroll
+        for (unsigned j = 0; j < kBatch; ++j) {
+            if (s0 + j >= live) continue;
+            const int a = __float_as_int(head[j][0]), a2 = __float_as_int(head[j][1]);
+            const int next = a > ref ? a : ref, next2 = a2 > ref2 ? a2 : ref2;
+            total = __builtin_amdgcn_ldexpf(total, ref - next) + __builtin_amdgcn_ldexpf(head[j][2], a - next);
+#pragma unroll
+            for (unsigned r = 0; r < 4u; ++r) {
+                acc[r] = __builtin_amdgcn_ldexpf(acc[r], ref2 - next2) + __builtin_amdgcn_ldexpf(sums[j][r], a2 - next2);
+            }
+            ref = next;
+            ref2 = next2;
+        }
+    }
+    float4v y;
+#pragma unroll
+    for (unsigned r = 0; r < 4u; ++r) {
+        y[r] = total == 0.0f ? 0.0f : __builtin_amdgcn_ldexpf(acc[r] / total, ref2 - kPBits - ref);
+    }
+    return y;
+}
+
+// Joins the splits of a tile's vectors.
 template <unsigned D, unsigned NV, bool RUNS>
 __global__ __launch_bounds__(kThreads) void kv8_merge_kernel(
     const std::int32_t* __restrict__ positions, std::uint32_t m, std::uint32_t q_heads, std::uint32_t kv_heads,
@@ -526,7 +591,6 @@ __global__ __launch_bounds__(kThreads) void kv8_merge_kernel(
     std::uint32_t split_chunks, std::uint32_t splits, const float* __restrict__ partials, float2* __restrict__ stats,
     float* __restrict__ out) {
     constexpr unsigned kTile = kVectors * NV;
-    constexpr unsigned kBatch = 8;
     const std::uint32_t group = q_heads / kv_heads, parts = (group + kTile - 1u) / kTile;
     const std::uint32_t kvh = blockIdx.x / parts, part = blockIdx.x % parts;
     Tile tile{blockIdx.y, 1u, 0u, 0u};
@@ -539,61 +603,40 @@ __global__ __launch_bounds__(kThreads) void kv8_merge_kernel(
         const int p = positions[tile.row + r];
         reach = p > reach ? p : reach;
     }
-    const int most = static_cast<int>(max_tokens) - 1;
-    reach = reach < most ? reach : most;
-    const std::uint32_t chunks = reach < 0 ? 0u : static_cast<std::uint32_t>(reach) / kChunkTokens + 1u;
-    const std::uint32_t live = (chunks + split_chunks - 1u) / split_chunks;
+    const std::uint32_t live = live_splits(reach, max_tokens, split_chunks);
     if (live <= 1u) return;   // the attention kernel wrote this tile
     for (unsigned idx = threadIdx.x; idx < tile.rows * tile.heads * (D / 4u); idx += kThreads) {
         const unsigned v = idx / (D / 4u), d4 = idx % (D / 4u);
         const std::uint64_t vector =
             static_cast<std::uint64_t>(tile.row + v / tile.heads) * q_heads + tile.head + v % tile.heads;
-        const float* const base = partials + vector * splits * (D + kStat);
-        int ref = kNone, ref2 = kNone;
-        float total = 0.0f;
-        float4v acc = {0.f, 0.f, 0.f, 0.f};
-        for (std::uint32_t s0 = 0; s0 < live; s0 += kBatch) {
-            float4v head[kBatch], part_sum[kBatch];
-#pragma unroll
-            for (unsigned j = 0; j < kBatch; ++j) {
-                const std::uint32_t at = (s0 + j < live ? s0 + j : live - 1u) * (D + kStat);
-                head[j] = *reinterpret_cast<const float4v*>(base + at);
-                part_sum[j] = *reinterpret_cast<const float4v*>(base + at + kStat + 4u * d4);
-            }
-#pragma unroll
-            for (unsigned j = 0; j < kBatch; ++j) {
-                if (s0 + j >= live) continue;
-                const int a = __float_as_int(head[j][0]), a2 = __float_as_int(head[j][1]);
-                const int next = a > ref ? a : ref, next2 = a2 > ref2 ? a2 : ref2;
-                total = __builtin_amdgcn_ldexpf(total, ref - next) + __builtin_amdgcn_ldexpf(head[j][2], a - next);
-#pragma unroll
-                for (unsigned r = 0; r < 4u; ++r) {
-                    acc[r] = __builtin_amdgcn_ldexpf(acc[r], ref2 - next2) + __builtin_amdgcn_ldexpf(part_sum[j][r], a2 - next2);
-                }
-                ref = next;
-                ref2 = next2;
-            }
-        }
-        float4v y;
-#pragma unroll
-        for (unsigned r = 0; r < 4u; ++r) {
-            y[r] = total == 0.0f ? 0.0f : __builtin_amdgcn_ldexpf(acc[r] / total, ref2 - kPBits - ref);
-        }
+        int ref;
+        float total;
+        const float4v y = join_splits<D>(partials + vector * splits * (D + kStat), live, d4, ref, total);
         *reinterpret_cast<float4v*>(out + vector * D + 4u * d4) = y;
         if (stats && d4 == 0u) stats[vector] = make_float2(static_cast<float>(ref), total == 0.0f ? 0.0f : 1.0f / total);
     }
 }
+
 // The weights a run's rows give one chunk of tokens: the scores again, by the
-// same instructions as in the attention, and p from the rows' statistics.
-// A chunk of a (run, KV head) has one wave, which adds its sums with one
-// atomic a token: a page that two runs share loses nothing, and elsewhere the
-// single addition leaves one order.
-template <int TYPE, unsigned D>
+// same instructions as in the attention, and p from the rows' statistics
+// (M and 1 / l).  A chunk of a (run, KV head) is one wave's, or with SHARED,
+// for runs of many vectors, the four waves' of a workgroup, which take the
+// vectors in turn and add up in LDS.  It adds with one atomic a token: a page
+// that two runs share loses nothing, and elsewhere a single addition leaves
+// one order.  Reading K again takes half of the attention's bytes; keeping
+// the scores would take 4 bytes a vector and token, written and read.
+//
+// MERGE, for tiles of single rows that were split: the grid's first column
+// joins the splits of a run's rows, and the others take the statistics from
+// the partials themselves, so that one launch follows the attention.
+template <int TYPE, unsigned D, bool SHARED, bool MERGE>
 __global__ __launch_bounds__(kThreads) void kv8_weights_kernel(
     Kv8Geometry g, const float* __restrict__ qkv, std::uint64_t stride, std::uint32_t m,
     const std::int32_t* __restrict__ positions, const std::int32_t* __restrict__ tables, std::uint32_t layer,
-    std::uint32_t q_heads, const std::int32_t* __restrict__ run_starts, std::uint64_t max_tokens, float2 score_scale,
-    const float2* __restrict__ stats, bool add) {
+    std::uint32_t q_heads, const std::int32_t* __restrict__ run_starts, std::uint64_t max_tokens, float score_scale,
+    const float2* __restrict__ stats, bool add, std::uint32_t split_chunks, std::uint32_t splits,
+    const float* __restrict__ partials, float* __restrict__ out) {
+    __shared__ float shared_sum[SHARED ? kWaves : 1u][kChunkTokens];
     const unsigned tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, grp = lane >> 4, col = lane & 15u;
     const std::uint32_t kvh = blockIdx.y, run = blockIdx.z;
     std::int64_t begin = run, end = static_cast<std::int64_t>(run) + 1;
@@ -604,65 +647,108 @@ __global__ __launch_bounds__(kThreads) void kv8_weights_kernel(
     begin = begin < 0 ? 0 : begin;
     end = end > static_cast<std::int64_t>(m) ? static_cast<std::int64_t>(m) : end;
     if (begin >= end) return;
-    const std::uint32_t chunk = blockIdx.x * kWaves + wave;
-    const std::int64_t token0 = static_cast<std::int64_t>(chunk) * kChunkTokens;
-    const std::int32_t* const table = tables + static_cast<std::uint64_t>(begin) * g.max_pages;
     const std::uint32_t group = q_heads / g.kv_heads;
+    const std::uint32_t vectors = static_cast<std::uint32_t>(end - begin) * group;
+    const std::uint32_t row0 = static_cast<std::uint32_t>(begin), head0 = kvh * group;
+    if (MERGE && blockIdx.x == 0u) {
+        for (unsigned idx = tid; idx < vectors * (D / 4u); idx += kThreads) {
+            const unsigned v = idx / (D / 4u), d4 = idx % (D / 4u);
+            const std::uint32_t r = row0 + v / group;
+            const std::uint64_t vector = static_cast<std::uint64_t>(r) * q_heads + head0 + v % group;
+            const std::uint32_t live = live_splits(positions[r], max_tokens, split_chunks);
+            if (live <= 1u) continue;   // the attention kernel wrote this row
+            int ref;
+            float total;
+            *reinterpret_cast<float4v*>(out + vector * D + 4u * d4) =
+                join_splits<D>(partials + vector * splits * (D + kStat), live, d4, ref, total);
+        }
+        return;
+    }
+    const std::uint32_t column = blockIdx.x - (MERGE ? 1u : 0u);
+    const std::uint32_t chunk = SHARED ? column : column * kWaves + wave;
+    const int token0 = static_cast<int>(chunk * kChunkTokens);
+    const std::int32_t* const table = tables + static_cast<std::uint64_t>(row0) * g.max_pages;
     // Tokens past the run's last position (or max_tokens) are not held.
-    std::int64_t last = -1;
+    const int most = static_cast<int>(max_tokens) - 1;
+    int last = -1;
     for (std::int64_t r = begin + lane; r < end; r += 64) last = positions[r] > last ? positions[r] : last;
     for (int off = 32; off > 0; off >>= 1) {
-        const std::int64_t o = __shfl_xor(static_cast<int>(last), off);
+        const int o = __shfl_xor(last, off);
         last = o > last ? o : last;
     }
-    if (last >= static_cast<std::int64_t>(max_tokens)) last = static_cast<std::int64_t>(max_tokens) - 1;
-    if (token0 > last) return;
-    const unsigned char* const krec0 = kv8_record(g, table, layer, kvh, chunk * kChunkBlocks + (col >> 2));
-    unsigned char* const vrec0 = kv8_record(g, table, layer, kvh, chunk * kChunkBlocks + grp);
+    last = last < most ? last : most;
+    if (token0 > last) return;   // all of a workgroup's waves, where they share a chunk
+    const Kv8Byte* const none = (const Kv8Byte*)g_no_record;
+    const Kv8Byte* const krec = (const Kv8Byte*)kv8_record(g, table, layer, kvh, chunk * kChunkBlocks + (col >> 2));
+    unsigned char* const vrec = kv8_record(g, table, layer, kvh, chunk * kChunkBlocks + grp);
     KeyCodes<D> keys;
-    load_keys<D>(krec0 ? krec0 : g_no_record, lane, keys);
-    const float k_scale = *reinterpret_cast<const float*>(vrec0 ? vrec0 : g_no_record);
-    const std::int64_t first = token0 + grp * kKv8Block;
-    float sum[4][4] = {};
-    const std::int64_t vectors = (end - begin) * group;
-    for (std::int64_t v0 = 0; v0 < vectors; v0 += kVectors) {
-        const std::int64_t v = v0 + col;
+    load_keys<D>(krec ? krec : none, lane, keys);
+    const float k_scale = load_scales(vrec ? (const Kv8Byte*)vrec : none).x;
+    const int first = token0 + static_cast<int>(grp * kKv8Block);
+    float sum[16] = {};
+    for (std::uint32_t v0 = SHARED ? wave * kVectors : 0u; v0 < vectors; v0 += (SHARED ? kWaves : 1u) * kVectors) {
+        const std::uint32_t v = v0 + col;
         const bool active = v < vectors;
-        const std::int64_t r = begin + (active ? v / group : 0);
-        const std::uint64_t head = static_cast<std::uint64_t>(kvh) * group + (active ? v % group : 0);
-        std::int64_t upto = active ? positions[r] : -1;
-        if (upto >= static_cast<std::int64_t>(max_tokens)) upto = static_cast<std::int64_t>(max_tokens) - 1;
+        const std::uint32_t r = row0 + (active ? v / group : 0u);
+        const std::uint64_t vector = static_cast<std::uint64_t>(r) * q_heads + head0 + (active ? v % group : 0u);
+        const int position = positions[r];
+        int upto = active ? position : -1;
+        upto = upto < most ? upto : most;
         if (!__any(upto >= token0)) continue;
         QueryFragments<D> q;
-        load_query<D>(active ? qkv + static_cast<std::uint64_t>(r) * stride + head * D : nullptr, grp, q);
-        const float2 st = active ? stats[static_cast<std::uint64_t>(r) * q_heads + head] : make_float2(0.f, 0.f);
+        load_query<D>(active ? qkv + static_cast<std::uint64_t>(r) * stride + (vector - static_cast<std::uint64_t>(r) * q_heads) * D
+                             : nullptr,
+                      grp, q);
+        float base, share;   // M and 1 / l
+        const std::uint32_t live = MERGE ? live_splits(position, max_tokens, split_chunks) : 1u;
+        if (MERGE && live > 1u) {
+            int ref = kNone;
+            float total = 0.0f;
+            for (std::uint32_t s = 0; s < live; ++s) {
+                const float4v head = *reinterpret_cast<const float4v*>(partials + (vector * splits + s) * (D + kStat));
+                const int a = __float_as_int(head[0]), next = a > ref ? a : ref;
+                total = __builtin_amdgcn_ldexpf(total, ref - next) + __builtin_amdgcn_ldexpf(head[2], a - next);
+                ref = next;
+            }
+            base = static_cast<float>(ref);
+            share = total == 0.0f ? 0.0f : 1.0f / total;
+        } else {
+            const float2 st = stats[vector];
+            base = st.x;
+            share = st.y;
+        }
         float4v s[4];
         chunk_scores<TYPE, D>(keys, q, s);
-        const Factor factor = score_factor(q.undo, score_scale, k_scale);
-        const int limit = vrec0 == nullptr || upto < first ? -1 : upto - first > 15 ? 15 : static_cast<int>(upto - first);
+        const float factor = score_factor(q.undo, score_scale, k_scale);
+        const int limit = vrec == nullptr ? -1 : upto - first;
 #pragma unroll
-        for (unsigned b = 0; b < 4u; ++b) {
-#pragma unroll
-            for (unsigned i = 0; i < 4u; ++i) {
-                const float p = score_power(s[b][i], factor, st.x) * st.y;
-                sum[b][i] += static_cast<int>(4u * b + i) <= limit ? p : 0.0f;
-            }
+        for (unsigned t = 0; t < 16u; ++t) {
+            const float p = score_power(s[t >> 2][t & 3u], factor, base) * share;
+            sum[t] += static_cast<int>(t) <= limit ? p : 0.0f;
         }
     }
+    // Over the 16 vectors, halving what a lane keeps: lane col ends with token
+    // col of its block.
 #pragma unroll
-    for (unsigned b = 0; b < 4u; ++b) {
+    for (unsigned w = 8u; w >= 1u; w >>= 1) {
+        const bool upper = (col & w) != 0u;
 #pragma unroll
-        for (unsigned i = 0; i < 4u; ++i) {
-#pragma unroll
-            for (int off = 1; off < 16; off <<= 1) sum[b][i] += __shfl_xor(sum[b][i], off);
+        for (unsigned t = 0; t < w; ++t) {
+            const float keep = upper ? sum[t + w] : sum[t], give = upper ? sum[t] : sum[t + w];
+            sum[t] = keep + __shfl_xor(give, w);
         }
     }
-    if (vrec0 == nullptr) return;
-    float mine = 0.0f;   // lane (col, grp): token col of block grp
+    float mine = sum[0];
+    if constexpr (SHARED) {
+        shared_sum[wave][lane] = mine;
+        __syncthreads();
+        if (wave != 0u) return;
+        mine = 0.0f;
 #pragma unroll
-    for (unsigned t = 0; t < 16u; ++t) mine = col == t ? sum[t >> 2][t & 3u] : mine;
-    if (first + col > last) return;
-    float* const at = reinterpret_cast<float*>(vrec0 + kKv8Weights) + col;
+        for (unsigned w = 0; w < kWaves; ++w) mine += shared_sum[w][lane];
+    }
+    if (vrec == nullptr || first + static_cast<int>(col) > last) return;
+    float* const at = reinterpret_cast<float*>(vrec + kKv8Weights) + col;
     if (add) {
         atomicAdd(at, mine);
     } else {
@@ -703,42 +789,42 @@ std::uint64_t kv8_attention_scratch(const Kv8Shape& shape, std::uint32_t m, std:
 
 namespace {
 
-template <int TYPE, unsigned D, unsigned NV, bool RUNS>
-void launch_tiles(const Kv8Geometry& g, const float* qkv, std::uint64_t stride, std::uint32_t m,
-                  const std::int32_t* positions, const std::int32_t* tables, std::uint32_t layer, std::uint32_t q_heads,
-                  const std::int32_t* run_starts, std::uint32_t runs, std::uint64_t max_tokens, const Kv8Shape& shape,
-                  float2 scale, float* partials, float2* stats, float* out, hipStream_t stream) {
-    hipLaunchKernelGGL((kv8_attention_kernel<TYPE, D, NV, RUNS>), dim3(shape.tile_heads, shape.tiles, shape.splits),
-                       dim3(kThreads), 0, stream, g, qkv, stride, m, positions, tables, layer, q_heads, run_starts, runs,
-                       shape.tile_rows, max_tokens, shape.split_chunks, scale, partials, stats, out);
-    if (shape.splits > 1u) {
-        hipLaunchKernelGGL((kv8_merge_kernel<D, NV, RUNS>), dim3(shape.tile_heads, shape.tiles), dim3(kThreads), 0,
-                           stream, positions, m, q_heads, g.kv_heads, run_starts, runs, shape.tile_rows, max_tokens,
-                           shape.split_chunks, shape.splits, partials, stats, out);
-    }
-}
-
 template <int TYPE, unsigned D>
 void launch_typed(const Kv8Geometry& g, const float* qkv, std::uint64_t stride, std::uint32_t m,
                   const std::int32_t* positions, const std::int32_t* tables, std::uint32_t layer, std::uint32_t q_heads,
                   const std::int32_t* run_starts, std::uint32_t runs, std::uint64_t max_tokens, int weights,
                   const Kv8Shape& shape, float* partials, float2* stats, float* out, hipStream_t stream) {
     // Scores in powers of two: s log2(e) = (q . k) * log2(e) / sqrt(D).
-    const double exact = 1.4426950408889634 / __builtin_sqrt(static_cast<double>(D));
-    const float2 scale = make_float2(static_cast<float>(exact), static_cast<float>(exact - static_cast<float>(exact)));
-    if (shape.tile_rows != 0u) {
-        launch_tiles<TYPE, D, kPromptTiles, true>(g, qkv, stride, m, positions, tables, layer, q_heads, run_starts, runs,
-                                                  max_tokens, shape, scale, partials, stats, out, stream);
+    const float scale = static_cast<float>(1.4426950408889634 / __builtin_sqrt(static_cast<double>(D)));
+    const dim3 grid(shape.tile_heads, shape.tiles, shape.splits), merge_grid(shape.tile_heads, shape.tiles);
+    const bool split = shape.splits > 1u, by_run = shape.tile_rows != 0u;
+#define AIR_KV8_ATTENTION(NV, RUNS)                                                                                  \
+    hipLaunchKernelGGL((kv8_attention_kernel<TYPE, D, NV, RUNS>), grid, dim3(kThreads), 0, stream, g, qkv, stride, m, \
+                       positions, tables, layer, q_heads, run_starts, runs, shape.tile_rows, max_tokens,             \
+                       shape.split_chunks, scale, partials, stats, out)
+#define AIR_KV8_MERGE(NV, RUNS)                                                                                      \
+    hipLaunchKernelGGL((kv8_merge_kernel<D, NV, RUNS>), merge_grid, dim3(kThreads), 0, stream, positions, m, q_heads, \
+                       g.kv_heads, run_starts, runs, shape.tile_rows, max_tokens, shape.split_chunks, shape.splits,  \
+                       partials, stats, out)
+#define AIR_KV8_WEIGHTS(SHARED, MERGE, COLUMNS)                                                                      \
+    hipLaunchKernelGGL((kv8_weights_kernel<TYPE, D, SHARED, MERGE>), dim3(COLUMNS, g.kv_heads, run_starts ? runs : m), \
+                       dim3(kThreads), 0, stream, g, qkv, stride, m, positions, tables, layer, q_heads, run_starts,  \
+                       max_tokens, scale, stats, weights == 1, shape.split_chunks, shape.splits, partials, out)
+    const std::uint32_t chunks = static_cast<std::uint32_t>((max_tokens + kChunkTokens - 1u) / kChunkTokens);
+    const std::uint32_t columns = (chunks + kWaves - 1u) / kWaves;
+    if (by_run) {
+        AIR_KV8_ATTENTION(kPromptTiles, true);
+        if (split) AIR_KV8_MERGE(kPromptTiles, true);
+        if (weights) AIR_KV8_WEIGHTS(true, false, chunks);
     } else {
-        launch_tiles<TYPE, D, 1u, false>(g, qkv, stride, m, positions, tables, layer, q_heads, nullptr, 0u, max_tokens,
-                                         shape, scale, partials, stats, out, stream);
+        AIR_KV8_ATTENTION(1u, false);
+        if (weights && split) AIR_KV8_WEIGHTS(false, true, columns + 1u);
+        else if (weights) AIR_KV8_WEIGHTS(false, false, columns);
+        else if (split) AIR_KV8_MERGE(1u, false);
     }
-    if (weights) {
-        const std::uint64_t chunks = (max_tokens + kChunkTokens - 1u) / kChunkTokens;
-        const dim3 grid(static_cast<unsigned>((chunks + kWaves - 1u) / kWaves), g.kv_heads, run_starts ? runs : m);
-        hipLaunchKernelGGL((kv8_weights_kernel<TYPE, D>), grid, dim3(kThreads), 0, stream, g, qkv, stride, m, positions,
-                           tables, layer, q_heads, run_starts, max_tokens, scale, stats, weights == 1);
-    }
+#undef AIR_KV8_ATTENTION
+#undef AIR_KV8_MERGE
+#undef AIR_KV8_WEIGHTS
 }
 
 } // namespace

@@ -45,60 +45,130 @@ __device__ __forceinline__ float nan_f32() { return __builtin_nanf(""); }
 // K: (token, 16 dims), one 16-byte store each; threads [D, 2 D) own V: one
 // dim of all 16 tokens.  The magnitudes meet as the bit patterns of |x|,
 // whose unsigned order puts infinities and NaN above every finite value.
+// Latency bounds it (a decode step stores 2 KB a row): the block's codes and
+// scale and the row's own values are asked for before the other rows are
+// looked through, and in a decode step nothing else has to be read.
 template <int TYPE, unsigned D>
 __global__ __launch_bounds__(2 * D) void kv8_append_kernel(Kv8Geometry g, const float* __restrict__ qkv,
                                                            std::uint64_t stride, std::uint64_t q_width,
                                                            std::uint32_t m, const std::int32_t* __restrict__ positions,
                                                            const std::int32_t* __restrict__ tables,
-                                                           std::uint32_t layer) {
+                                                           std::uint32_t layer, bool aligned) {
 #pragma clang fp contract(off)
+    constexpr unsigned kThreads = 2 * D;
+    constexpr unsigned kAtOnce = 4;       // rows a thread looks through at a time
     __shared__ int winner[kKv8Block];
-    __shared__ int earlier;
-    __shared__ std::uint32_t wave_top[2 * D / 64];
+    __shared__ int earlier, named;
+    __shared__ std::uint32_t wave_top[kThreads / 64];
     const std::uint32_t r = blockIdx.x, head = blockIdx.y;
     const unsigned tid = threadIdx.x;
-    const auto record_of = [&](std::uint32_t row, std::int32_t pos) __attribute__((always_inline)) {
-        return pos < 0 ? nullptr
-                       : kv8_record(g, tables + static_cast<std::uint64_t>(row) * g.max_pages, layer, head,
-                                    static_cast<std::uint32_t>(pos) / kKv8Block);
-    };
-    unsigned char* const rec = record_of(r, positions[r]);
-    if (rec == nullptr) return;
-    // In a prompt the row before names the same block for 15 of 16 rows.
-    if (r > 0u && record_of(r - 1u, positions[r - 1u]) == rec) return;
-    if (tid < kKv8Block) winner[tid] = -1;
-    if (tid == 0u) earlier = 0;
-    __syncthreads();
-    for (std::uint32_t o = tid; o < m; o += 2u * D) {
-        const std::int32_t pos = positions[o];
-        if (record_of(o, pos) != rec) continue;
-        if (o < r) {
-            earlier = 1;
+    const bool value = tid >= D;
+    const unsigned part = value ? tid - D : tid;
+    const unsigned token = part / (D / 16u), chunk = part % (D / 16u);   // of a K thread
+    const float* const base = qkv + q_width + (value ? static_cast<std::uint64_t>(g.kv_heads) * D : 0u) +
+                              static_cast<std::uint64_t>(head) * D;
+    // What this thread stores of row `row` in its token (K: 16 dims; V: one).
+    const auto load_row = [&](std::uint32_t row, float* x) __attribute__((always_inline)) {
+        const float* const src = base + static_cast<std::uint64_t>(row) * stride + chunk * 16u;
+        if (aligned) {
+#pragma unroll
+            for (unsigned i = 0; i < 4u; ++i) {
+                const float4 f = reinterpret_cast<const float4*>(src)[i];
+                x[4u * i] = f.x;
+                x[4u * i + 1u] = f.y;
+                x[4u * i + 2u] = f.z;
+                x[4u * i + 3u] = f.w;
+            }
         } else {
-            atomicMax(&winner[static_cast<std::uint32_t>(pos) % kKv8Block], static_cast<int>(o));
+#pragma unroll
+            for (unsigned i = 0; i < 16u; ++i) x[i] = src[i];
+        }
+    };
+    const auto page_of = [&](std::uint32_t row, std::int32_t pos, std::uint32_t& slot) __attribute__((always_inline)) {
+        slot = pos < 0 ? 0u : kv8_slot(g, static_cast<std::uint32_t>(pos) / kKv8Block);
+        return pos < 0 || slot >= g.max_pages ? -1 : tables[static_cast<std::uint64_t>(row) * g.max_pages + slot];
+    };
+    // Two rows name one block if they name one page and its same block.
+    const auto place_of = [&](std::int32_t pos, std::uint32_t slot) __attribute__((always_inline)) {
+        return static_cast<std::uint32_t>(pos) / kKv8Block - slot * g.page_blocks;
+    };
+    const std::int32_t pos = positions[r], pos_before = r > 0u ? positions[r - 1u] : -1;
+    std::uint32_t slot, slot_before;
+    const std::int32_t page = page_of(r, pos, slot), page_before = page_of(r > 0u ? r - 1u : 0u, pos_before, slot_before);
+    if (page < 0) return;
+    const std::uint32_t place = place_of(pos, slot);
+    // In a prompt the row before names the same block for 15 of 16 rows.
+    if (page_before == page && place_of(pos_before, slot_before) == place) return;
+    unsigned char* const rec = (unsigned char*)kv8_record_in(g, page, slot, layer, head,
+                                                             static_cast<std::uint32_t>(pos) / kKv8Block);
+    if (rec == nullptr) return;
+    const unsigned at = value ? kv8_v_offset(D, 0u, part) : kv8_k_offset(D, token, chunk * 16u);
+    u32x4* const codes_at = reinterpret_cast<u32x4*>(rec + at);
+    u32x4 codes = *codes_at;
+    float* const scale_at = reinterpret_cast<float*>(rec) + (value ? 1 : 0);
+    const float old_scale = *scale_at;
+    float x[16];
+    if (value) {
+        x[0] = base[static_cast<std::uint64_t>(r) * stride + part];
+    } else {
+        load_row(r, x);
+    }
+    if (tid < kKv8Block) winner[tid] = -1;
+    if (tid == 0u) earlier = named = 0;
+    __syncthreads();
+    for (std::uint32_t o0 = tid; o0 < m; o0 += kAtOnce * kThreads) {
+        std::int32_t their_pos[kAtOnce], their_page[kAtOnce];
+        std::uint32_t their_slot[kAtOnce];
+#pragma unroll
+        for (unsigned j = 0; j < kAtOnce; ++j) {
+            const std::uint32_t o = o0 + j * kThreads;
+            their_pos[j] = o < m ? positions[o] : -1;
+        }
+#pragma unroll
+        for (unsigned j = 0; j < kAtOnce; ++j) {
+            const std::uint32_t o = o0 + j * kThreads;
+            their_page[j] = page_of(o < m ? o : 0u, their_pos[j], their_slot[j]);
+        }
+#pragma unroll
+        for (unsigned j = 0; j < kAtOnce; ++j) {
+            const std::uint32_t o = o0 + j * kThreads;
+            if (their_page[j] != page || place_of(their_pos[j], their_slot[j]) != place) continue;
+            if (o < r) {
+                earlier = 1;
+            } else {
+                atomicMax(&winner[static_cast<std::uint32_t>(their_pos[j]) % kKv8Block], static_cast<int>(o));
+                if (o > r) named = 1;
+            }
         }
     }
     __syncthreads();
     if (earlier != 0) return;
     unsigned first = 0u;
     while (winner[first] < 0) ++first;   // row r itself is in
+    const unsigned own = static_cast<std::uint32_t>(pos) % kKv8Block;
 
-    const bool value = tid >= D;
-    const unsigned part = value ? tid - D : tid;
-    const unsigned token = part / (D / 16u), chunk = part % (D / 16u);   // of a K thread
-    float x[16];
+    if (value) {
+        const float mine = x[0];
+#pragma unroll
+        for (unsigned i = 0; i < 16u; ++i) {
+            const int row = winner[i];
+            x[i] = i == own && named == 0 ? mine
+                   : row >= 0 && named != 0 ? base[static_cast<std::uint64_t>(row) * stride + part] : 0.0f;
+        }
+    } else {
+        const int row = winner[token];
+        if (row >= 0 && static_cast<std::uint32_t>(row) != r) load_row(static_cast<std::uint32_t>(row), x);
+        if (row < 0) {
+#pragma unroll
+            for (unsigned i = 0; i < 16u; ++i) x[i] = 0.0f;
+        }
+    }
     std::uint32_t top = 0u;
-    const float* const base = qkv + q_width + (value ? static_cast<std::uint64_t>(g.kv_heads) * D : 0u) +
-                              static_cast<std::uint64_t>(head) * D;
 #pragma unroll
     for (unsigned i = 0; i < 16u; ++i) {
-        const int row = winner[value ? i : token];
-        x[i] = row >= 0 ? base[static_cast<std::uint64_t>(row) * stride + (value ? part : chunk * 16u + i)] : 0.0f;
         const std::uint32_t mag = __float_as_uint(x[i]) & 0x7fffffffu;
         top = mag > top ? mag : top;
     }
-    float* const scale_at = reinterpret_cast<float*>(rec) + (value ? 1 : 0);
-    const float old_scale = *scale_at;
     top = wave_max_u32(top);
     if ((tid & 63u) == 0u) wave_top[tid >> 6] = top;
     __syncthreads();   // also: every thread has the old scale before it is replaced
@@ -114,9 +184,6 @@ __global__ __launch_bounds__(2 * D) void kv8_append_kernel(Kv8Geometry g, const 
     const bool grows = held && old_scale == old_scale && !(need <= old_scale);
     const float scale = held && !grows ? old_scale : need;
     const float ratio = grows && scale > 0.0f ? old_scale / scale : 1.0f;
-    const unsigned at = value ? kv8_v_offset(D, 0u, part) : kv8_k_offset(D, token, chunk * 16u);
-    u32x4* const codes_at = reinterpret_cast<u32x4*>(rec + at);
-    u32x4 codes = *codes_at;
 #pragma unroll
     for (unsigned i = 0; i < 16u; ++i) {
         const unsigned t = value ? i : token;
@@ -138,15 +205,17 @@ __global__ __launch_bounds__(2 * D) void kv8_append_kernel(Kv8Geometry g, const 
 }
 
 // Tokens starts[i] .. starts[i] + lengths[i] - 1 of every sequence as f32
-// rows; one workgroup per (block, KV head, sequence and layer), a thread per
-// four dims of a token.
-template <int TYPE>
-__global__ __launch_bounds__(256) void kv8_read_kernel(Kv8Geometry g, std::uint32_t seqs,
-                                                       const std::int32_t* __restrict__ starts,
-                                                       const std::int32_t* __restrict__ lengths,
-                                                       const std::int32_t* __restrict__ tables, std::uint32_t layer,
-                                                       std::uint64_t max_tokens, float* __restrict__ k,
-                                                       float* __restrict__ v, float* __restrict__ weights) {
+// rows; one workgroup per (block, KV head, sequence and layer).  Half of the
+// threads read K, half V, each four tokens of four dims: four dwords of codes
+// and four 16-byte stores, a token's stores of a wave being contiguous.
+template <int TYPE, unsigned D>
+__global__ __launch_bounds__(2 * D) void kv8_read_kernel(Kv8Geometry g, std::uint32_t seqs,
+                                                         const std::int32_t* __restrict__ starts,
+                                                         const std::int32_t* __restrict__ lengths,
+                                                         const std::int32_t* __restrict__ tables, std::uint32_t layer,
+                                                         std::uint64_t max_tokens, float* __restrict__ k,
+                                                         float* __restrict__ v, float* __restrict__ weights,
+                                                         bool aligned) {
     const std::uint32_t head = blockIdx.y;
     const std::uint32_t seq = blockIdx.z % seqs, l = blockIdx.z / seqs;
     const std::int64_t start = starts ? starts[seq] : 0;
@@ -159,24 +228,37 @@ __global__ __launch_bounds__(256) void kv8_read_kernel(Kv8Geometry g, std::uint3
     const unsigned char* const rec = kv8_record(g, tables + static_cast<std::uint64_t>(seq) * g.max_pages, layer + l,
                                                 head, static_cast<std::uint32_t>(block));
     if (rec == nullptr) return;
-    const unsigned d = g.head_dim, quads = d / 4u;
+    const bool value = threadIdx.x >= D;
+    const unsigned part = value ? threadIdx.x - D : threadIdx.x;
+    const unsigned token0 = part / (D / 4u) * 4u, dim = part % (D / 4u) * 4u;
     const std::uint64_t row0 = (static_cast<std::uint64_t>(l) * seqs + seq) * max_tokens;
-    const std::uint64_t width = static_cast<std::uint64_t>(g.kv_heads) * d;
-    const float ks = reinterpret_cast<const float*>(rec)[0], vs = reinterpret_cast<const float*>(rec)[1];
-    for (unsigned idx = threadIdx.x; idx < kKv8Block * quads; idx += 256u) {
-        const unsigned token = idx / quads, dim = idx % quads * 4u;
-        const std::int64_t t = base + token;
-        if (t < start || t >= start + count) continue;
-        const std::uint64_t at = (row0 + static_cast<std::uint64_t>(t - start)) * width +
-                                 static_cast<std::uint64_t>(head) * d + dim;
-        if (k) {
-            const std::uint32_t c = *reinterpret_cast<const std::uint32_t*>(rec + kv8_k_offset(d, token, dim));
+    const std::uint64_t width = static_cast<std::uint64_t>(g.kv_heads) * D;
+    float* const dst = value ? v : k;
+    if (dst != nullptr) {
+        const float scale = reinterpret_cast<const float*>(rec)[value ? 1 : 0];
+        std::uint32_t c[4];   // of K a token's four dims, of V a dim's four tokens
 #pragma unroll
-            for (unsigned i = 0; i < 4u; ++i) k[at + i] = kv8_value<TYPE>(c >> (8u * i)) * ks;
+        for (unsigned i = 0; i < 4u; ++i) {
+            c[i] = *reinterpret_cast<const std::uint32_t*>(
+                rec + (value ? kv8_v_offset(D, token0, dim + i) : kv8_k_offset(D, token0 + i, dim)));
         }
-        if (v) {
 #pragma unroll
-            for (unsigned i = 0; i < 4u; ++i) v[at + i] = kv8_value<TYPE>(rec[kv8_v_offset(d, token, dim + i)]) * vs;
+        for (unsigned t = 0; t < 4u; ++t) {
+            const std::int64_t at_token = base + token0 + t;
+            if (at_token < start || at_token >= start + count) continue;
+            float x[4];
+#pragma unroll
+            for (unsigned i = 0; i < 4u; ++i) {
+                x[i] = kv8_value<TYPE>(value ? c[i] >> (8u * t) : c[t] >> (8u * i)) * scale;
+            }
+            float* const to = dst + (row0 + static_cast<std::uint64_t>(at_token - start)) * width +
+                              static_cast<std::uint64_t>(head) * D + dim;
+            if (aligned) {
+                *reinterpret_cast<float4*>(to) = make_float4(x[0], x[1], x[2], x[3]);
+            } else {
+#pragma unroll
+                for (unsigned i = 0; i < 4u; ++i) to[i] = x[i];
+            }
         }
     }
     if (weights && threadIdx.x < kKv8Block) {
@@ -188,9 +270,32 @@ __global__ __launch_bounds__(256) void kv8_read_kernel(Kv8Geometry g, std::uint3
     }
 }
 
+// The weights alone: a thread per (token, KV head), the heads of a token
+// side by side as they are stored.
+__global__ __launch_bounds__(256) void kv8_read_weights_kernel(Kv8Geometry g, std::uint32_t seqs,
+                                                               const std::int32_t* __restrict__ starts,
+                                                               const std::int32_t* __restrict__ lengths,
+                                                               const std::int32_t* __restrict__ tables,
+                                                               std::uint32_t layer, std::uint64_t max_tokens,
+                                                               float* __restrict__ weights) {
+    const std::uint32_t seq = blockIdx.y % seqs, l = blockIdx.y / seqs;
+    const std::uint64_t idx = static_cast<std::uint64_t>(blockIdx.x) * 256u + threadIdx.x;
+    const std::uint64_t j = idx / g.kv_heads;
+    const std::uint32_t head = static_cast<std::uint32_t>(idx % g.kv_heads);
+    const std::int64_t start = starts ? starts[seq] : 0;
+    const std::int64_t t = start + static_cast<std::int64_t>(j);
+    if (j >= max_tokens || start < 0 || static_cast<std::int64_t>(j) >= lengths[seq] || t > 0x7fffffff) return;
+    const unsigned char* const rec = kv8_record(g, tables + static_cast<std::uint64_t>(seq) * g.max_pages, layer + l,
+                                                head, static_cast<std::uint32_t>(t / kKv8Block));
+    if (rec == nullptr) return;
+    weights[((static_cast<std::uint64_t>(l) * seqs + seq) * max_tokens + j) * g.kv_heads + head] =
+        reinterpret_cast<const float*>(rec + kKv8Weights)[t % kKv8Block];
+}
+
 // ---- eviction ----------------------------------------------------------------
 
-constexpr unsigned kSelectThreads = 256;
+constexpr unsigned kSelectThreads = 1024;
+constexpr std::uint32_t kSelectKeys = 16384;   // keys held in LDS; longer sequences are read again each pass
 
 // Weights as unsigned integers of the same order; NaN (and a token whose page
 // is absent) lowest, the two zeros equal.
@@ -212,11 +317,14 @@ __device__ __forceinline__ std::int64_t held_tokens(const Kv8Geometry& g, std::i
 // top (a histogram of the next byte over the keys that agree so far); then one
 // pass in token order writes the first keep_first, every larger key, as many
 // equal ones as are still wanted (the lowest tokens) and the last keep_last.
+// One workgroup has nothing to overlap its waits with, so the keys are read
+// once, into LDS, and a wave finds a byte's bin with a prefix sum.
 __global__ __launch_bounds__(kSelectThreads) void kv8_select_kernel(
     Kv8Geometry g, const std::int32_t* __restrict__ lengths, const std::int32_t* __restrict__ tables,
     std::uint32_t layer, std::uint32_t layers, std::uint32_t keep_first, std::uint32_t keep_last, std::uint32_t budget,
     std::uint64_t max_tokens, std::int32_t* __restrict__ kept) {
     constexpr unsigned kWaves = kSelectThreads / 64u;
+    __shared__ std::uint32_t keys[kSelectKeys];
     __shared__ std::uint32_t bins[256];
     __shared__ std::uint32_t found_prefix, found_want;
     __shared__ std::uint32_t wave_above[kWaves], wave_equal[kWaves];
@@ -231,46 +339,65 @@ __global__ __launch_bounds__(kSelectThreads) void kv8_select_kernel(
         }
         return;
     }
-    const auto key_of = [&](std::int64_t t) __attribute__((always_inline)) -> std::uint32_t {
-        const unsigned char* const rec =
-            kv8_record(g, table, layer + l, head, static_cast<std::uint32_t>(t / kKv8Block));
+    const auto read_key = [&](std::uint32_t t) __attribute__((always_inline)) -> std::uint32_t {
+        const unsigned char* const rec = kv8_record(g, table, layer + l, head, t / kKv8Block);
         return rec ? weight_key(reinterpret_cast<const float*>(rec + kKv8Weights)[t % kKv8Block]) : 0u;
     };
-    const std::int64_t lo = keep_first, hi = n - keep_last;
-    const std::uint32_t want = budget - keep_first - keep_last;   // of the hi - lo > want middle tokens
+    // The middle tokens are lo + i, i < count; more of them than are wanted.
+    const std::uint32_t lo = keep_first, count = static_cast<std::uint32_t>(n - keep_last) - lo;
+    const std::uint32_t want = budget - keep_first - keep_last;
+    for (std::uint32_t i = tid; i < keep_first; i += kSelectThreads) out[i] = static_cast<std::int32_t>(i);
+    for (std::uint32_t i = tid; i < keep_last; i += kSelectThreads) {
+        out[budget - keep_last + i] = static_cast<std::int32_t>(lo + count + i);
+    }
+    if (want == 0u) return;
+    const std::uint32_t in_lds = count < kSelectKeys ? count : kSelectKeys;
+#pragma unroll 4
+    for (std::uint32_t i = tid; i < in_lds; i += kSelectThreads) keys[i] = read_key(lo + i);
+    const auto key_of = [&](std::uint32_t i) __attribute__((always_inline)) -> std::uint32_t {
+        return i < kSelectKeys ? keys[i] : read_key(lo + i);
+    };
     std::uint32_t prefix = 0u, left = want;
-    if (want > 0u) {
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            for (unsigned b = tid; b < 256u; b += kSelectThreads) bins[b] = 0u;
-            __syncthreads();
-            for (std::int64_t t = lo + tid; t < hi; t += kSelectThreads) {
-                const std::uint32_t key = key_of(t);
-                // Shifts of 32 are undefined: the first round takes every key.
-                if (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&bins[(key >> shift) & 255u], 1u);
-            }
-            __syncthreads();
-            if (tid == 0u) {
-                std::uint32_t rest = left;
-                int b = 255;
-                while (b > 0 && bins[b] < rest) rest -= bins[b--];
-                found_prefix = prefix | static_cast<std::uint32_t>(b) << shift;
-                found_want = rest;
-            }
-            __syncthreads();
-            prefix = found_prefix;
-            left = found_want;
+    for (int shift = 24; shift >= 0; shift -= 8) {
+        if (tid < 256u) bins[tid] = 0u;
+        __syncthreads();
+        for (std::uint32_t i = tid; i < count; i += kSelectThreads) {
+            const std::uint32_t key = key_of(i);
+            // Shifts of 32 are undefined: the first round takes every key.
+            if (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&bins[(key >> shift) & 255u], 1u);
         }
+        __syncthreads();
+        if (wave == 0u) {
+            // Lane i holds bins 255 - 4 i and down; sums from the top.
+            std::uint32_t b[4], sum = 0u;
+#pragma unroll
+            for (unsigned j = 0; j < 4u; ++j) sum += b[j] = bins[255u - 4u * lane - j];
+            std::uint32_t upto = sum;
+#pragma unroll
+            for (unsigned off = 1; off < 64u; off <<= 1) {
+                const std::uint32_t o = static_cast<std::uint32_t>(__shfl_up(static_cast<int>(upto), off));
+                if (lane >= off) upto += o;
+            }
+            std::uint32_t before = upto - sum;
+#pragma unroll
+            for (unsigned j = 0; j < 4u; ++j) {
+                if (before < left && before + b[j] >= left) {   // one bin of one lane: the left-th key is in it
+                    found_prefix = prefix | (255u - 4u * lane - j) << shift;
+                    found_want = left - before;
+                }
+                before += b[j];
+            }
+        }
+        __syncthreads();
+        prefix = found_prefix;
+        left = found_want;
     }
     // prefix is the want-th largest key, left how many keys equal to it stay.
-    for (std::int64_t i = tid; i < keep_first; i += kSelectThreads) out[i] = static_cast<std::int32_t>(i);
-    for (std::int64_t i = tid; i < keep_last; i += kSelectThreads) {
-        out[budget - keep_last + i] = static_cast<std::int32_t>(hi + i);
-    }
     std::uint32_t base_above = 0u, base_equal = 0u;   // larger and equal keys before this round
-    for (std::int64_t t0 = lo; want > 0u && t0 < hi; t0 += kSelectThreads) {
-        const std::int64_t t = t0 + tid;
-        const std::uint32_t key = t < hi ? key_of(t) : 0u;
-        const bool above = t < hi && key > prefix, equal = t < hi && key == prefix;
+    for (std::uint32_t i0 = 0; i0 < count; i0 += kSelectThreads) {
+        const std::uint32_t i = i0 + tid;
+        const std::uint32_t key = i < count ? key_of(i) : 0u;
+        const bool above = i < count && key > prefix, equal = i < count && key == prefix;
         const std::uint64_t above_mask = __ballot(above), equal_mask = __ballot(equal);
         if (lane == 0u) {
             wave_above[wave] = static_cast<std::uint32_t>(__popcll(above_mask));
@@ -278,11 +405,10 @@ __global__ __launch_bounds__(kSelectThreads) void kv8_select_kernel(
         }
         __syncthreads();
         std::uint32_t a = base_above, e = base_equal, all_above = 0u, all_equal = 0u;
+#pragma unroll
         for (unsigned w = 0; w < kWaves; ++w) {
-            if (w < wave) {
-                a += wave_above[w];
-                e += wave_equal[w];
-            }
+            a += w < wave ? wave_above[w] : 0u;
+            e += w < wave ? wave_equal[w] : 0u;
             all_above += wave_above[w];
             all_equal += wave_equal[w];
         }
@@ -290,7 +416,7 @@ __global__ __launch_bounds__(kSelectThreads) void kv8_select_kernel(
         a += static_cast<std::uint32_t>(__popcll(above_mask & below));
         e += static_cast<std::uint32_t>(__popcll(equal_mask & below));
         if (above || (equal && e < left)) {
-            out[keep_first + a + (e < left ? e : left)] = static_cast<std::int32_t>(t);
+            out[keep_first + a + (e < left ? e : left)] = static_cast<std::int32_t>(lo + i);
         }
         base_above += all_above;
         base_equal += all_equal;
@@ -364,12 +490,15 @@ __global__ __launch_bounds__(2 * D) void kv8_compact_kernel(Kv8Geometry g, const
 #pragma unroll
         for (unsigned i = 0; i < 4u; ++i) codes[i] = kv8_zero_code<TYPE>() * 0x01010101u;
         if (value) {
+            std::uint32_t was[16];   // all asked for before the first is used
 #pragma unroll
             for (unsigned i = 0; i < 16u; ++i) {
-                if (source[i] == nullptr) continue;
-                const std::uint32_t was = source[i][kv8_v_offset(D, source_slot[i], part)];
+                was[i] = source[i] ? source[i][kv8_v_offset(D, source_slot[i], part)] : kv8_zero_code<TYPE>();
+            }
+#pragma unroll
+            for (unsigned i = 0; i < 16u; ++i) {
                 const std::uint32_t now =
-                    scales[i] == scale ? was : kv8_recode<TYPE>(was, scale > 0.0f ? scales[i] / scale : 0.0f);
+                    scales[i] == scale ? was[i] : kv8_recode<TYPE>(was[i], scale > 0.0f ? scales[i] / scale : 0.0f);
                 codes[i >> 2] = (codes[i >> 2] & ~(0xffu << (8u * (i & 3u)))) | now << (8u * (i & 3u));
             }
         } else if (source[token] != nullptr) {
@@ -402,9 +531,10 @@ hipError_t launch_kv8_append(const Kv8Geometry& g, const float* qkv, std::uint64
                              std::uint32_t m, const std::int32_t* positions, const std::int32_t* tables,
                              std::uint32_t layer, hipStream_t stream) {
     const dim3 grid(m, g.kv_heads);
+    const bool aligned = reinterpret_cast<std::uintptr_t>(qkv) % 16u == 0 && stride % 4u == 0 && q_width % 4u == 0;
 #define AIR_KV8_APPEND(T, D)                                                                                     \
     hipLaunchKernelGGL((kv8_append_kernel<T, D>), grid, dim3(2 * D), 0, stream, g, qkv, stride, q_width, m, positions, \
-                       tables, layer)
+                       tables, layer, aligned)
     if (g.type == kKv8I8) {
         if (g.head_dim == 128u) AIR_KV8_APPEND(kKv8I8, 128);
         else AIR_KV8_APPEND(kKv8I8, 64);
@@ -420,16 +550,27 @@ hipError_t launch_kv8_read(const Kv8Geometry& g, std::uint32_t seqs, const std::
                            const std::int32_t* lengths, const std::int32_t* tables, std::uint32_t layer,
                            std::uint32_t layers, std::uint64_t max_tokens, float* k, float* v, float* weights,
                            hipStream_t stream) {
+    if (!k && !v) {
+        const std::uint64_t threads = max_tokens * g.kv_heads;
+        hipLaunchKernelGGL(kv8_read_weights_kernel, dim3(static_cast<unsigned>((threads + 255u) / 256u), seqs * layers),
+                           dim3(256), 0, stream, g, seqs, starts, lengths, tables, layer, max_tokens, weights);
+        return hipGetLastError();
+    }
     // A start inside a block makes the tokens span one more.
     const std::uint64_t blocks = (max_tokens + kKv8Block - 1u) / kKv8Block + (starts ? 1u : 0u);
     const dim3 grid(static_cast<unsigned>(blocks), g.kv_heads, seqs * layers);
+    const bool aligned = reinterpret_cast<std::uintptr_t>(k) % 16u == 0 && reinterpret_cast<std::uintptr_t>(v) % 16u == 0;
+#define AIR_KV8_READ(T, D)                                                                                           \
+    hipLaunchKernelGGL((kv8_read_kernel<T, D>), grid, dim3(2 * D), 0, stream, g, seqs, starts, lengths, tables, layer, \
+                       max_tokens, k, v, weights, aligned)
     if (g.type == kKv8I8) {
-        hipLaunchKernelGGL(kv8_read_kernel<kKv8I8>, grid, dim3(256), 0, stream, g, seqs, starts, lengths, tables, layer,
-                           max_tokens, k, v, weights);
+        if (g.head_dim == 128u) AIR_KV8_READ(kKv8I8, 128);
+        else AIR_KV8_READ(kKv8I8, 64);
     } else {
-        hipLaunchKernelGGL(kv8_read_kernel<kKv8E4M3>, grid, dim3(256), 0, stream, g, seqs, starts, lengths, tables,
-                           layer, max_tokens, k, v, weights);
+        if (g.head_dim == 128u) AIR_KV8_READ(kKv8E4M3, 128);
+        else AIR_KV8_READ(kKv8E4M3, 64);
     }
+#undef AIR_KV8_READ
     return hipGetLastError();
 }
 

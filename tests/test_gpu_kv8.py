@@ -361,6 +361,7 @@ def test_attention_where_it_can_go_wrong(torch_cuda, hip_ctx, kind):
     rewrite(3, 16, 20, 1.0, 1e-30)
     bad = rows(rng, 1, 0, kvh, d)
     bad[0, 5] = np.nan
+    bad[0, 2 * kvh * d - 1] = np.inf                  # V of the last KV head
     cache.append(bad, 0, [99], tables[4:5], 1)        # sequence 4: its last block is poisoned
     dev = Device(torch_cuda, hip_ctx, cache)
     named = [(0, 149), (1, 39), (1, 15), (1, 31), (2, 89), (3, 19), (3, 15), (4, 95)]
@@ -374,7 +375,7 @@ def test_attention_where_it_can_go_wrong(torch_cuda, hip_ctx, kind):
     within(got, want, tol)
     poisoned = dev.attention(x[:2], [99, 39], tables[[4, 1]], 1, q_heads, 150)
     assert np.isnan(poisoned[0, :q_heads // kvh * d]).all()      # K of KV head 0
-    assert np.isfinite(poisoned[0, q_heads // kvh * d:]).all()
+    assert np.isnan(poisoned[0, -d:]).all() and np.isnan(poisoned[0]).all()   # V of KV head 1
     assert np.isfinite(poisoned[1]).all()
     broken = x[:2].copy()
     broken[0, 3] = np.nan
