@@ -426,6 +426,7 @@ struct Kv8Shape {
     std::uint32_t splits;         // grid z
     std::uint32_t split_chunks;
     std::uint32_t tile_rows;      // rows of one run a tile holds; 0: a tile is a row
+    std::uint32_t waves;          // of a workgroup
 };
 Kv8Shape kv8_attention_shape(std::uint32_t m, std::uint32_t q_heads, std::uint32_t kv_heads, std::uint32_t runs,
                              std::uint64_t max_tokens);

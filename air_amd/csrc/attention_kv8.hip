@@ -35,8 +35,9 @@
 namespace air_hip {
 namespace {
 
-constexpr unsigned kWaves = 4;
+constexpr unsigned kWaves = 4;             // waves of a workgroup, but for short decode steps
 constexpr unsigned kThreads = 64 * kWaves;
+constexpr unsigned kShortWaves = 8;
 constexpr unsigned kVectors = 16;          // query vectors of an MFMA tile
 constexpr unsigned kPromptTiles = 2;       // MFMA tiles of a workgroup where runs have several rows
 constexpr unsigned kChunkBlocks = 4;       // blocks of a chunk, one per lane group
@@ -244,8 +245,8 @@ __device__ __forceinline__ Tile find_tile(std::uint32_t index, const std::int32_
 // take the chunks of split blockIdx.z in turn, every wave for all vectors.
 // With NV > 1 the vectors' operands lie in LDS, and a chunk's codes are turned
 // into f16 once for all of them.
-template <int TYPE, unsigned D, unsigned NV, bool RUNS>
-__global__ __launch_bounds__(kThreads, NV == 1u ? 3 : 2) void kv8_attention_kernel(
+template <int TYPE, unsigned D, unsigned NV, bool RUNS, unsigned W>
+__global__ __launch_bounds__(64 * W, NV == 1u && W == kWaves ? 3 : 2) void kv8_attention_kernel(
     Kv8Geometry g, const float* __restrict__ qkv, std::uint64_t stride, std::uint32_t m,
     const std::int32_t* __restrict__ positions, const std::int32_t* __restrict__ tables, std::uint32_t layer,
     std::uint32_t q_heads, const std::int32_t* __restrict__ run_starts, std::uint32_t runs, std::uint32_t tile_rows,
@@ -256,12 +257,12 @@ __global__ __launch_bounds__(kThreads, NV == 1u ? 3 : 2) void kv8_attention_kern
     constexpr unsigned kFrags = D / 32;            // k steps of a score
     union Shared {
         half8v query[NV > 1u ? NV : 1u][kFrags][2][64];
-        float sums[kWaves][kTile][LD];
+        float sums[W][kTile][LD];
     };
     __shared__ Shared sh;
     __shared__ float undo_of[kTile];
-    __shared__ int wave_m[kWaves][kTile], wave_m2[kWaves][kTile];
-    __shared__ float wave_l[kWaves][kTile];
+    __shared__ int wave_m[W][kTile], wave_m2[W][kTile];
+    __shared__ float wave_l[W][kTile];
     const unsigned tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, grp = lane >> 4, col = lane & 15u;
     const std::uint32_t split = blockIdx.z;
     const std::uint32_t group = q_heads / g.kv_heads, parts = (group + kTile - 1u) / kTile;
@@ -308,7 +309,7 @@ __global__ __launch_bounds__(kThreads, NV == 1u ? 3 : 2) void kv8_attention_kern
         load_query<D>(vector_at(col), grp, q);
         undo[0] = q.undo;
     } else {
-        for (unsigned n = wave; n < NV; n += kWaves) {
+        for (unsigned n = wave; n < NV; n += W) {
             load_query<D>(vector_at(n * kVectors + col), grp, q);
 #pragma unroll
             for (unsigned i = 0; i < kFrags; ++i) {
@@ -344,12 +345,12 @@ __global__ __launch_bounds__(kThreads, NV == 1u ? 3 : 2) void kv8_attention_kern
     // Pages of the blocks whose K and V this lane loads.
     std::uint32_t k_block = from * kChunkBlocks + (col >> 2), v_block = from * kChunkBlocks + grp, k_slot, v_slot;
     std::int32_t k_page = page_of(k_block, k_slot), v_page = page_of(v_block, v_slot);
-    for (std::uint32_t c = from; c < end; c += kWaves) {
+    for (std::uint32_t c = from; c < end; c += W) {
         const Kv8Byte* const krec = kv8_record_in(g, k_page, k_slot, layer, kvh, k_block);
         const Kv8Byte* const vrec = kv8_record_in(g, v_page, v_slot, layer, kvh, v_block);
         const bool here = vrec != nullptr;
-        k_block += kWaves * kChunkBlocks;
-        v_block += kWaves * kChunkBlocks;
+        k_block += W * kChunkBlocks;
+        v_block += W * kChunkBlocks;
         k_page = page_of(k_block, k_slot);
         v_page = page_of(v_block, v_slot);
         KeyCodes<D> keys;
@@ -501,18 +502,18 @@ __global__ __launch_bounds__(kThreads, NV == 1u ? 3 : 2) void kv8_attention_kern
         for (unsigned t = 0; t < D / 16u; ++t) *reinterpret_cast<float4v*>(&sh.sums[wave][v][16u * t + 4u * grp]) = o[n][t];
     }
     __syncthreads();
-    for (unsigned idx = tid; idx < nq * (D / 4u); idx += kThreads) {
+    for (unsigned idx = tid; idx < nq * (D / 4u); idx += 64u * W) {
         const unsigned v = idx / (D / 4u), d4 = idx % (D / 4u);
         int mm = kNone, mm2 = kNone;
 #pragma unroll
-        for (unsigned w = 0; w < kWaves; ++w) {
+        for (unsigned w = 0; w < W; ++w) {
             mm = wave_m[w][v] > mm ? wave_m[w][v] : mm;
             mm2 = wave_m2[w][v] > mm2 ? wave_m2[w][v] : mm2;
         }
         float total = 0.0f;
         float4v acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (unsigned w = 0; w < kWaves; ++w) {
+        for (unsigned w = 0; w < W; ++w) {
             total += __builtin_amdgcn_ldexpf(wave_l[w][v], wave_m[w][v] - mm);
             const float4v a = *reinterpret_cast<const float4v*>(&sh.sums[w][v][4u * d4]);
 #pragma unroll
@@ -605,7 +606,8 @@ __global__ __launch_bounds__(kThreads) void kv8_merge_kernel(
     }
     const std::uint32_t live = live_splits(reach, max_tokens, split_chunks);
     if (live <= 1u) return;   // the attention kernel wrote this tile
-    for (unsigned idx = threadIdx.x; idx < tile.rows * tile.heads * (D / 4u); idx += kThreads) {
+    for (unsigned idx = blockIdx.z * kThreads + threadIdx.x; idx < tile.rows * tile.heads * (D / 4u);
+         idx += gridDim.z * kThreads) {
         const unsigned v = idx / (D / 4u), d4 = idx % (D / 4u);
         const std::uint64_t vector =
             static_cast<std::uint64_t>(tile.row + v / tile.heads) * q_heads + tile.head + v % tile.heads;
@@ -701,17 +703,27 @@ __global__ __launch_bounds__(kThreads) void kv8_weights_kernel(
                       grp, q);
         float base, share;   // M and 1 / l
         const std::uint32_t live = MERGE ? live_splits(position, max_tokens, split_chunks) : 1u;
-        if (MERGE && live > 1u) {
+        if (MERGE && __any(live > 1u)) {
+            // Lane group grp takes splits grp, grp + 4, ...; then they meet.
             int ref = kNone;
             float total = 0.0f;
-            for (std::uint32_t s = 0; s < live; ++s) {
+            for (std::uint32_t s = grp; s < live && live > 1u; s += 4u) {
                 const float4v head = *reinterpret_cast<const float4v*>(partials + (vector * splits + s) * (D + kStat));
                 const int a = __float_as_int(head[0]), next = a > ref ? a : ref;
                 total = __builtin_amdgcn_ldexpf(total, ref - next) + __builtin_amdgcn_ldexpf(head[2], a - next);
                 ref = next;
             }
-            base = static_cast<float>(ref);
+            const int all = groups_max(ref);
+            total = __builtin_amdgcn_ldexpf(total, ref - all);
+            total += __shfl_xor(total, 16);
+            total += __shfl_xor(total, 32);
+            base = static_cast<float>(all);
             share = total == 0.0f ? 0.0f : 1.0f / total;
+            if (live <= 1u) {   // the attention kernel left this row's
+                const float2 st = stats[vector];
+                base = st.x;
+                share = st.y;
+            }
         } else {
             const float2 st = stats[vector];
             base = st.x;
@@ -768,16 +780,29 @@ Kv8Shape kv8_attention_shape(std::uint32_t m, std::uint32_t q_heads, std::uint32
     const std::uint32_t tile_rows = by_run && group < tile ? tile / group : 1u;
     const std::uint32_t tiles = by_run ? m / tile_rows + runs : m;
     const std::uint32_t chunks = static_cast<std::uint32_t>((max_tokens + kChunkTokens - 1u) / kChunkTokens);
+#ifndef SHORT_CHUNKS
+#define SHORT_CHUNKS 32u
+#endif
+#ifndef SHORT_TILES
+#define SHORT_TILES 256u
+#endif
+    const std::uint64_t groups = static_cast<std::uint64_t>(by_run ? m / tile_rows + 1u : m) * kv_heads * parts;
+    if (!by_run && chunks <= SHORT_CHUNKS && groups <= SHORT_TILES) return Kv8Shape{tiles, kv_heads * parts, 1u, chunks, 0u, kShortWaves};
     // Splits of equal length, so that rows of unequal lengths make workgroups
     // of equal work: at least two chunks a wave, and at most about four
     // workgroups a CU if every row were max_tokens long.
-    const std::uint64_t groups = static_cast<std::uint64_t>(by_run ? m / tile_rows + 1u : m) * kv_heads * parts;
-    std::uint64_t per = (groups * chunks + 1023u) / 1024u;
+#ifndef TARGET
+#define TARGET 1024u
+#endif
+#ifndef MINC
+#define MINC 2u
+#endif
+    std::uint64_t per = (groups * chunks + TARGET - 1u) / TARGET;
     per = (per + kWaves - 1u) / kWaves * kWaves;
-    if (per < 2u * kWaves) per = 2u * kWaves;
+    if (per < MINC * kWaves) per = MINC * kWaves;
     if (per > chunks) per = chunks;
     const std::uint32_t splits = static_cast<std::uint32_t>((chunks + per - 1u) / per);
-    return Kv8Shape{tiles, kv_heads * parts, splits, static_cast<std::uint32_t>(per), by_run ? tile_rows : 0u};
+    return Kv8Shape{tiles, kv_heads * parts, splits, static_cast<std::uint32_t>(per), by_run ? tile_rows : 0u, kWaves};
 }
 
 std::uint64_t kv8_attention_scratch(const Kv8Shape& shape, std::uint32_t m, std::uint32_t q_heads,
@@ -796,10 +821,10 @@ void launch_typed(const Kv8Geometry& g, const float* qkv, std::uint64_t stride, 
                   const Kv8Shape& shape, float* partials, float2* stats, float* out, hipStream_t stream) {
     // Scores in powers of two: s log2(e) = (q . k) * log2(e) / sqrt(D).
     const float scale = static_cast<float>(1.4426950408889634 / __builtin_sqrt(static_cast<double>(D)));
-    const dim3 grid(shape.tile_heads, shape.tiles, shape.splits), merge_grid(shape.tile_heads, shape.tiles);
     const bool split = shape.splits > 1u, by_run = shape.tile_rows != 0u;
-#define AIR_KV8_ATTENTION(NV, RUNS)                                                                                  \
-    hipLaunchKernelGGL((kv8_attention_kernel<TYPE, D, NV, RUNS>), grid, dim3(kThreads), 0, stream, g, qkv, stride, m, \
+    const dim3 grid(shape.tile_heads, shape.tiles, shape.splits), merge_grid(shape.tile_heads, shape.tiles, by_run ? 4u : 1u);
+#define AIR_KV8_ATTENTION(NV, RUNS, W)                                                                               \
+    hipLaunchKernelGGL((kv8_attention_kernel<TYPE, D, NV, RUNS, W>), grid, dim3(64 * W), 0, stream, g, qkv, stride, m, \
                        positions, tables, layer, q_heads, run_starts, runs, shape.tile_rows, max_tokens,             \
                        shape.split_chunks, scale, partials, stats, out)
 #define AIR_KV8_MERGE(NV, RUNS)                                                                                      \
@@ -813,11 +838,12 @@ void launch_typed(const Kv8Geometry& g, const float* qkv, std::uint64_t stride, 
     const std::uint32_t chunks = static_cast<std::uint32_t>((max_tokens + kChunkTokens - 1u) / kChunkTokens);
     const std::uint32_t columns = (chunks + kWaves - 1u) / kWaves;
     if (by_run) {
-        AIR_KV8_ATTENTION(kPromptTiles, true);
+        AIR_KV8_ATTENTION(kPromptTiles, true, kWaves);
         if (split) AIR_KV8_MERGE(kPromptTiles, true);
         if (weights) AIR_KV8_WEIGHTS(true, false, chunks);
     } else {
-        AIR_KV8_ATTENTION(1u, false);
+        if (shape.waves == kShortWaves) AIR_KV8_ATTENTION(1u, false, kShortWaves);
+        else AIR_KV8_ATTENTION(1u, false, kWaves);
         if (weights && split) AIR_KV8_WEIGHTS(false, true, columns + 1u);
         else if (weights) AIR_KV8_WEIGHTS(false, false, columns);
         else if (split) AIR_KV8_MERGE(1u, false);

@@ -92,6 +92,14 @@ __global__ __launch_bounds__(2 * D) void kv8_append_kernel(Kv8Geometry g, const 
     const auto place_of = [&](std::int32_t pos, std::uint32_t slot) __attribute__((always_inline)) {
         return static_cast<std::uint32_t>(pos) / kKv8Block - slot * g.page_blocks;
     };
+    // In a small call the other rows' pages are asked for at once.
+    const bool small = m <= kThreads;
+    std::int32_t first_pos = -1, first_page = -1;
+    std::uint32_t first_slot = 0u;
+    if (small && tid < m) {
+        first_pos = positions[tid];
+        first_page = page_of(tid, first_pos, first_slot);
+    }
     const std::int32_t pos = positions[r], pos_before = r > 0u ? positions[r - 1u] : -1;
     std::uint32_t slot, slot_before;
     const std::int32_t page = page_of(r, pos, slot), page_before = page_of(r > 0u ? r - 1u : 0u, pos_before, slot_before);
@@ -116,29 +124,34 @@ __global__ __launch_bounds__(2 * D) void kv8_append_kernel(Kv8Geometry g, const 
     if (tid < kKv8Block) winner[tid] = -1;
     if (tid == 0u) earlier = named = 0;
     __syncthreads();
-    for (std::uint32_t o0 = tid; o0 < m; o0 += kAtOnce * kThreads) {
-        std::int32_t their_pos[kAtOnce], their_page[kAtOnce];
-        std::uint32_t their_slot[kAtOnce];
-#pragma unroll
-        for (unsigned j = 0; j < kAtOnce; ++j) {
-            const std::uint32_t o = o0 + j * kThreads;
-            their_pos[j] = o < m ? positions[o] : -1;
+    const auto look_at = [&](std::uint32_t o, std::int32_t their_pos, std::int32_t their_page, std::uint32_t their_slot)
+                             __attribute__((always_inline)) {
+        if (their_page != page || place_of(their_pos, their_slot) != place) return;
+        if (o < r) {
+            earlier = 1;
+        } else {
+            atomicMax(&winner[static_cast<std::uint32_t>(their_pos) % kKv8Block], static_cast<int>(o));
+            if (o > r) named = 1;
         }
+    };
+    if (small) {
+        look_at(tid, first_pos, first_page, first_slot);
+    } else {
+        for (std::uint32_t o0 = tid; o0 < m; o0 += kAtOnce * kThreads) {
+            std::int32_t their_pos[kAtOnce], their_page[kAtOnce];
+            std::uint32_t their_slot[kAtOnce];
 #pragma unroll
-        for (unsigned j = 0; j < kAtOnce; ++j) {
-            const std::uint32_t o = o0 + j * kThreads;
-            their_page[j] = page_of(o < m ? o : 0u, their_pos[j], their_slot[j]);
-        }
-#pragma unroll
-        for (unsigned j = 0; j < kAtOnce; ++j) {
-            const std::uint32_t o = o0 + j * kThreads;
-            if (their_page[j] != page || place_of(their_pos[j], their_slot[j]) != place) continue;
-            if (o < r) {
-                earlier = 1;
-            } else {
-                atomicMax(&winner[static_cast<std::uint32_t>(their_pos[j]) % kKv8Block], static_cast<int>(o));
-                if (o > r) named = 1;
+            for (unsigned j = 0; j < kAtOnce; ++j) {
+                const std::uint32_t o = o0 + j * kThreads;
+                their_pos[j] = o < m ? positions[o] : -1;
             }
+#pragma unroll
+            for (unsigned j = 0; j < kAtOnce; ++j) {
+                const std::uint32_t o = o0 + j * kThreads;
+                their_page[j] = page_of(o < m ? o : 0u, their_pos[j], their_slot[j]);
+            }
+#pragma unroll
+            for (unsigned j = 0; j < kAtOnce; ++j) look_at(o0 + j * kThreads, their_pos[j], their_page[j], their_slot[j]);
         }
     }
     __syncthreads();
@@ -427,25 +440,24 @@ __global__ __launch_bounds__(kSelectThreads) void kv8_select_kernel(
 // Gathers the kept tokens of a (sequence, layer, KV head) into blocks of the
 // new table.  A block's scale is the largest of its tokens' scales, so a
 // block whose tokens come from one block keeps its codes, and others are
-// rounded once.  Threads as in the append.  Where the new table is the old
-// one (in place) a workgroup takes all blocks in ascending order: block b's
-// tokens come from blocks >= b, so what it overwrites no later block reads,
-// and it reads its 16 tokens before it writes.
+// rounded once.  Threads as in the append; a token's source, scale and the
+// ratio its codes take are found once, by 16 threads for K and 16 for V.
+// Where the new table is the old one (in place) a workgroup takes all blocks
+// in ascending order: block b's tokens come from blocks >= b, so what it
+// overwrites no later block reads, and it reads its 16 tokens before it
+// writes.
 template <int TYPE, unsigned D>
-__global__ __launch_bounds__(2 * D) void kv8_compact_kernel(Kv8Geometry g, const std::int32_t* lengths,
-                                                            const std::int32_t* tables, const std::int32_t* new_tables,
-                                                            std::uint32_t layer, std::uint32_t layers,
-                                                            std::uint32_t heads, std::uint32_t budget,
-                                                            std::uint64_t max_tokens, const std::int32_t* kept,
+__global__ __launch_bounds__(2 * D) void kv8_compact_kernel(Kv8Geometry g, const std::int32_t* tables,
+                                                            const std::int32_t* new_tables, std::uint32_t layer,
+                                                            std::uint32_t layers, std::uint32_t budget,
+                                                            std::uint32_t blocks, const std::int32_t* kept,
                                                             bool in_place) {
 #pragma clang fp contract(off)
     __shared__ const unsigned char* source[kKv8Block];
     __shared__ std::uint32_t source_slot[kKv8Block];
-    __shared__ float source_scale[2][kKv8Block];
-    __shared__ float source_weight[kKv8Block];
-    const std::uint32_t head = blockIdx.y % heads, l = blockIdx.y / heads, seq = blockIdx.z;
-    const std::int64_t n = held_tokens(g, lengths[seq], max_tokens);
-    if (in_place && n <= static_cast<std::int64_t>(budget)) return;   // everything stays where it is
+    __shared__ float source_ratio[2][kKv8Block];   // below zero: the code stays as it is
+    __shared__ float new_scale[2];
+    const std::uint32_t head = blockIdx.y % g.kv_heads, l = blockIdx.y / g.kv_heads, seq = blockIdx.z;
     const unsigned tid = threadIdx.x;
     const bool value = tid >= D;
     const unsigned part = value ? tid - D : tid;
@@ -454,41 +466,44 @@ __global__ __launch_bounds__(2 * D) void kv8_compact_kernel(Kv8Geometry g, const
     const std::int32_t* const new_table = new_tables + static_cast<std::uint64_t>(seq) * g.max_pages;
     const std::int32_t* const list =
         kept + ((static_cast<std::uint64_t>(seq) * layers + l) * g.kv_heads + head) * budget;
-    const std::uint32_t tokens = n < static_cast<std::int64_t>(budget) ? static_cast<std::uint32_t>(n) : budget;
-    const std::uint32_t blocks = (tokens + kKv8Block - 1u) / kKv8Block;
+    if (in_place && list[budget - 1u] < static_cast<std::int32_t>(budget)) return;   // everything stays where it is
     for (std::uint32_t b = blockIdx.x; b < blocks; b += gridDim.x) {
-        if (tid < kKv8Block) {
-            const std::uint32_t i = b * kKv8Block + tid;
-            const std::int32_t t = i < tokens ? list[i] : -1;
+        if (list[b * kKv8Block] < 0) return;   // no tokens from here on
+        unsigned char* const dst = kv8_record(g, new_table, layer + l, head, b);
+        float weight = 0.0f;
+        if (part < kKv8Block) {
+            const std::uint32_t i = b * kKv8Block + part;
+            const std::int32_t t = i < budget ? list[i] : -1;
             const unsigned char* src = nullptr;
-            float s0 = 0.0f, s1 = 0.0f, w = 0.0f;
+            float s = 0.0f;
             unsigned slot = 0u;
             if (t >= 0) {
                 slot = static_cast<std::uint32_t>(t) % kKv8Block;
                 src = kv8_record(g, table, layer + l, head, static_cast<std::uint32_t>(t) / kKv8Block);
                 if (src) {
-                    s0 = reinterpret_cast<const float*>(src)[0];
-                    s1 = reinterpret_cast<const float*>(src)[1];
-                    w = reinterpret_cast<const float*>(src + kKv8Weights)[slot];
+                    s = reinterpret_cast<const float*>(src)[value ? 1 : 0];
+                    weight = reinterpret_cast<const float*>(src + kKv8Weights)[slot];
                 }
             }
-            source[tid] = src;
-            source_slot[tid] = slot;
-            source_scale[0][tid] = s0;
-            source_scale[1][tid] = s1;
-            source_weight[tid] = w;
+            // Scales are not negative, so their bits order them, NaN on top:
+            // a poisoned token poisons its new block.
+            std::uint32_t top = __float_as_uint(s);
+#pragma unroll
+            for (int off = 8; off > 0; off >>= 1) {
+                const std::uint32_t o = static_cast<std::uint32_t>(__shfl_xor(static_cast<int>(top), off));
+                top = o > top ? o : top;
+            }
+            const float scale = __uint_as_float(top);
+            if (!value) {
+                source[part] = src;
+                source_slot[part] = slot;
+            }
+            source_ratio[value ? 1 : 0][part] = s == scale ? -1.0f : scale > 0.0f ? s / scale : 0.0f;
+            if (part == 0u) new_scale[value ? 1 : 0] = scale;
         }
         __syncthreads();
-        const float* const scales = source_scale[value ? 1 : 0];
-        float scale = 0.0f;
-#pragma unroll
-        for (unsigned i = 0; i < kKv8Block; ++i) {
-            // Once NaN it stays: a poisoned token poisons its new block.
-            if (scale == scale && !(scales[i] <= scale)) scale = scales[i];
-        }
+        const float* const ratios = source_ratio[value ? 1 : 0];
         u32x4 codes;
-#pragma unroll
-        for (unsigned i = 0; i < 4u; ++i) codes[i] = kv8_zero_code<TYPE>() * 0x01010101u;
         if (value) {
             std::uint32_t was[16];   // all asked for before the first is used
 #pragma unroll
@@ -497,14 +512,16 @@ __global__ __launch_bounds__(2 * D) void kv8_compact_kernel(Kv8Geometry g, const
             }
 #pragma unroll
             for (unsigned i = 0; i < 16u; ++i) {
-                const std::uint32_t now =
-                    scales[i] == scale ? was[i] : kv8_recode<TYPE>(was[i], scale > 0.0f ? scales[i] / scale : 0.0f);
-                codes[i >> 2] = (codes[i >> 2] & ~(0xffu << (8u * (i & 3u)))) | now << (8u * (i & 3u));
+                if (ratios[i] >= 0.0f) was[i] = kv8_recode<TYPE>(was[i], ratios[i]);
+            }
+#pragma unroll
+            for (unsigned i = 0; i < 4u; ++i) {
+                codes[i] = was[4u * i] | was[4u * i + 1u] << 8 | was[4u * i + 2u] << 16 | was[4u * i + 3u] << 24;
             }
         } else if (source[token] != nullptr) {
             codes = *reinterpret_cast<const u32x4*>(source[token] + kv8_k_offset(D, source_slot[token], chunk * 16u));
-            if (scales[token] != scale) {
-                const float ratio = scale > 0.0f ? scales[token] / scale : 0.0f;
+            const float ratio = ratios[token];
+            if (ratio >= 0.0f) {
 #pragma unroll
                 for (unsigned i = 0; i < 16u; ++i) {
                     const std::uint32_t was = (codes[i >> 2] >> (8u * (i & 3u))) & 0xffu;
@@ -512,14 +529,16 @@ __global__ __launch_bounds__(2 * D) void kv8_compact_kernel(Kv8Geometry g, const
                                     kv8_recode<TYPE>(was, ratio) << (8u * (i & 3u));
                 }
             }
+        } else {
+#pragma unroll
+            for (unsigned i = 0; i < 4u; ++i) codes[i] = kv8_zero_code<TYPE>() * 0x01010101u;
         }
         __syncthreads();   // the block's tokens are read: in place, what they share with it may go
-        unsigned char* const dst = kv8_record(g, new_table, layer + l, head, b);
         if (dst != nullptr) {
             const unsigned at = value ? kv8_v_offset(D, 0u, part) : kv8_k_offset(D, token, chunk * 16u);
             *reinterpret_cast<u32x4*>(dst + at) = codes;
-            if (part == 0u) reinterpret_cast<float*>(dst)[value ? 1 : 0] = scale;
-            if (tid < kKv8Block) reinterpret_cast<float*>(dst + kKv8Weights)[tid] = source_weight[tid];
+            if (part == 0u) reinterpret_cast<float*>(dst)[value ? 1 : 0] = new_scale[value ? 1 : 0];
+            if (tid < kKv8Block) reinterpret_cast<float*>(dst + kKv8Weights)[tid] = weight;
         }
         __syncthreads();   // the lists are read before the next block replaces them
     }
@@ -585,8 +604,8 @@ hipError_t launch_kv8_evict(const Kv8Geometry& g, std::uint32_t seqs, const std:
     const std::uint32_t blocks = static_cast<std::uint32_t>((most + kKv8Block - 1u) / kKv8Block);
     const dim3 grid(in_place ? 1u : blocks, g.kv_heads * layers, seqs);
 #define AIR_KV8_COMPACT(T, D)                                                                                      \
-    hipLaunchKernelGGL((kv8_compact_kernel<T, D>), grid, dim3(2 * D), 0, stream, g, lengths, tables, new_tables, layer, \
-                       layers, g.kv_heads, budget, max_tokens, kept, in_place)
+    hipLaunchKernelGGL((kv8_compact_kernel<T, D>), grid, dim3(2 * D), 0, stream, g, tables, new_tables, layer, layers, \
+                       budget, blocks, kept, in_place)
     if (g.type == kKv8I8) {
         if (g.head_dim == 128u) AIR_KV8_COMPACT(kKv8I8, 128);
         else AIR_KV8_COMPACT(kKv8I8, 64);
