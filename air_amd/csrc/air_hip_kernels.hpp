@@ -392,7 +392,8 @@ constexpr int kKv8I8 = 1, kKv8E4M3 = 2;
 struct Kv8Geometry {
     unsigned char* pool;              // contiguous pool, or null when chunks is set
     unsigned char* const* chunks;     // pool_pages >> chunk_shift chunk bases (null: not allocated)
-    std::uint64_t page_bytes;
+    std::uint32_t page_bytes;
+    std::uint32_t head_bytes;         // of a layer's KV head in a page: page_blocks records
     std::uint32_t record_bytes;       // of a block: 128 + 32 * head_dim
     std::uint32_t page_blocks;        // blocks per page
     std::uint32_t page_magic;         // block / page_blocks = umulhi(block, magic); 0: one block a page
@@ -418,6 +419,9 @@ hipError_t launch_kv8_evict(const Kv8Geometry& g, std::uint32_t seqs, const std:
                             std::uint32_t layers, std::uint32_t keep_first, std::uint32_t keep_last,
                             std::uint32_t budget, std::uint64_t max_tokens, std::int32_t* kept, hipStream_t stream);
 
+// The kernels of the attention: tiles of single rows, the same in one launch
+// of larger workgroups, and tiles of a run's rows.
+constexpr int kKv8Rows = 0, kKv8ShortRows = 1, kKv8Runs = 2;
 // How a call's attention is cut: `splits` workgroups of split_chunks 64-token
 // chunks over a tile's keys.
 struct Kv8Shape {
@@ -426,7 +430,7 @@ struct Kv8Shape {
     std::uint32_t splits;         // grid z
     std::uint32_t split_chunks;
     std::uint32_t tile_rows;      // rows of one run a tile holds; 0: a tile is a row
-    std::uint32_t waves;          // of a workgroup
+    int kernel;                   // kKv8Rows ..
 };
 Kv8Shape kv8_attention_shape(std::uint32_t m, std::uint32_t q_heads, std::uint32_t kv_heads, std::uint32_t runs,
                              std::uint64_t max_tokens);

@@ -28,8 +28,18 @@ namespace air_hip {
 constexpr unsigned kKv8Weights = 64;    // byte offset of the weights
 constexpr unsigned kKv8Codes = 128;     // byte offset of the K codes
 
-// A record in global memory: its address as the loads take it.
+// A record in global memory, and loads and stores that say so: through a
+// pointer that came out of memory they would be flat, which wait together
+// with LDS.
 typedef __attribute__((address_space(1))) unsigned char Kv8Byte;
+template <typename T>
+__device__ __forceinline__ T kv8_load(const Kv8Byte* p) {
+    return *(const __attribute__((address_space(1))) T*)p;
+}
+template <typename T>
+__device__ __forceinline__ void kv8_store(Kv8Byte* p, T x) {
+    *(__attribute__((address_space(1))) T*)p = x;
+}
 
 // Entry of a page table that names block `block`'s page.
 __device__ __forceinline__ std::uint32_t kv8_slot(const Kv8Geometry& g, std::uint32_t block) {
@@ -48,18 +58,17 @@ __device__ __forceinline__ Kv8Byte* kv8_record_in(const Kv8Geometry& g, std::int
         if (base == nullptr) return nullptr;
         p &= (1u << g.chunk_shift) - 1u;
     }
-    const std::uint64_t index = (static_cast<std::uint64_t>(layer) * g.kv_heads + head) * g.page_blocks +
-                                (block - slot * g.page_blocks);
-    return (Kv8Byte*)(base + p * g.page_bytes + index * g.record_bytes);
+    const std::uint32_t offset = (layer * g.kv_heads + head) * g.head_bytes + (block - slot * g.page_blocks) * g.record_bytes;
+    return (Kv8Byte*)(base + static_cast<std::uint64_t>(p) * g.page_bytes + offset);
 }
 
 // Record of block `block` of the sequence with this page table, or null when
 // the table does not name a page of the pool.
-__device__ __forceinline__ unsigned char* kv8_record(const Kv8Geometry& g, const std::int32_t* table,
-                                                     std::uint32_t layer, std::uint32_t head, std::uint32_t block) {
+__device__ __forceinline__ Kv8Byte* kv8_record(const Kv8Geometry& g, const std::int32_t* table, std::uint32_t layer,
+                                               std::uint32_t head, std::uint32_t block) {
     const std::uint32_t slot = kv8_slot(g, block);
     if (slot >= g.max_pages) return nullptr;
-    return (unsigned char*)kv8_record_in(g, table[slot], slot, layer, head, block);
+    return kv8_record_in(g, table[slot], slot, layer, head, block);
 }
 
 // Offset of (token, dim) in a record's K and V codes.

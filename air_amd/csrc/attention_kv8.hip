@@ -39,7 +39,7 @@ constexpr unsigned kWaves = 4;             // waves of a workgroup, but for shor
 constexpr unsigned kThreads = 64 * kWaves;
 constexpr unsigned kShortWaves = 8;
 constexpr unsigned kVectors = 16;          // query vectors of an MFMA tile
-constexpr unsigned kPromptTiles = 2;       // MFMA tiles of a workgroup where runs have several rows
+constexpr unsigned kRunTiles = 2;          // MFMA tiles of a workgroup where runs have several rows
 constexpr unsigned kChunkBlocks = 4;       // blocks of a chunk, one per lane group
 constexpr unsigned kChunkTokens = kChunkBlocks * kKv8Block;
 constexpr int kNone = -(1 << 30);          // a reference that no score has set
@@ -145,15 +145,15 @@ __device__ __forceinline__ void load_keys(const Kv8Byte* rec, unsigned lane, Key
     for (unsigned b = 0; b < 4u; ++b) {
 #pragma unroll
         for (unsigned s = 0; s < D / 64u; ++s) {
-            k.c[b][s] = *(const __attribute__((address_space(1))) u32x4*)(at + b * (D * 4u) + s * 256u);
+            k.c[b][s] = kv8_load<u32x4>(at + b * (D * 4u) + s * 256u);
         }
     }
 }
 
 // What a block's scores are multiplied by.  A block without a scale has codes
 // of zero; any factor will do, and one makes its masked scores -inf.
-__device__ __forceinline__ float score_factor(float undo, float score_scale, float k_scale) {
-    const float f = undo * score_scale * k_scale;      // undo is a power of two
+__device__ __forceinline__ float score_factor(float unit, float k_scale) {
+    const float f = unit * k_scale;
     return f == 0.0f ? 1.0f : f;
 }
 // 2^(score * factor - base), one rounding
@@ -166,12 +166,12 @@ template <unsigned D>
 __device__ __forceinline__ void load_values(const Kv8Byte* rec, unsigned lane, u32x4 (&v)[D / 16]) {
     const Kv8Byte* const at = rec + kKv8Codes + kKv8Block * D + (lane & 15u) * 16u;
 #pragma unroll
-    for (unsigned t = 0; t < D / 16u; ++t) v[t] = *(const __attribute__((address_space(1))) u32x4*)(at + t * 256u);
+    for (unsigned t = 0; t < D / 16u; ++t) v[t] = kv8_load<u32x4>(at + t * 256u);
 }
 
 // The two scales of a record.
 __device__ __forceinline__ float2 load_scales(const Kv8Byte* rec) {
-    const u32x2 v = *(const __attribute__((address_space(1))) u32x2*)rec;
+    const u32x2 v = kv8_load<u32x2>(rec);
     return make_float2(__uint_as_float(v.x), __uint_as_float(v.y));
 }
 
@@ -202,6 +202,82 @@ __device__ __forceinline__ int groups_max(int x) {
     const auto q = __builtin_amdgcn_permlane16_swap(m, m, false, false);
     const int c = static_cast<int>(q[0]), d = static_cast<int>(q[1]);
     return c > d ? c : d;
+}
+
+// The scores of a chunk into p' = hi + lo, the B operands of the products
+// with V, and into the denominator.  `ahead`: how far this lane's vector lies
+// behind the block's first token (it sees tokens 0..ahead); `here`: the block
+// has a page; scale: of K and V.
+template <unsigned D>
+__device__ __forceinline__ void soften(float4v (&s)[4], float unit, float2 scale, bool here, int ahead, int& ref, int& ref2,
+                                       float& l, float4v (&o)[D / 16], half8v (&p_hi)[2], half8v (&p_lo)[2]) {
+    float factor = score_factor(unit, scale.x);
+    float v_scale = scale.y;
+    const int exponent = __builtin_amdgcn_frexp_expf(v_scale);   // scale of V < 2^exponent
+    if (!__all(here && ahead >= 15)) {
+        // What a vector does not see scores -inf; a block that it sees
+        // nothing of has no scales either (they may be NaN).
+        const int limit = here ? ahead : -1;
+        factor = limit < 0 ? 1.0f : factor;
+        v_scale = limit < 0 ? 0.0f : v_scale;
+#pragma unroll
+        for (unsigned b = 0; b < 4u; ++b) {
+#pragma unroll
+            for (unsigned r = 0; r < 4u; ++r) {
+                s[b][r] = static_cast<int>(4u * b + r) <= limit ? s[b][r] : -__builtin_huge_valf();
+            }
+        }
+    }
+    float top = s[0][0];
+#pragma unroll
+    for (unsigned b = 0; b < 4u; ++b) {
+#pragma unroll
+        for (unsigned r = 0; r < 4u; ++r) top = fmaxf(top, s[b][r]);
+    }
+    // The block's own references; the vector's only move when one of its
+    // blocks passes them.
+    const float bound = fminf(ceilf(top * factor), 0x1p28f);
+    const int block_m = bound < -0x1p28f ? kNone : static_cast<int>(bound);   // differences stay in 32 bits
+    const int block_m2 = block_m == kNone || v_scale == 0.0f ? kNone : block_m + exponent;
+    if (__any(block_m > ref || block_m2 > ref2)) {
+        const int next = groups_max(block_m > ref ? block_m : ref);
+        const int next2 = groups_max(block_m2 > ref2 ? block_m2 : ref2);
+        l = __builtin_amdgcn_ldexpf(l, ref - next);
+        const int down = ref2 - next2;
+#pragma unroll
+        for (unsigned t = 0; t < D / 16u; ++t) {
+#pragma unroll
+            for (unsigned r = 0; r < 4u; ++r) o[t][r] = __builtin_amdgcn_ldexpf(o[t][r], down);
+        }
+        ref = next;
+        ref2 = next2;
+    }
+    // p' = 2^(s - base) * share, below 2^kPBits; a scale of V far below the
+    // others' (or zero) keeps base near M, so the same powers also sum up the
+    // denominator.  s - base is small where p is large, and rounded once.
+    int e = ref2 - ref - 40;
+    e = v_scale == 0.0f || exponent < e ? e : exponent;
+    const int base = ref2 - e;
+    const float share = __builtin_amdgcn_ldexpf(v_scale, kPBits - e);
+    const float fbase = static_cast<float>(base);
+    float sum = 0.0f;
+#pragma unroll
+    for (unsigned b = 0; b < 4u; ++b) {
+#pragma unroll
+        for (unsigned r = 0; r < 4u; r += 2u) {
+            const float x0 = score_power(s[b][r], factor, fbase);
+            const float x1 = score_power(s[b][r + 1u], factor, fbase);
+            sum += x0;
+            sum += x1;
+            half2v hi, lo;
+            split_products(x0, x1, share, hi, lo);
+            p_hi[b >> 1][4u * (b & 1u) + r] = hi[0];
+            p_hi[b >> 1][4u * (b & 1u) + r + 1u] = hi[1];
+            p_lo[b >> 1][4u * (b & 1u) + r] = lo[0];
+            p_lo[b >> 1][4u * (b & 1u) + r + 1u] = lo[1];
+        }
+    }
+    l += __builtin_amdgcn_ldexpf(sum, base - ref);
 }
 
 // The rows of a tile: with RUNS up to kRows rows of one run (kRows whole
@@ -384,78 +460,10 @@ __global__ __launch_bounds__(64 * W, NV == 1u && W == kWaves ? 3 : 2) void kv8_a
         }
         // Tokens of this lane's block that its vectors may attend to.
         const int first = static_cast<int>((c * kChunkBlocks + grp) * kKv8Block);
-        const int exponent = __builtin_amdgcn_frexp_expf(now.y);   // scale of V < 2^exponent
         half8v p_hi[NV][2], p_lo[NV][2];
 #pragma unroll
         for (unsigned n = 0; n < NV; ++n) {
-            float factor = score_factor(undo[n], score_scale, now.x);
-            float v_scale = now.y;
-            const int ahead = pos[n] - first;
-            if (!__all(here && ahead >= 15)) {
-                // What a vector does not see scores -inf; a block that it sees
-                // nothing of has no scales either (they may be NaN).
-                const int limit = here ? ahead : -1;
-                factor = limit < 0 ? 1.0f : factor;
-                v_scale = limit < 0 ? 0.0f : v_scale;
-#pragma unroll
-                for (unsigned b = 0; b < 4u; ++b) {
-#pragma unroll
-                    for (unsigned r = 0; r < 4u; ++r) {
-                        s[n][b][r] = static_cast<int>(4u * b + r) <= limit ? s[n][b][r] : -__builtin_huge_valf();
-                    }
-                }
-            }
-            float top = s[n][0][0];
-#pragma unroll
-            for (unsigned b = 0; b < 4u; ++b) {
-#pragma unroll
-                for (unsigned r = 0; r < 4u; ++r) top = fmaxf(top, s[n][b][r]);
-            }
-            // The block's own references; the vector's only move when one of
-            // its blocks passes them.
-            const float bound = fminf(ceilf(top * factor), 0x1p28f);
-            const int block_m = bound < -0x1p28f ? kNone : static_cast<int>(bound);   // differences stay in 32 bits
-            const int block_m2 = block_m == kNone || v_scale == 0.0f ? kNone : block_m + exponent;
-            if (__any(block_m > ref[n] || block_m2 > ref2[n])) {
-                const int next = groups_max(block_m > ref[n] ? block_m : ref[n]);
-                const int next2 = groups_max(block_m2 > ref2[n] ? block_m2 : ref2[n]);
-                l[n] = __builtin_amdgcn_ldexpf(l[n], ref[n] - next);
-                const int down = ref2[n] - next2;
-#pragma unroll
-                for (unsigned t = 0; t < D / 16u; ++t) {
-#pragma unroll
-                    for (unsigned r = 0; r < 4u; ++r) o[n][t][r] = __builtin_amdgcn_ldexpf(o[n][t][r], down);
-                }
-                ref[n] = next;
-                ref2[n] = next2;
-            }
-            // p' = 2^(s - base) * share, below 2^kPBits; a scale of V far below
-            // the others' (or zero) keeps base near M, so the same powers also
-            // sum up the denominator.  s - base is small where p is large, and
-            // rounded once.
-            int e = ref2[n] - ref[n] - 40;
-            e = v_scale == 0.0f || exponent < e ? e : exponent;
-            const int base = ref2[n] - e;
-            const float share = __builtin_amdgcn_ldexpf(v_scale, kPBits - e);
-            const float fbase = static_cast<float>(base);
-            float sum = 0.0f;
-#pragma unroll
-            for (unsigned b = 0; b < 4u; ++b) {
-#pragma unroll
-                for (unsigned r = 0; r < 4u; r += 2u) {
-                    const float x0 = score_power(s[n][b][r], factor, fbase);
-                    const float x1 = score_power(s[n][b][r + 1u], factor, fbase);
-                    sum += x0;
-                    sum += x1;
-                    half2v hi, lo;
-                    split_products(x0, x1, share, hi, lo);
-                    p_hi[n][b >> 1][4u * (b & 1u) + r] = hi[0];
-                    p_hi[n][b >> 1][4u * (b & 1u) + r + 1u] = hi[1];
-                    p_lo[n][b >> 1][4u * (b & 1u) + r] = lo[0];
-                    p_lo[n][b >> 1][4u * (b & 1u) + r + 1u] = lo[1];
-                }
-            }
-            l[n] += __builtin_amdgcn_ldexpf(sum, base - ref[n]);
+            soften<D>(s[n], undo[n] * score_scale, now, here, pos[n] - first, ref[n], ref2[n], l[n], o[n], p_hi[n], p_lo[n]);
         }
         if constexpr (TYPE == kKv8E4M3) {
             // Slots behind the tile's last token may hold NaN codes, which a
@@ -619,6 +627,18 @@ __global__ __launch_bounds__(kThreads) void kv8_merge_kernel(
     }
 }
 
+// A step of the sum over 16 vectors: lanes W apart exchange halves of what
+// they hold, so after steps 8, 4, 2 and 1 lane col has token col's sum.
+template <unsigned W>
+__device__ __forceinline__ void halve(float (&sum)[16], unsigned col) {
+    const bool upper = (col & W) != 0u;
+#pragma unroll
+    for (unsigned t = 0; t < W; ++t) {
+        const float keep = upper ? sum[t + W] : sum[t], give = upper ? sum[t] : sum[t + W];
+        sum[t] = keep + __shfl_xor(give, W);
+    }
+}
+
 // The weights a run's rows give one chunk of tokens: the scores again, by the
 // same instructions as in the attention, and p from the rows' statistics
 // (M and 1 / l).  A chunk of a (run, KV head) is one wave's, or with SHARED,
@@ -632,7 +652,7 @@ __global__ __launch_bounds__(kThreads) void kv8_merge_kernel(
 // joins the splits of a run's rows, and the others take the statistics from
 // the partials themselves, so that one launch follows the attention.
 template <int TYPE, unsigned D, bool SHARED, bool MERGE>
-__global__ __launch_bounds__(kThreads) void kv8_weights_kernel(
+__global__ __launch_bounds__(kThreads, 3) void kv8_weights_kernel(
     Kv8Geometry g, const float* __restrict__ qkv, std::uint64_t stride, std::uint32_t m,
     const std::int32_t* __restrict__ positions, const std::int32_t* __restrict__ tables, std::uint32_t layer,
     std::uint32_t q_heads, const std::int32_t* __restrict__ run_starts, std::uint64_t max_tokens, float score_scale,
@@ -681,11 +701,11 @@ __global__ __launch_bounds__(kThreads) void kv8_weights_kernel(
     last = last < most ? last : most;
     if (token0 > last) return;   // all of a workgroup's waves, where they share a chunk
     const Kv8Byte* const none = (const Kv8Byte*)g_no_record;
-    const Kv8Byte* const krec = (const Kv8Byte*)kv8_record(g, table, layer, kvh, chunk * kChunkBlocks + (col >> 2));
-    unsigned char* const vrec = kv8_record(g, table, layer, kvh, chunk * kChunkBlocks + grp);
+    const Kv8Byte* const krec = kv8_record(g, table, layer, kvh, chunk * kChunkBlocks + (col >> 2));
+    Kv8Byte* const vrec = kv8_record(g, table, layer, kvh, chunk * kChunkBlocks + grp);
     KeyCodes<D> keys;
     load_keys<D>(krec ? krec : none, lane, keys);
-    const float k_scale = load_scales(vrec ? (const Kv8Byte*)vrec : none).x;
+    const float k_scale = load_scales(vrec ? vrec : none).x;
     const int first = token0 + static_cast<int>(grp * kKv8Block);
     float sum[16] = {};
     for (std::uint32_t v0 = SHARED ? wave * kVectors : 0u; v0 < vectors; v0 += (SHARED ? kWaves : 1u) * kVectors) {
@@ -731,7 +751,7 @@ __global__ __launch_bounds__(kThreads) void kv8_weights_kernel(
         }
         float4v s[4];
         chunk_scores<TYPE, D>(keys, q, s);
-        const float factor = score_factor(q.undo, score_scale, k_scale);
+        const float factor = score_factor(q.undo * score_scale, k_scale);
         const int limit = vrec == nullptr ? -1 : upto - first;
 #pragma unroll
         for (unsigned t = 0; t < 16u; ++t) {
@@ -739,17 +759,10 @@ __global__ __launch_bounds__(kThreads) void kv8_weights_kernel(
             sum[t] += static_cast<int>(t) <= limit ? p : 0.0f;
         }
     }
-    // Over the 16 vectors, halving what a lane keeps: lane col ends with token
-    // col of its block.
-#pragma unroll
-    for (unsigned w = 8u; w >= 1u; w >>= 1) {
-        const bool upper = (col & w) != 0u;
-#pragma unroll
-        for (unsigned t = 0; t < w; ++t) {
-            const float keep = upper ? sum[t + w] : sum[t], give = upper ? sum[t] : sum[t + w];
-            sum[t] = keep + __shfl_xor(give, w);
-        }
-    }
+    halve<8>(sum, col);
+    halve<4>(sum, col);
+    halve<2>(sum, col);
+    halve<1>(sum, col);
     float mine = sum[0];
     if constexpr (SHARED) {
         shared_sum[wave][lane] = mine;
@@ -760,7 +773,7 @@ __global__ __launch_bounds__(kThreads) void kv8_weights_kernel(
         for (unsigned w = 0; w < kWaves; ++w) mine += shared_sum[w][lane];
     }
     if (vrec == nullptr || first + static_cast<int>(col) > last) return;
-    float* const at = reinterpret_cast<float*>(vrec + kKv8Weights) + col;
+    float* const at = (float*)(vrec + kKv8Weights) + col;
     if (add) {
         atomicAdd(at, mine);
     } else {
@@ -773,36 +786,32 @@ __global__ __launch_bounds__(kThreads) void kv8_weights_kernel(
 Kv8Shape kv8_attention_shape(std::uint32_t m, std::uint32_t q_heads, std::uint32_t kv_heads, std::uint32_t runs,
                              std::uint64_t max_tokens) {
     const std::uint32_t group = q_heads / kv_heads;
-    // Two rows a run on average share their keys; below that a tile is a row.
-    const bool by_run = runs != 0u && m >= 2u * runs;
-    const std::uint32_t tile = kVectors * (by_run ? kPromptTiles : 1u);
-    const std::uint32_t parts = (group + tile - 1u) / tile;
-    const std::uint32_t tile_rows = by_run && group < tile ? tile / group : 1u;
-    const std::uint32_t tiles = by_run ? m / tile_rows + runs : m;
     const std::uint32_t chunks = static_cast<std::uint32_t>((max_tokens + kChunkTokens - 1u) / kChunkTokens);
-#ifndef SHORT_CHUNKS
-#define SHORT_CHUNKS 32u
-#endif
-#ifndef SHORT_TILES
-#define SHORT_TILES 256u
-#endif
-    const std::uint64_t groups = static_cast<std::uint64_t>(by_run ? m / tile_rows + 1u : m) * kv_heads * parts;
-    if (!by_run && chunks <= SHORT_CHUNKS && groups <= SHORT_TILES) return Kv8Shape{tiles, kv_heads * parts, 1u, chunks, 0u, kShortWaves};
+    // Two rows a run on average share their keys; below that a tile is a row.
+    if (runs != 0u && m >= 2u * runs) {
+        const std::uint32_t tile = kVectors * kRunTiles, parts = (group + tile - 1u) / tile;
+        const std::uint32_t tile_rows = group < tile ? tile / group : 1u;
+        // Full tiles, and about one of them for each run's last rows.
+        const std::uint64_t groups = static_cast<std::uint64_t>(m / tile_rows + 1u) * kv_heads * parts;
+        std::uint64_t per = (groups * chunks + 511u) / 512u;
+        per = (per + kWaves - 1u) / kWaves * kWaves;
+        if (per < 2u * kWaves) per = 2u * kWaves;
+        if (per > chunks) per = chunks;
+        return Kv8Shape{m / tile_rows + runs, kv_heads * parts, static_cast<std::uint32_t>((chunks + per - 1u) / per),
+                        static_cast<std::uint32_t>(per), tile_rows, kKv8Runs};
+    }
+    const std::uint32_t parts = (group + kVectors - 1u) / kVectors;
+    const std::uint64_t groups = static_cast<std::uint64_t>(m) * kv_heads * parts;
+    if (chunks <= 32u && groups <= 256u) return Kv8Shape{m, kv_heads * parts, 1u, chunks, 0u, kKv8ShortRows};
     // Splits of equal length, so that rows of unequal lengths make workgroups
     // of equal work: at least two chunks a wave, and at most about four
     // workgroups a CU if every row were max_tokens long.
-#ifndef TARGET
-#define TARGET 1024u
-#endif
-#ifndef MINC
-#define MINC 2u
-#endif
-    std::uint64_t per = (groups * chunks + TARGET - 1u) / TARGET;
+    std::uint64_t per = (groups * chunks + 1023u) / 1024u;
     per = (per + kWaves - 1u) / kWaves * kWaves;
-    if (per < MINC * kWaves) per = MINC * kWaves;
+    if (per < 2u * kWaves) per = 2u * kWaves;
     if (per > chunks) per = chunks;
-    const std::uint32_t splits = static_cast<std::uint32_t>((chunks + per - 1u) / per);
-    return Kv8Shape{tiles, kv_heads * parts, splits, static_cast<std::uint32_t>(per), by_run ? tile_rows : 0u, kWaves};
+    return Kv8Shape{m, kv_heads * parts, static_cast<std::uint32_t>((chunks + per - 1u) / per),
+                    static_cast<std::uint32_t>(per), 0u, kKv8Rows};
 }
 
 std::uint64_t kv8_attention_scratch(const Kv8Shape& shape, std::uint32_t m, std::uint32_t q_heads,
@@ -838,11 +847,11 @@ void launch_typed(const Kv8Geometry& g, const float* qkv, std::uint64_t stride, 
     const std::uint32_t chunks = static_cast<std::uint32_t>((max_tokens + kChunkTokens - 1u) / kChunkTokens);
     const std::uint32_t columns = (chunks + kWaves - 1u) / kWaves;
     if (by_run) {
-        AIR_KV8_ATTENTION(kPromptTiles, true, kWaves);
-        if (split) AIR_KV8_MERGE(kPromptTiles, true);
+        AIR_KV8_ATTENTION(kRunTiles, true, kWaves);
+        if (split) AIR_KV8_MERGE(kRunTiles, true);
         if (weights) AIR_KV8_WEIGHTS(true, false, chunks);
     } else {
-        if (shape.waves == kShortWaves) AIR_KV8_ATTENTION(1u, false, kShortWaves);
+        if (shape.kernel == kKv8ShortRows) AIR_KV8_ATTENTION(1u, false, kShortWaves);
         else AIR_KV8_ATTENTION(1u, false, kWaves);
         if (weights && split) AIR_KV8_WEIGHTS(false, true, columns + 1u);
         else if (weights) AIR_KV8_WEIGHTS(false, false, columns);

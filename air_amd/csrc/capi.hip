@@ -2228,6 +2228,11 @@ int check_kv8_shape(const air_hip_kv8_layout* kv) {
         return fail(AIR_HIP_UNSUPPORTED, "8-bit KV tables of %u pages of %u tokens are too long", kv->max_pages,
                     kv->page_tokens);
     }
+    // 65535 layers and heads of 65536 tokens at most: no overflow in 64 bits.
+    if (static_cast<uint64_t>(kv->layers) * kv->kv_heads * per * kv8_record_bytes(kv) > 0xffffffffull) {
+        return fail(AIR_HIP_UNSUPPORTED, "a page of %u layers, %u KV heads and %u tokens is larger than 4 GiB", kv->layers,
+                    kv->kv_heads, kv->page_tokens);
+    }
     if (kv->pool_pages > static_cast<uint32_t>(INT32_MAX)) {
         return fail(AIR_HIP_INVALID_ARGUMENT, "8-bit KV pool pages must fit int32 page ids");
     }
@@ -2255,8 +2260,9 @@ Kv8Geometry kv8_geometry_of(const air_hip_kv8_layout* kv) {
     Kv8Geometry g{};
     g.pool = kv->chunks ? nullptr : static_cast<unsigned char*>(kv->pool);
     g.chunks = reinterpret_cast<unsigned char* const*>(kv->chunks);
-    g.page_bytes = kv8_page_bytes(kv);
+    g.page_bytes = static_cast<std::uint32_t>(kv8_page_bytes(kv));
     g.record_bytes = static_cast<std::uint32_t>(kv8_record_bytes(kv));
+    g.head_bytes = g.record_bytes * (kv->page_tokens / AIR_HIP_KV8_BLOCK_TOKENS);
     g.page_blocks = kv->page_tokens / AIR_HIP_KV8_BLOCK_TOKENS;
     g.page_magic = g.page_blocks == 1u ? 0u : static_cast<std::uint32_t>((1ull << 32) / g.page_blocks + 1u);
     g.max_pages = kv->max_pages;

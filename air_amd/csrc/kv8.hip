@@ -45,9 +45,10 @@ __device__ __forceinline__ float nan_f32() { return __builtin_nanf(""); }
 // K: (token, 16 dims), one 16-byte store each; threads [D, 2 D) own V: one
 // dim of all 16 tokens.  The magnitudes meet as the bit patterns of |x|,
 // whose unsigned order puts infinities and NaN above every finite value.
-// Latency bounds it (a decode step stores 2 KB a row): the block's codes and
-// scale and the row's own values are asked for before the other rows are
-// looked through, and in a decode step nothing else has to be read.
+// Latency bounds it (a decode step stores 2 KB a row, a prompt's 264 blocks
+// take 8 dependent loads): the block's codes and scale and the rows that a
+// decode step or a prompt stores in it (the next rows in the next slots) are
+// asked for before the other rows are looked through.
 template <int TYPE, unsigned D>
 __global__ __launch_bounds__(2 * D) void kv8_append_kernel(Kv8Geometry g, const float* __restrict__ qkv,
                                                            std::uint64_t stride, std::uint64_t q_width,
@@ -58,7 +59,7 @@ __global__ __launch_bounds__(2 * D) void kv8_append_kernel(Kv8Geometry g, const 
     constexpr unsigned kThreads = 2 * D;
     constexpr unsigned kAtOnce = 4;       // rows a thread looks through at a time
     __shared__ int winner[kKv8Block];
-    __shared__ int earlier, named;
+    __shared__ int earlier;
     __shared__ std::uint32_t wave_top[kThreads / 64];
     const std::uint32_t r = blockIdx.x, head = blockIdx.y;
     const unsigned tid = threadIdx.x;
@@ -107,22 +108,32 @@ __global__ __launch_bounds__(2 * D) void kv8_append_kernel(Kv8Geometry g, const 
     const std::uint32_t place = place_of(pos, slot);
     // In a prompt the row before names the same block for 15 of 16 rows.
     if (page_before == page && place_of(pos_before, slot_before) == place) return;
-    unsigned char* const rec = (unsigned char*)kv8_record_in(g, page, slot, layer, head,
-                                                             static_cast<std::uint32_t>(pos) / kKv8Block);
+    Kv8Byte* const rec = kv8_record_in(g, page, slot, layer, head, static_cast<std::uint32_t>(pos) / kKv8Block);
     if (rec == nullptr) return;
     const unsigned at = value ? kv8_v_offset(D, 0u, part) : kv8_k_offset(D, token, chunk * 16u);
-    u32x4* const codes_at = reinterpret_cast<u32x4*>(rec + at);
-    u32x4 codes = *codes_at;
-    float* const scale_at = reinterpret_cast<float*>(rec) + (value ? 1 : 0);
-    const float old_scale = *scale_at;
+    u32x4 codes = kv8_load<u32x4>(rec + at);
+    Kv8Byte* const scale_at = rec + (value ? 4 : 0);
+    const float old_scale = kv8_load<float>(scale_at);
+    const unsigned own = static_cast<std::uint32_t>(pos) % kKv8Block;
+    // The row that slot t takes if rows and slots go on together.
+    const auto next_row = [&](unsigned t) __attribute__((always_inline)) -> int {
+        return t >= own && t - own < m - r ? static_cast<int>(r + t - own) : -1;
+    };
     float x[16];
     if (value) {
-        x[0] = base[static_cast<std::uint64_t>(r) * stride + part];
+#pragma unroll
+        for (unsigned i = 0; i < 16u; ++i) {
+            const int row = next_row(i);
+            x[i] = row >= 0 ? base[static_cast<std::uint64_t>(row) * stride + part] : 0.0f;
+        }
+    } else if (const int row = next_row(token); row >= 0) {
+        load_row(static_cast<std::uint32_t>(row), x);
     } else {
-        load_row(r, x);
+#pragma unroll
+        for (unsigned i = 0; i < 16u; ++i) x[i] = 0.0f;
     }
     if (tid < kKv8Block) winner[tid] = -1;
-    if (tid == 0u) earlier = named = 0;
+    if (tid == 0u) earlier = 0;
     __syncthreads();
     const auto look_at = [&](std::uint32_t o, std::int32_t their_pos, std::int32_t their_page, std::uint32_t their_slot)
                              __attribute__((always_inline)) {
@@ -131,7 +142,6 @@ __global__ __launch_bounds__(2 * D) void kv8_append_kernel(Kv8Geometry g, const 
             earlier = 1;
         } else {
             atomicMax(&winner[static_cast<std::uint32_t>(their_pos) % kKv8Block], static_cast<int>(o));
-            if (o > r) named = 1;
         }
     };
     if (small) {
@@ -158,20 +168,16 @@ __global__ __launch_bounds__(2 * D) void kv8_append_kernel(Kv8Geometry g, const 
     if (earlier != 0) return;
     unsigned first = 0u;
     while (winner[first] < 0) ++first;   // row r itself is in
-    const unsigned own = static_cast<std::uint32_t>(pos) % kKv8Block;
-
     if (value) {
-        const float mine = x[0];
 #pragma unroll
         for (unsigned i = 0; i < 16u; ++i) {
             const int row = winner[i];
-            x[i] = i == own && named == 0 ? mine
-                   : row >= 0 && named != 0 ? base[static_cast<std::uint64_t>(row) * stride + part] : 0.0f;
+            if (row != next_row(i)) x[i] = row >= 0 ? base[static_cast<std::uint64_t>(row) * stride + part] : 0.0f;
         }
-    } else {
-        const int row = winner[token];
-        if (row >= 0 && static_cast<std::uint32_t>(row) != r) load_row(static_cast<std::uint32_t>(row), x);
-        if (row < 0) {
+    } else if (const int row = winner[token]; row != next_row(token)) {
+        if (row >= 0) {
+            load_row(static_cast<std::uint32_t>(row), x);
+        } else {
 #pragma unroll
             for (unsigned i = 0; i < 16u; ++i) x[i] = 0.0f;
         }
@@ -210,10 +216,10 @@ __global__ __launch_bounds__(2 * D) void kv8_append_kernel(Kv8Geometry g, const 
         }
         codes[i >> 2] = (codes[i >> 2] & ~(0xffu << shift)) | (now << shift);
     }
-    *codes_at = codes;
-    if (part == 0u) *scale_at = scale;
+    kv8_store(rec + at, codes);
+    if (part == 0u) kv8_store(scale_at, scale);
     if (tid < kKv8Block && winner[tid] >= 0) {
-        reinterpret_cast<float*>(rec + kKv8Weights)[tid] = 0.0f;   // a new token has gathered no weight
+        kv8_store(rec + kKv8Weights + 4u * tid, 0.0f);   // a new token has gathered no weight
     }
 }
 
@@ -238,8 +244,8 @@ __global__ __launch_bounds__(2 * D) void kv8_read_kernel(Kv8Geometry g, std::uin
     const std::int64_t block = start / kKv8Block + blockIdx.x;
     const std::int64_t base = block * kKv8Block;   // first token of the block
     if (base >= start + count || block > 0x7fffffff / static_cast<std::int64_t>(kKv8Block)) return;
-    const unsigned char* const rec = kv8_record(g, tables + static_cast<std::uint64_t>(seq) * g.max_pages, layer + l,
-                                                head, static_cast<std::uint32_t>(block));
+    const Kv8Byte* const rec = kv8_record(g, tables + static_cast<std::uint64_t>(seq) * g.max_pages, layer + l, head,
+                                          static_cast<std::uint32_t>(block));
     if (rec == nullptr) return;
     const bool value = threadIdx.x >= D;
     const unsigned part = value ? threadIdx.x - D : threadIdx.x;
@@ -248,11 +254,11 @@ __global__ __launch_bounds__(2 * D) void kv8_read_kernel(Kv8Geometry g, std::uin
     const std::uint64_t width = static_cast<std::uint64_t>(g.kv_heads) * D;
     float* const dst = value ? v : k;
     if (dst != nullptr) {
-        const float scale = reinterpret_cast<const float*>(rec)[value ? 1 : 0];
+        const float scale = kv8_load<float>(rec + (value ? 4 : 0));
         std::uint32_t c[4];   // of K a token's four dims, of V a dim's four tokens
 #pragma unroll
         for (unsigned i = 0; i < 4u; ++i) {
-            c[i] = *reinterpret_cast<const std::uint32_t*>(
+            c[i] = kv8_load<std::uint32_t>(
                 rec + (value ? kv8_v_offset(D, token0, dim + i) : kv8_k_offset(D, token0 + i, dim)));
         }
 #pragma unroll
@@ -278,7 +284,7 @@ __global__ __launch_bounds__(2 * D) void kv8_read_kernel(Kv8Geometry g, std::uin
         const std::int64_t t = base + threadIdx.x;
         if (t >= start && t < start + count) {
             weights[(row0 + static_cast<std::uint64_t>(t - start)) * g.kv_heads + head] =
-                reinterpret_cast<const float*>(rec + kKv8Weights)[threadIdx.x];
+                kv8_load<float>(rec + kKv8Weights + 4u * threadIdx.x);
         }
     }
 }
@@ -298,11 +304,11 @@ __global__ __launch_bounds__(256) void kv8_read_weights_kernel(Kv8Geometry g, st
     const std::int64_t start = starts ? starts[seq] : 0;
     const std::int64_t t = start + static_cast<std::int64_t>(j);
     if (j >= max_tokens || start < 0 || static_cast<std::int64_t>(j) >= lengths[seq] || t > 0x7fffffff) return;
-    const unsigned char* const rec = kv8_record(g, tables + static_cast<std::uint64_t>(seq) * g.max_pages, layer + l,
-                                                head, static_cast<std::uint32_t>(t / kKv8Block));
+    const Kv8Byte* const rec = kv8_record(g, tables + static_cast<std::uint64_t>(seq) * g.max_pages, layer + l, head,
+                                          static_cast<std::uint32_t>(t / kKv8Block));
     if (rec == nullptr) return;
     weights[((static_cast<std::uint64_t>(l) * seqs + seq) * max_tokens + j) * g.kv_heads + head] =
-        reinterpret_cast<const float*>(rec + kKv8Weights)[t % kKv8Block];
+        kv8_load<float>(rec + kKv8Weights + 4u * static_cast<std::uint32_t>(t % kKv8Block));
 }
 
 // ---- eviction ----------------------------------------------------------------
@@ -353,8 +359,8 @@ __global__ __launch_bounds__(kSelectThreads) void kv8_select_kernel(
         return;
     }
     const auto read_key = [&](std::uint32_t t) __attribute__((always_inline)) -> std::uint32_t {
-        const unsigned char* const rec = kv8_record(g, table, layer + l, head, t / kKv8Block);
-        return rec ? weight_key(reinterpret_cast<const float*>(rec + kKv8Weights)[t % kKv8Block]) : 0u;
+        const Kv8Byte* const rec = kv8_record(g, table, layer + l, head, t / kKv8Block);
+        return rec ? weight_key(kv8_load<float>(rec + kKv8Weights + 4u * (t % kKv8Block))) : 0u;
     };
     // The middle tokens are lo + i, i < count; more of them than are wanted.
     const std::uint32_t lo = keep_first, count = static_cast<std::uint32_t>(n - keep_last) - lo;
@@ -442,6 +448,12 @@ __global__ __launch_bounds__(kSelectThreads) void kv8_select_kernel(
 // block whose tokens come from one block keeps its codes, and others are
 // rounded once.  Threads as in the append; a token's source, scale and the
 // ratio its codes take are found once, by 16 threads for K and 16 for V.
+// With a quarter of the tokens kept nearly every 64-byte piece of the old
+// codes is touched: the old sequence is read whole (six layers of sequences
+// of 900..4100 tokens, 63 MB, and 25 MB written, in 33 us).  Measured slower:
+// four blocks a workgroup with their loads together (41 us), and 16 bytes a
+// dim and old block with the tokens picked from registers (52 us); fewer
+// workgroups a CU then cover each other's waits.
 // Where the new table is the old one (in place) a workgroup takes all blocks
 // in ascending order: block b's tokens come from blocks >= b, so what it
 // overwrites no later block reads, and it reads its 16 tokens before it
@@ -469,7 +481,7 @@ __global__ __launch_bounds__(2 * D) void kv8_compact_kernel(Kv8Geometry g, const
     if (in_place && list[budget - 1u] < static_cast<std::int32_t>(budget)) return;   // everything stays where it is
     for (std::uint32_t b = blockIdx.x; b < blocks; b += gridDim.x) {
         if (list[b * kKv8Block] < 0) return;   // no tokens from here on
-        unsigned char* const dst = kv8_record(g, new_table, layer + l, head, b);
+        unsigned char* const dst = (unsigned char*)kv8_record(g, new_table, layer + l, head, b);
         float weight = 0.0f;
         if (part < kKv8Block) {
             const std::uint32_t i = b * kKv8Block + part;
@@ -479,7 +491,7 @@ __global__ __launch_bounds__(2 * D) void kv8_compact_kernel(Kv8Geometry g, const
             unsigned slot = 0u;
             if (t >= 0) {
                 slot = static_cast<std::uint32_t>(t) % kKv8Block;
-                src = kv8_record(g, table, layer + l, head, static_cast<std::uint32_t>(t) / kKv8Block);
+                src = (const unsigned char*)kv8_record(g, table, layer + l, head, static_cast<std::uint32_t>(t) / kKv8Block);
                 if (src) {
                     s = reinterpret_cast<const float*>(src)[value ? 1 : 0];
                     weight = reinterpret_cast<const float*>(src + kKv8Weights)[slot];

@@ -28,8 +28,8 @@ def test_page_bytes():
     assert capi.kv8_page_bytes(lay) == 3 * 4 * 3 * (128 + 32 * 64)
     for field, bad in [("page_tokens", 24), ("page_tokens", 0), ("head_dim", 96), ("kv_heads", 0), ("layers", 0),
                        ("type", 0), ("type", 3), ("max_pages", 0), ("pool_pages", 0), ("max_pages", 2 ** 31),
-                       ("pool_pages", 2 ** 31), ("page_tokens", 65552)]:
-        broken = capi.Kv8Layout(None, 48, 4, 64, 3, 7, 9, None, 0, I8)
+                       ("pool_pages", 2 ** 31), ("page_tokens", 65552), ("layers", 65535)]:
+        broken = capi.Kv8Layout(None, 48, 12, 64, 3, 7, 9, None, 0, I8)
         setattr(broken, field, bad)
         assert capi.kv8_page_bytes(broken) == 0, (field, bad)
     assert capi.lib().air_hip_kv8_page_bytes(None) == 0
