@@ -422,18 +422,19 @@ hipError_t launch_kv8_evict(const Kv8Geometry& g, std::uint32_t seqs, const std:
 // The kernels of the attention: tiles of single rows, the same in one launch
 // of larger workgroups, and tiles of a run's rows.
 constexpr int kKv8Rows = 0, kKv8ShortRows = 1, kKv8Runs = 2;
-// How a call's attention is cut: `splits` workgroups of split_chunks 64-token
-// chunks over a tile's keys.
+// How a call's attention is cut into workgroups: of its (tile, heads) pairs
+// the first `whole` are one each, the others `splits` of split_chunks 64-token
+// chunks.
+struct Kv8Cut {
+    std::uint32_t pairs, whole, splits, split_chunks;
+};
 struct Kv8Shape {
-    std::uint32_t tiles;          // grid y
-    std::uint32_t tile_heads;     // grid x
-    std::uint32_t splits;         // grid z
-    std::uint32_t split_chunks;
-    std::uint32_t tile_rows;      // rows of one run a tile holds; 0: a tile is a row
+    Kv8Cut cut;
+    std::uint32_t tile_rows;      // rows of one run a tile holds
     int kernel;                   // kKv8Rows ..
 };
-Kv8Shape kv8_attention_shape(std::uint32_t m, std::uint32_t q_heads, std::uint32_t kv_heads, std::uint32_t runs,
-                             std::uint64_t max_tokens);
+Kv8Shape kv8_attention_shape(std::uint32_t m, std::uint32_t q_heads, std::uint32_t kv_heads, std::uint32_t head_dim,
+                             std::uint32_t runs, std::uint64_t max_tokens);
 // Bytes of scratch: the splits' partials and, with weights, the rows' softmax
 // statistics.
 std::uint64_t kv8_attention_scratch(const Kv8Shape& shape, std::uint32_t m, std::uint32_t q_heads,

@@ -317,6 +317,23 @@ __device__ __forceinline__ Tile find_tile(std::uint32_t index, const std::int32_
     return Tile{static_cast<std::uint32_t>(row), static_cast<std::uint32_t>(left < tile_rows ? left : tile_rows), 0u, 0u};
 }
 
+// The (tile, heads) pairs of a launch, one workgroup for each of the first
+// `whole` ones and `splits` of split_chunks chunks for each of the others.
+// The tiles count down: the last rows of a run reach furthest and start first.
+struct Kv8Work {
+    std::uint32_t tile, tile_head, split, split_chunks;
+};
+__device__ __forceinline__ Kv8Work kv8_work(const Kv8Cut& cut, std::uint32_t block, std::uint32_t tile_heads) {
+    std::uint32_t pair = block, split = 0u, chunks = 0x7fffffffu / kChunkTokens;   // more than any tile has
+    if (block >= cut.whole) {
+        const std::uint32_t pairs = cut.pairs - cut.whole;
+        pair = cut.whole + (block - cut.whole) % pairs;
+        split = (block - cut.whole) / pairs;
+        chunks = cut.split_chunks;
+    }
+    return Kv8Work{cut.pairs / tile_heads - 1u - pair / tile_heads, pair % tile_heads, split, chunks};
+}
+
 // A tile of up to 16 NV query vectors of one KV head per workgroup; its waves
 // take the chunks of split blockIdx.z in turn, every wave for all vectors.
 // With NV > 1 the vectors' operands lie in LDS, and a chunk's codes are turned
@@ -326,8 +343,8 @@ __global__ __launch_bounds__(64 * W, NV == 1u && W == kWaves ? 3 : 2) void kv8_a
     Kv8Geometry g, const float* __restrict__ qkv, std::uint64_t stride, std::uint32_t m,
     const std::int32_t* __restrict__ positions, const std::int32_t* __restrict__ tables, std::uint32_t layer,
     std::uint32_t q_heads, const std::int32_t* __restrict__ run_starts, std::uint32_t runs, std::uint32_t tile_rows,
-    std::uint64_t max_tokens, std::uint32_t split_chunks, float score_scale, float* __restrict__ partials,
-    float2* __restrict__ stats, float* __restrict__ out) {
+    std::uint64_t max_tokens, Kv8Cut cut, float score_scale, float* __restrict__ partials, float2* __restrict__ stats,
+    float* __restrict__ out) {
     constexpr unsigned LD = D + 4;
     constexpr unsigned kTile = kVectors * NV;
     constexpr unsigned kFrags = D / 32;            // k steps of a score
@@ -340,13 +357,12 @@ __global__ __launch_bounds__(64 * W, NV == 1u && W == kWaves ? 3 : 2) void kv8_a
     __shared__ int wave_m[W][kTile], wave_m2[W][kTile];
     __shared__ float wave_l[W][kTile];
     const unsigned tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, grp = lane >> 4, col = lane & 15u;
-    const std::uint32_t split = blockIdx.z;
     const std::uint32_t group = q_heads / g.kv_heads, parts = (group + kTile - 1u) / kTile;
-    const std::uint32_t kvh = blockIdx.x / parts, part = blockIdx.x % parts;
-    // The last rows of a run reach furthest: they start first.
-    const std::uint32_t index = gridDim.y - 1u - blockIdx.y;
-    Tile tile{index, 1u, 0u, 0u};
-    if constexpr (RUNS) tile = find_tile(index, run_starts, runs, m, tile_rows);
+    const Kv8Work work = kv8_work(cut, blockIdx.x, g.kv_heads * parts);
+    const std::uint32_t split = work.split, split_chunks = work.split_chunks;
+    const std::uint32_t kvh = work.tile_head / parts, part = work.tile_head % parts;
+    Tile tile{work.tile, 1u, 0u, 0u};
+    if constexpr (RUNS) tile = find_tile(work.tile, run_starts, runs, m, tile_rows);
     if (tile.rows == 0u) return;
     tile.head = kvh * group + part * kTile;
     tile.heads = group - part * kTile < kTile ? group - part * kTile : kTile;
@@ -445,15 +461,12 @@ __global__ __launch_bounds__(64 * W, NV == 1u && W == kWaves ? 3 : 2) void kv8_a
 #pragma unroll
                 for (unsigned i = 0; i < kFrags / 2u; ++i) codes_to_half<TYPE>(keys.c[b][i], a[2u * i], a[2u * i + 1u]);
 #pragma unroll
-                for (unsigned n = 0; n < NV; ++n) s[n][b] = float4v{0.f, 0.f, 0.f, 0.f};
+                for (unsigned n = 0; n < NV; ++n) {
+                    s[n][b] = float4v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (unsigned h = 0; h < 2u; ++h) {       // low parts first
-#pragma unroll
-                    for (unsigned i = 0; i < kFrags; ++i) {
-#pragma unroll
-                        for (unsigned n = 0; n < NV; ++n) {
-                            s[n][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i], sh.query[n][i][h][lane], s[n][b], 0, 0, 0);
-                        }
+                    for (unsigned i = 0; i < 2u * kFrags; ++i) {   // low parts first
+                        s[n][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i % kFrags], sh.query[n][i % kFrags][i / kFrags][lane],
+                                                                         s[n][b], 0, 0, 0);
                     }
                 }
             }
@@ -484,9 +497,11 @@ __global__ __launch_bounds__(64 * W, NV == 1u && W == kWaves ? 3 : 2) void kv8_a
             half8v a[2];
             codes_to_half<TYPE>(vals[t], a[0], a[1]);
 #pragma unroll
-            for (unsigned i = 0; i < 4u; ++i) {
+            for (unsigned n = 0; n < NV; ++n) {
+                // One accumulator's products in a row: an MFMA takes 19.5
+                // cycles so, 22.6 with two accumulators in turn, 26 with four.
 #pragma unroll
-                for (unsigned n = 0; n < NV; ++n) {
+                for (unsigned i = 0; i < 4u; ++i) {
                     const half8v f = i < 2u ? p_lo[n][i] : p_hi[n][i - 2u];
                     o[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i & 1u], f, o[n][t], 0, 0, 0);
                 }
@@ -538,7 +553,7 @@ __global__ __launch_bounds__(64 * W, NV == 1u && W == kWaves ? 3 : 2) void kv8_a
             *reinterpret_cast<float4v*>(out + vector * D + 4u * d4) = y;
             if (stats && d4 == 0u) stats[vector] = make_float2(static_cast<float>(mm), total == 0.0f ? 0.0f : 1.0f / total);
         } else {
-            float* const p = partials + (vector * gridDim.z + split) * (D + kStat);
+            float* const p = partials + (vector * cut.splits + split) * (D + kStat);
             if (d4 == 0u) *reinterpret_cast<float4v*>(p) = float4v{__int_as_float(mm), __int_as_float(mm2), total, 0.0f};
             *reinterpret_cast<float4v*>(p + kStat + 4u * d4) = acc;
         }
@@ -597,13 +612,13 @@ template <unsigned D, unsigned NV, bool RUNS>
 __global__ __launch_bounds__(kThreads) void kv8_merge_kernel(
     const std::int32_t* __restrict__ positions, std::uint32_t m, std::uint32_t q_heads, std::uint32_t kv_heads,
     const std::int32_t* __restrict__ run_starts, std::uint32_t runs, std::uint32_t tile_rows, std::uint64_t max_tokens,
-    std::uint32_t split_chunks, std::uint32_t splits, const float* __restrict__ partials, float2* __restrict__ stats,
-    float* __restrict__ out) {
+    Kv8Cut cut, const float* __restrict__ partials, float2* __restrict__ stats, float* __restrict__ out) {
     constexpr unsigned kTile = kVectors * NV;
     const std::uint32_t group = q_heads / kv_heads, parts = (group + kTile - 1u) / kTile;
-    const std::uint32_t kvh = blockIdx.x / parts, part = blockIdx.x % parts;
-    Tile tile{blockIdx.y, 1u, 0u, 0u};
-    if constexpr (RUNS) tile = find_tile(blockIdx.y, run_starts, runs, m, tile_rows);
+    const Kv8Work work = kv8_work(cut, cut.whole + blockIdx.x, kv_heads * parts);
+    const std::uint32_t kvh = work.tile_head / parts, part = work.tile_head % parts;
+    Tile tile{work.tile, 1u, 0u, 0u};
+    if constexpr (RUNS) tile = find_tile(work.tile, run_starts, runs, m, tile_rows);
     if (tile.rows == 0u) return;
     tile.head = kvh * group + part * kTile;
     tile.heads = group - part * kTile < kTile ? group - part * kTile : kTile;
@@ -612,10 +627,10 @@ __global__ __launch_bounds__(kThreads) void kv8_merge_kernel(
         const int p = positions[tile.row + r];
         reach = p > reach ? p : reach;
     }
-    const std::uint32_t live = live_splits(reach, max_tokens, split_chunks);
+    const std::uint32_t live = live_splits(reach, max_tokens, cut.split_chunks), splits = cut.splits;
     if (live <= 1u) return;   // the attention kernel wrote this tile
-    for (unsigned idx = blockIdx.z * kThreads + threadIdx.x; idx < tile.rows * tile.heads * (D / 4u);
-         idx += gridDim.z * kThreads) {
+    for (unsigned idx = blockIdx.y * kThreads + threadIdx.x; idx < tile.rows * tile.heads * (D / 4u);
+         idx += gridDim.y * kThreads) {
         const unsigned v = idx / (D / 4u), d4 = idx % (D / 4u);
         const std::uint64_t vector =
             static_cast<std::uint64_t>(tile.row + v / tile.heads) * q_heads + tile.head + v % tile.heads;
@@ -783,42 +798,58 @@ __global__ __launch_bounds__(kThreads, 3) void kv8_weights_kernel(
 
 } // namespace
 
-Kv8Shape kv8_attention_shape(std::uint32_t m, std::uint32_t q_heads, std::uint32_t kv_heads, std::uint32_t runs,
-                             std::uint64_t max_tokens) {
+Kv8Shape kv8_attention_shape(std::uint32_t m, std::uint32_t q_heads, std::uint32_t kv_heads, std::uint32_t head_dim,
+                             std::uint32_t runs, std::uint64_t max_tokens) {
     const std::uint32_t group = q_heads / kv_heads;
     const std::uint32_t chunks = static_cast<std::uint32_t>((max_tokens + kChunkTokens - 1u) / kChunkTokens);
     // Two rows a run on average share their keys; below that a tile is a row.
     if (runs != 0u && m >= 2u * runs) {
         const std::uint32_t tile = kVectors * kRunTiles, parts = (group + tile - 1u) / tile;
         const std::uint32_t tile_rows = group < tile ? tile / group : 1u;
-        // Full tiles, and about one of them for each run's last rows.
-        const std::uint64_t groups = static_cast<std::uint64_t>(m / tile_rows + 1u) * kv_heads * parts;
-        std::uint64_t per = (groups * chunks + 511u) / 512u;
-        per = (per + kWaves - 1u) / kWaves * kWaves;
-        if (per < 2u * kWaves) per = 2u * kWaves;
-        if (per > chunks) per = chunks;
-        return Kv8Shape{m / tile_rows + runs, kv_heads * parts, static_cast<std::uint32_t>((chunks + per - 1u) / per),
-                        static_cast<std::uint32_t>(per), tile_rows, kKv8Runs};
+        const std::uint64_t pairs = (static_cast<std::uint64_t>(m / tile_rows) + runs) * kv_heads * parts;
+        // Workgroups that run at a time: two a CU, with the registers of two
+        // MFMA tiles of 128 dims, or three.  What fills them is not cut; the
+        // pairs left over are, so that they fill them once more together.
+        const std::uint64_t slots = head_dim == 128u ? 512u : 768u;
+        const std::uint64_t whole = chunks >= 4u * kWaves ? pairs / slots * slots : pairs;
+        std::uint64_t per = chunks;
+        if (pairs > whole) {
+            const std::uint64_t splits = slots / (pairs - whole);
+            per = (chunks + splits - 1u) / splits;
+            per = (per + kWaves - 1u) / kWaves * kWaves;
+            if (per < 2u * kWaves) per = 2u * kWaves;
+            if (per > chunks) per = chunks;
+        }
+        const std::uint32_t splits = static_cast<std::uint32_t>((chunks + per - 1u) / per);
+        return Kv8Shape{{static_cast<std::uint32_t>(pairs), static_cast<std::uint32_t>(splits > 1u ? whole : 0u), splits,
+                         static_cast<std::uint32_t>(per)},
+                        tile_rows, kKv8Runs};
     }
     const std::uint32_t parts = (group + kVectors - 1u) / kVectors;
-    const std::uint64_t groups = static_cast<std::uint64_t>(m) * kv_heads * parts;
-    if (chunks <= 32u && groups <= 256u) return Kv8Shape{m, kv_heads * parts, 1u, chunks, 0u, kKv8ShortRows};
+    const std::uint64_t pairs = static_cast<std::uint64_t>(m) * kv_heads * parts;
+    const auto shape = [&](std::uint64_t per, int kernel) {
+        return Kv8Shape{{static_cast<std::uint32_t>(pairs), 0u, static_cast<std::uint32_t>((chunks + per - 1u) / per),
+                         static_cast<std::uint32_t>(per)},
+                        0u, kernel};
+    };
+    // Few short rows: eight waves a workgroup walk a row's chunks in at most
+    // four turns, without a second launch (32 rows over 500..1200 tokens: 11.2
+    // us against 14; over 3000..4000 tokens 30 us against 19 with splits).
+    if (chunks <= 32u && pairs <= 256u) return shape(chunks, kKv8ShortRows);
     // Splits of equal length, so that rows of unequal lengths make workgroups
     // of equal work: at least two chunks a wave, and at most about four
     // workgroups a CU if every row were max_tokens long.
-    std::uint64_t per = (groups * chunks + 1023u) / 1024u;
+    std::uint64_t per = (pairs * chunks + 1023u) / 1024u;
     per = (per + kWaves - 1u) / kWaves * kWaves;
     if (per < 2u * kWaves) per = 2u * kWaves;
-    if (per > chunks) per = chunks;
-    return Kv8Shape{m, kv_heads * parts, static_cast<std::uint32_t>((chunks + per - 1u) / per),
-                    static_cast<std::uint32_t>(per), 0u, kKv8Rows};
+    return shape(per > chunks ? chunks : per, kKv8Rows);
 }
 
 std::uint64_t kv8_attention_scratch(const Kv8Shape& shape, std::uint32_t m, std::uint32_t q_heads,
                                     std::uint32_t head_dim, bool weights) {
     const std::uint64_t vectors = static_cast<std::uint64_t>(m) * q_heads;
     const std::uint64_t stats = weights ? (vectors * sizeof(float2) + 255u) / 256u * 256u : 0u;
-    return stats + (shape.splits > 1u ? vectors * shape.splits * (head_dim + kStat) * sizeof(float) : 0u);
+    return stats + (shape.cut.splits > 1u ? vectors * shape.cut.splits * (head_dim + kStat) * sizeof(float) : 0u);
 }
 
 namespace {
@@ -830,20 +861,22 @@ void launch_typed(const Kv8Geometry& g, const float* qkv, std::uint64_t stride, 
                   const Kv8Shape& shape, float* partials, float2* stats, float* out, hipStream_t stream) {
     // Scores in powers of two: s log2(e) = (q . k) * log2(e) / sqrt(D).
     const float scale = static_cast<float>(1.4426950408889634 / __builtin_sqrt(static_cast<double>(D)));
-    const bool split = shape.splits > 1u, by_run = shape.tile_rows != 0u;
-    const dim3 grid(shape.tile_heads, shape.tiles, shape.splits), merge_grid(shape.tile_heads, shape.tiles, by_run ? 4u : 1u);
+    const Kv8Cut& cut = shape.cut;
+    const bool split = cut.splits > 1u, by_run = shape.kernel == kKv8Runs;
+    const dim3 grid(cut.whole + (cut.pairs - cut.whole) * cut.splits);
+    // A tile of several MFMA tiles is joined by several workgroups.
+    const dim3 merge_grid(cut.pairs - cut.whole, by_run ? 4u : 1u);
 #define AIR_KV8_ATTENTION(NV, RUNS, W)                                                                               \
     hipLaunchKernelGGL((kv8_attention_kernel<TYPE, D, NV, RUNS, W>), grid, dim3(64 * W), 0, stream, g, qkv, stride, m, \
-                       positions, tables, layer, q_heads, run_starts, runs, shape.tile_rows, max_tokens,             \
-                       shape.split_chunks, scale, partials, stats, out)
+                       positions, tables, layer, q_heads, run_starts, runs, shape.tile_rows, max_tokens, cut, scale, \
+                       partials, stats, out)
 #define AIR_KV8_MERGE(NV, RUNS)                                                                                      \
     hipLaunchKernelGGL((kv8_merge_kernel<D, NV, RUNS>), merge_grid, dim3(kThreads), 0, stream, positions, m, q_heads, \
-                       g.kv_heads, run_starts, runs, shape.tile_rows, max_tokens, shape.split_chunks, shape.splits,  \
-                       partials, stats, out)
+                       g.kv_heads, run_starts, runs, shape.tile_rows, max_tokens, cut, partials, stats, out)
 #define AIR_KV8_WEIGHTS(SHARED, MERGE, COLUMNS)                                                                      \
     hipLaunchKernelGGL((kv8_weights_kernel<TYPE, D, SHARED, MERGE>), dim3(COLUMNS, g.kv_heads, run_starts ? runs : m), \
                        dim3(kThreads), 0, stream, g, qkv, stride, m, positions, tables, layer, q_heads, run_starts,  \
-                       max_tokens, scale, stats, weights == 1, shape.split_chunks, shape.splits, partials, out)
+                       max_tokens, scale, stats, weights == 1, cut.split_chunks, cut.splits, partials, out)
     const std::uint32_t chunks = static_cast<std::uint32_t>((max_tokens + kChunkTokens - 1u) / kChunkTokens);
     const std::uint32_t columns = (chunks + kWaves - 1u) / kWaves;
     if (by_run) {
