@@ -132,6 +132,26 @@ __device__ __forceinline__ void load_query(const float* q, unsigned grp, QueryFr
     }
 }
 
+// A vector's operands, kept for the kernel that gathers weights: 16 bytes of
+// lane group grp at (2 i + part) * 4 + grp, so that a load takes 64 bytes of a
+// vector together.
+template <unsigned D>
+__device__ __forceinline__ void keep_query(half8v* at, unsigned grp, const QueryFragments<D>& f) {
+#pragma unroll
+    for (unsigned i = 0; i < D / 32u; ++i) {
+        at[8u * i + grp] = f.lo[i];
+        at[8u * i + 4u + grp] = f.hi[i];
+    }
+}
+template <unsigned D>
+__device__ __forceinline__ void kept_query(const half8v* at, unsigned grp, QueryFragments<D>& f) {
+#pragma unroll
+    for (unsigned i = 0; i < D / 32u; ++i) {
+        f.lo[i] = at[8u * i + grp];
+        f.hi[i] = at[8u * i + 4u + grp];
+    }
+}
+
 // A lane's codes of the chunk's K: tile b, 64-dim step s.
 template <unsigned D>
 struct KeyCodes {
@@ -344,7 +364,7 @@ __global__ __launch_bounds__(64 * W, NV == 1u && W == kWaves ? 3 : 2) void kv8_a
     const std::int32_t* __restrict__ positions, const std::int32_t* __restrict__ tables, std::uint32_t layer,
     std::uint32_t q_heads, const std::int32_t* __restrict__ run_starts, std::uint32_t runs, std::uint32_t tile_rows,
     std::uint64_t max_tokens, Kv8Cut cut, float score_scale, float* __restrict__ partials, float2* __restrict__ stats,
-    float* __restrict__ out) {
+    half8v* __restrict__ queries, float* __restrict__ undos, float* __restrict__ out) {
     constexpr unsigned LD = D + 4;
     constexpr unsigned kTile = kVectors * NV;
     constexpr unsigned kFrags = D / 32;            // k steps of a score
@@ -408,7 +428,14 @@ __global__ __launch_bounds__(64 * W, NV == 1u && W == kWaves ? 3 : 2) void kv8_a
                 sh.query[n][i][0][lane] = q.lo[i];
                 sh.query[n][i][1][lane] = q.hi[i];
             }
-            if (grp == 0u) undo_of[n * kVectors + col] = q.undo;
+            const unsigned v = n * kVectors + col;
+            if (grp == 0u) undo_of[v] = q.undo;
+            if (queries && split == 0u && v < nq) {   // for the weights
+                const std::uint64_t vector =
+                    static_cast<std::uint64_t>(tile.row + v / tile.heads) * q_heads + tile.head + v % tile.heads;
+                keep_query<D>(queries + vector * (D / 4u), grp, q);
+                if (grp == 0u) undos[vector] = q.undo;
+            }
         }
         __syncthreads();
 #pragma unroll
@@ -654,26 +681,68 @@ __device__ __forceinline__ void halve(float (&sum)[16], unsigned col) {
     }
 }
 
+// The last position of rows begin..end - 1, at most `most`, in every lane.
+__device__ __forceinline__ int last_position(const std::int32_t* __restrict__ positions, std::int64_t begin,
+                                             std::int64_t end, unsigned lane, int most) {
+    int last = -1;
+    for (std::int64_t r = begin + lane; r < end; r += 64) last = positions[r] > last ? positions[r] : last;
+    for (int off = 32; off > 0; off >>= 1) {
+        const int o = __shfl_xor(last, off);
+        last = o > last ? o : last;
+    }
+    return last < most ? last : most;
+}
+
+// A token's weight to its record, if the token is held.
+__device__ __forceinline__ void put_weight(Kv8Byte* record, int first, int last, unsigned col, float weight, bool add) {
+    if (record == nullptr || first + static_cast<int>(col) > last) return;
+    float* const at = (float*)(record + kKv8Weights) + col;
+    if (add) {
+        atomicAdd(at, weight);
+    } else {
+        *at = weight;
+    }
+}
+
+// A chunk's records: each lane looks one of the four blocks up (so two loads
+// follow on each other, not four), of which `page` is the page, and the wave
+// shares them.
+struct ChunkRecords {
+    Kv8Byte* key;      // of the block whose K this lane loads
+    Kv8Byte* value;    // of block lane / 16
+};
+
+__device__ __forceinline__ ChunkRecords chunk_records(const Kv8Geometry& g, std::int32_t page, std::uint32_t slot,
+                                                      std::uint32_t layer, std::uint32_t kvh, std::uint32_t chunk,
+                                                      unsigned lane) {
+    Kv8Byte* const mine = kv8_record_in(g, page, slot, layer, kvh, chunk * kChunkBlocks + (lane & 3u));
+    const std::uint64_t address = reinterpret_cast<std::uint64_t>((unsigned char*)mine);
+    const int low = static_cast<int>(address), high = static_cast<int>(address >> 32);
+    const auto of = [&](unsigned b) __attribute__((always_inline)) {
+        const std::uint64_t h = static_cast<std::uint32_t>(__shfl(high, b));
+        return (Kv8Byte*)(h << 32 | static_cast<std::uint32_t>(__shfl(low, b)));
+    };
+    return ChunkRecords{of((lane & 15u) >> 2), of(lane >> 4)};
+}
+
 // The weights a run's rows give one chunk of tokens: the scores again, by the
 // same instructions as in the attention, and p from the rows' statistics
-// (M and 1 / l).  A chunk of a (run, KV head) is one wave's, or with SHARED,
-// for runs of many vectors, the four waves' of a workgroup, which take the
-// vectors in turn and add up in LDS.  It adds with one atomic a token: a page
-// that two runs share loses nothing, and elsewhere a single addition leaves
-// one order.  Reading K again takes half of the attention's bytes; keeping
-// the scores would take 4 bytes a vector and token, written and read.
+// (M and 1 / l).  Reading K again takes half of the attention's bytes; keeping
+// the scores would take 4 bytes a vector and token, written and read.  Each
+// token takes one atomic addition: a page that two runs share loses nothing,
+// and elsewhere a single addition leaves one order.
 //
-// MERGE, for tiles of single rows that were split: the grid's first column
-// joins the splits of a run's rows, and the others take the statistics from
-// the partials themselves, so that one launch follows the attention.
-template <int TYPE, unsigned D, bool SHARED, bool MERGE>
+// For tiles of single rows: a chunk of a (run, KV head) is one wave's.  MERGE,
+// where they were split: the grid's first column joins the splits of a run's
+// rows, and the others take the statistics from the partials themselves, so
+// that one launch follows the attention.
+template <int TYPE, unsigned D, bool MERGE>
 __global__ __launch_bounds__(kThreads, 3) void kv8_weights_kernel(
     Kv8Geometry g, const float* __restrict__ qkv, std::uint64_t stride, std::uint32_t m,
     const std::int32_t* __restrict__ positions, const std::int32_t* __restrict__ tables, std::uint32_t layer,
     std::uint32_t q_heads, const std::int32_t* __restrict__ run_starts, std::uint64_t max_tokens, float score_scale,
     const float2* __restrict__ stats, bool add, std::uint32_t split_chunks, std::uint32_t splits,
     const float* __restrict__ partials, float* __restrict__ out) {
-    __shared__ float shared_sum[SHARED ? kWaves : 1u][kChunkTokens];
     const unsigned tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, grp = lane >> 4, col = lane & 15u;
     const std::uint32_t kvh = blockIdx.y, run = blockIdx.z;
     std::int64_t begin = run, end = static_cast<std::int64_t>(run) + 1;
@@ -702,28 +771,25 @@ __global__ __launch_bounds__(kThreads, 3) void kv8_weights_kernel(
         return;
     }
     const std::uint32_t column = blockIdx.x - (MERGE ? 1u : 0u);
-    const std::uint32_t chunk = SHARED ? column : column * kWaves + wave;
+    const std::uint32_t chunk = column * kWaves + wave;
     const int token0 = static_cast<int>(chunk * kChunkTokens);
     const std::int32_t* const table = tables + static_cast<std::uint64_t>(row0) * g.max_pages;
+    const std::uint32_t slot = kv8_slot(g, chunk * kChunkBlocks + (lane & 3u));
+    const std::int32_t page = slot < g.max_pages ? table[slot] : -1;
     // Tokens past the run's last position (or max_tokens) are not held.
     const int most = static_cast<int>(max_tokens) - 1;
-    int last = -1;
-    for (std::int64_t r = begin + lane; r < end; r += 64) last = positions[r] > last ? positions[r] : last;
-    for (int off = 32; off > 0; off >>= 1) {
-        const int o = __shfl_xor(last, off);
-        last = o > last ? o : last;
-    }
-    last = last < most ? last : most;
-    if (token0 > last) return;   // all of a workgroup's waves, where they share a chunk
+    const int last = last_position(positions, begin, end, lane, most);
+    if (token0 > last) return;
     const Kv8Byte* const none = (const Kv8Byte*)g_no_record;
-    const Kv8Byte* const krec = kv8_record(g, table, layer, kvh, chunk * kChunkBlocks + (col >> 2));
-    Kv8Byte* const vrec = kv8_record(g, table, layer, kvh, chunk * kChunkBlocks + grp);
+    const ChunkRecords at = chunk_records(g, page, slot, layer, kvh, chunk, lane);
+    const Kv8Byte* const krec = at.key;
+    Kv8Byte* const vrec = at.value;
     KeyCodes<D> keys;
     load_keys<D>(krec ? krec : none, lane, keys);
     const float k_scale = load_scales(vrec ? vrec : none).x;
     const int first = token0 + static_cast<int>(grp * kKv8Block);
     float sum[16] = {};
-    for (std::uint32_t v0 = SHARED ? wave * kVectors : 0u; v0 < vectors; v0 += (SHARED ? kWaves : 1u) * kVectors) {
+    for (std::uint32_t v0 = 0u; v0 < vectors; v0 += kVectors) {
         const std::uint32_t v = v0 + col;
         const bool active = v < vectors;
         const std::uint32_t r = row0 + (active ? v / group : 0u);
@@ -778,22 +844,113 @@ __global__ __launch_bounds__(kThreads, 3) void kv8_weights_kernel(
     halve<4>(sum, col);
     halve<2>(sum, col);
     halve<1>(sum, col);
-    float mine = sum[0];
-    if constexpr (SHARED) {
-        shared_sum[wave][lane] = mine;
-        __syncthreads();
-        if (wave != 0u) return;
-        mine = 0.0f;
+    put_weight(vrec, first, last, col, sum[0], add);
+}
+
+// The same for runs of several rows: a chunk is a workgroup's, whose waves take
+// the vectors 16 at a time in turn and add up in LDS.  The attention left the
+// vectors' operands, and a wave reads 16 vectors ahead (four runs of 32 rows
+// over 2900..4100 tokens, 28 q heads on 4 KV heads of 128 dims: 30 us where
+// every chunk made the operands anew, 25 reading them, 22.7 reading ahead and
+// with K's codes as f16 in registers for all vectors).
+template <int TYPE, unsigned D>
+__global__ __launch_bounds__(kThreads, 2) void kv8_run_weights_kernel(
+    Kv8Geometry g, std::uint32_t m, const std::int32_t* __restrict__ positions, const std::int32_t* __restrict__ tables,
+    std::uint32_t layer, std::uint32_t q_heads, const std::int32_t* __restrict__ run_starts, std::uint64_t max_tokens,
+    float score_scale, const float2* __restrict__ stats, const half8v* __restrict__ queries,
+    const float* __restrict__ undos, bool add) {
+    __shared__ float shared_sum[kWaves][kChunkTokens];
+    const unsigned tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, grp = lane >> 4, col = lane & 15u;
+    const std::uint32_t kvh = blockIdx.y, run = blockIdx.z, chunk = blockIdx.x;
+    std::int64_t begin = run_starts[run], end = run_starts[run + 1u];
+    begin = begin < 0 ? 0 : begin;
+    end = end > static_cast<std::int64_t>(m) ? static_cast<std::int64_t>(m) : end;
+    if (begin >= end) return;
+    const std::uint32_t group = q_heads / g.kv_heads;
+    const std::uint32_t vectors = static_cast<std::uint32_t>(end - begin) * group;
+    const std::uint32_t row0 = static_cast<std::uint32_t>(begin), head0 = kvh * group;
+    const std::int32_t* const table = tables + static_cast<std::uint64_t>(row0) * g.max_pages;
+    const std::uint32_t slot = kv8_slot(g, chunk * kChunkBlocks + (lane & 3u));
+    const std::int32_t page = slot < g.max_pages ? table[slot] : -1;
+    // Tokens past the run's last position (or max_tokens) are not held.
+    const int most = static_cast<int>(max_tokens) - 1;
+    const int last = last_position(positions, begin, end, lane, most);
+    const int token0 = static_cast<int>(chunk * kChunkTokens);
+    if (token0 > last) return;   // all of the workgroup's waves
+    const ChunkRecords at = chunk_records(g, page, slot, layer, kvh, chunk, lane);
+    const Kv8Byte* const none = (const Kv8Byte*)g_no_record;
+    half8v a[4][D / 32];
+    {
+        KeyCodes<D> keys;
+        load_keys<D>(at.key ? (const Kv8Byte*)at.key : none, lane, keys);
 #pragma unroll
-        for (unsigned w = 0; w < kWaves; ++w) mine += shared_sum[w][lane];
+        for (unsigned b = 0; b < 4u; ++b) {
+#pragma unroll
+            for (unsigned i = 0; i < D / 64u; ++i) codes_to_half<TYPE>(keys.c[b][i], a[b][2u * i], a[b][2u * i + 1u]);
+        }
     }
-    if (vrec == nullptr || first + static_cast<int>(col) > last) return;
-    float* const at = (float*)(vrec + kKv8Weights) + col;
-    if (add) {
-        atomicAdd(at, mine);
-    } else {
-        *at = mine;
+    const float k_scale = load_scales(at.value ? (const Kv8Byte*)at.value : none).x;
+    const int first = token0 + static_cast<int>(grp * kKv8Block);
+    float sum[16] = {};
+    struct Vector {
+        QueryFragments<D> q;
+        float2 st;
+        int upto;
+    };
+    const auto fetch = [&](std::uint32_t v0, Vector& x) __attribute__((always_inline)) {
+        const bool active = v0 + col < vectors;   // places without a vector repeat the first
+        const std::uint32_t v = active ? v0 + col : 0u, r = row0 + v / group;
+        const std::uint64_t vector = static_cast<std::uint64_t>(r) * q_heads + head0 + v % group;
+        x.upto = positions[r];
+        x.st = stats[vector];
+        x.q.undo = undos[vector];
+        kept_query<D>(queries + vector * (D / 4u), grp, x.q);
+    };
+    Vector now;
+    fetch(wave * kVectors, now);
+    for (std::uint32_t v0 = wave * kVectors; v0 < vectors; v0 += kWaves * kVectors) {
+        Vector next;
+        fetch(v0 + kWaves * kVectors, next);
+        const int upto = v0 + col < vectors ? (now.upto < most ? now.upto : most) : -1;
+        const int limit = at.value == nullptr ? -1 : upto - first;
+        if (__any(limit >= 0)) {
+            float4v s[4];
+#pragma unroll
+            for (unsigned b = 0; b < 4u; ++b) {
+                s[b] = float4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (unsigned i = 0; i < D / 16u; ++i) {   // low parts first
+                    s[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[b][i % (D / 32u)], i < D / 32u ? now.q.lo[i] : now.q.hi[i - D / 32u],
+                                                                  s[b], 0, 0, 0);
+                }
+            }
+            const float factor = score_factor(now.q.undo * score_scale, k_scale);
+            if (__all(limit >= 15)) {
+#pragma unroll
+                for (unsigned t = 0; t < 16u; ++t) {
+                    sum[t] = __builtin_fmaf(score_power(s[t >> 2][t & 3u], factor, now.st.x), now.st.y, sum[t]);
+                }
+            } else {
+#pragma unroll
+                for (unsigned t = 0; t < 16u; ++t) {
+                    const float p = score_power(s[t >> 2][t & 3u], factor, now.st.x);
+                    sum[t] = static_cast<int>(t) <= limit ? __builtin_fmaf(p, now.st.y, sum[t]) : sum[t];
+                }
+            }
+        }
+        now = next;
     }
+    halve<8>(sum, col);
+    halve<4>(sum, col);
+    halve<2>(sum, col);
+    halve<1>(sum, col);
+    shared_sum[wave][lane] = sum[0];
+    __syncthreads();
+    if (wave != 0u) return;
+    float mine = 0.0f;
+#pragma unroll
+    for (unsigned w = 0; w < kWaves; ++w) mine += shared_sum[w][lane];
+    put_weight(at.value, first, last, col, mine, add);
 }
 
 } // namespace
@@ -809,12 +966,16 @@ Kv8Shape kv8_attention_shape(std::uint32_t m, std::uint32_t q_heads, std::uint32
         const std::uint64_t pairs = (static_cast<std::uint64_t>(m / tile_rows) + runs) * kv_heads * parts;
         // Workgroups that run at a time: two a CU, with the registers of two
         // MFMA tiles of 128 dims, or three.  What fills them is not cut; the
-        // pairs left over are, so that they fill them once more together.
+        // pairs left over are, so that they fill them once more together (of
+        // them about as many hold a tile as if all runs were of one length).
         const std::uint64_t slots = head_dim == 128u ? 512u : 768u;
         const std::uint64_t whole = chunks >= 4u * kWaves ? pairs / slots * slots : pairs;
         std::uint64_t per = chunks;
         if (pairs > whole) {
-            const std::uint64_t splits = slots / (pairs - whole);
+            const std::uint64_t run_rows = (m + runs - 1u) / runs;
+            const std::uint64_t held = static_cast<std::uint64_t>(runs) * ((run_rows + tile_rows - 1u) / tile_rows) * kv_heads * parts;
+            const std::uint64_t left = (pairs - whole) * (held < pairs ? held : pairs) / pairs;
+            const std::uint64_t splits = slots / (left > 0u ? left : 1u);
             per = (chunks + splits - 1u) / splits;
             per = (per + kWaves - 1u) / kWaves * kWaves;
             if (per < 2u * kWaves) per = 2u * kWaves;
@@ -845,11 +1006,31 @@ Kv8Shape kv8_attention_shape(std::uint32_t m, std::uint32_t q_heads, std::uint32
     return shape(per > chunks ? chunks : per, kKv8Rows);
 }
 
+namespace {
+
+// The parts of the scratch memory: rows' statistics, and for runs of several
+// rows their vectors' operands, where weights are gathered; splits' partials.
+struct Scratch {
+    std::uint64_t queries, undos, partials, bytes;
+};
+
+Scratch scratch_of(const Kv8Shape& shape, std::uint32_t m, std::uint32_t q_heads, std::uint32_t head_dim, bool weights) {
+    const std::uint64_t vectors = static_cast<std::uint64_t>(m) * q_heads;
+    const auto padded = [](std::uint64_t bytes) { return (bytes + 255u) / 256u * 256u; };
+    Scratch s{};
+    s.queries = weights ? padded(vectors * sizeof(float2)) : 0u;
+    const bool keep = weights && shape.kernel == kKv8Runs;
+    s.undos = s.queries + (keep ? vectors * head_dim * 2u * sizeof(_Float16) : 0u);
+    s.partials = s.undos + (keep ? padded(vectors * sizeof(float)) : 0u);
+    s.bytes = s.partials + (shape.cut.splits > 1u ? vectors * shape.cut.splits * (head_dim + kStat) * sizeof(float) : 0u);
+    return s;
+}
+
+} // namespace
+
 std::uint64_t kv8_attention_scratch(const Kv8Shape& shape, std::uint32_t m, std::uint32_t q_heads,
                                     std::uint32_t head_dim, bool weights) {
-    const std::uint64_t vectors = static_cast<std::uint64_t>(m) * q_heads;
-    const std::uint64_t stats = weights ? (vectors * sizeof(float2) + 255u) / 256u * 256u : 0u;
-    return stats + (shape.cut.splits > 1u ? vectors * shape.cut.splits * (head_dim + kStat) * sizeof(float) : 0u);
+    return scratch_of(shape, m, q_heads, head_dim, weights).bytes;
 }
 
 namespace {
@@ -858,7 +1039,8 @@ template <int TYPE, unsigned D>
 void launch_typed(const Kv8Geometry& g, const float* qkv, std::uint64_t stride, std::uint32_t m,
                   const std::int32_t* positions, const std::int32_t* tables, std::uint32_t layer, std::uint32_t q_heads,
                   const std::int32_t* run_starts, std::uint32_t runs, std::uint64_t max_tokens, int weights,
-                  const Kv8Shape& shape, float* partials, float2* stats, float* out, hipStream_t stream) {
+                  const Kv8Shape& shape, float* partials, float2* stats, half8v* queries, float* undos, float* out,
+                  hipStream_t stream) {
     // Scores in powers of two: s log2(e) = (q . k) * log2(e) / sqrt(D).
     const float scale = static_cast<float>(1.4426950408889634 / __builtin_sqrt(static_cast<double>(D)));
     const Kv8Cut& cut = shape.cut;
@@ -869,12 +1051,12 @@ void launch_typed(const Kv8Geometry& g, const float* qkv, std::uint64_t stride, 
 #define AIR_KV8_ATTENTION(NV, RUNS, W)                                                                               \
     hipLaunchKernelGGL((kv8_attention_kernel<TYPE, D, NV, RUNS, W>), grid, dim3(64 * W), 0, stream, g, qkv, stride, m, \
                        positions, tables, layer, q_heads, run_starts, runs, shape.tile_rows, max_tokens, cut, scale, \
-                       partials, stats, out)
+                       partials, stats, queries, undos, out)
 #define AIR_KV8_MERGE(NV, RUNS)                                                                                      \
     hipLaunchKernelGGL((kv8_merge_kernel<D, NV, RUNS>), merge_grid, dim3(kThreads), 0, stream, positions, m, q_heads, \
                        g.kv_heads, run_starts, runs, shape.tile_rows, max_tokens, cut, partials, stats, out)
-#define AIR_KV8_WEIGHTS(SHARED, MERGE, COLUMNS)                                                                      \
-    hipLaunchKernelGGL((kv8_weights_kernel<TYPE, D, SHARED, MERGE>), dim3(COLUMNS, g.kv_heads, run_starts ? runs : m), \
+#define AIR_KV8_WEIGHTS(MERGE, COLUMNS)                                                                              \
+    hipLaunchKernelGGL((kv8_weights_kernel<TYPE, D, MERGE>), dim3(COLUMNS, g.kv_heads, run_starts ? runs : m), \
                        dim3(kThreads), 0, stream, g, qkv, stride, m, positions, tables, layer, q_heads, run_starts,  \
                        max_tokens, scale, stats, weights == 1, cut.split_chunks, cut.splits, partials, out)
     const std::uint32_t chunks = static_cast<std::uint32_t>((max_tokens + kChunkTokens - 1u) / kChunkTokens);
@@ -882,12 +1064,16 @@ void launch_typed(const Kv8Geometry& g, const float* qkv, std::uint64_t stride, 
     if (by_run) {
         AIR_KV8_ATTENTION(kRunTiles, true, kWaves);
         if (split) AIR_KV8_MERGE(kRunTiles, true);
-        if (weights) AIR_KV8_WEIGHTS(true, false, chunks);
+        if (weights) {
+            hipLaunchKernelGGL((kv8_run_weights_kernel<TYPE, D>), dim3(chunks, g.kv_heads, runs), dim3(kThreads), 0, stream, g,
+                               m, positions, tables, layer, q_heads, run_starts, max_tokens, scale, stats, queries, undos,
+                               weights == 1);
+        }
     } else {
         if (shape.kernel == kKv8ShortRows) AIR_KV8_ATTENTION(1u, false, kShortWaves);
         else AIR_KV8_ATTENTION(1u, false, kWaves);
-        if (weights && split) AIR_KV8_WEIGHTS(false, true, columns + 1u);
-        else if (weights) AIR_KV8_WEIGHTS(false, false, columns);
+        if (weights && split) AIR_KV8_WEIGHTS(true, columns + 1u);
+        else if (weights) AIR_KV8_WEIGHTS(false, columns);
         else if (split) AIR_KV8_MERGE(1u, false);
     }
 #undef AIR_KV8_ATTENTION
@@ -902,14 +1088,17 @@ hipError_t launch_kv8_attention(const Kv8Geometry& g, const float* qkv, std::uin
                                 std::uint32_t q_heads, const std::int32_t* run_starts, std::uint32_t runs,
                                 std::uint64_t max_tokens, int weights, const Kv8Shape& shape, void* scratch, float* out,
                                 hipStream_t stream) {
-    const std::uint64_t vectors = static_cast<std::uint64_t>(m) * q_heads;
-    float2* const stats = weights ? static_cast<float2*>(scratch) : nullptr;
-    float* const partials = reinterpret_cast<float*>(
-        static_cast<unsigned char*>(scratch) + (weights ? (vectors * sizeof(float2) + 255u) / 256u * 256u : 0u));
+    const Scratch at = scratch_of(shape, m, q_heads, g.head_dim, weights != 0);
+    unsigned char* const base = static_cast<unsigned char*>(scratch);
+    float2* const stats = weights ? reinterpret_cast<float2*>(base) : nullptr;
+    const bool keep = weights && shape.kernel == kKv8Runs;
+    half8v* const queries = keep ? reinterpret_cast<half8v*>(base + at.queries) : nullptr;
+    float* const undos = keep ? reinterpret_cast<float*>(base + at.undos) : nullptr;
+    float* const partials = reinterpret_cast<float*>(base + at.partials);
     const auto launch = g.type == kKv8I8 ? (g.head_dim == 128u ? launch_typed<kKv8I8, 128> : launch_typed<kKv8I8, 64>)
                                          : (g.head_dim == 128u ? launch_typed<kKv8E4M3, 128> : launch_typed<kKv8E4M3, 64>);
     launch(g, qkv, stride, m, positions, tables, layer, q_heads, run_starts, runs, max_tokens, weights, shape, partials,
-           stats, out, stream);
+           stats, queries, undos, out, stream);
     return hipGetLastError();
 }
 
