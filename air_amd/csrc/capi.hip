@@ -2278,6 +2278,11 @@ int check_kv8_tokens(const air_hip_kv8_layout* kv, uint64_t max_tokens) {
     if (max_tokens == 0 || max_tokens > static_cast<uint64_t>(kv->max_pages) * kv->page_tokens) {
         return fail(AIR_HIP_INVALID_ARGUMENT, "max_tokens must be in [1, max_pages * page_tokens]");
     }
+    // Grids hold a thread per 16-byte piece of a head's tokens, and less than
+    // 2^32 threads.
+    if (max_tokens > (1u << 27) || max_tokens * kv->kv_heads > (1ull << 31)) {
+        return fail(AIR_HIP_UNSUPPORTED, "at most 2^27 tokens and 2^31 (token, KV head) pairs per sequence and call");
+    }
     return AIR_HIP_OK;
 }
 int check_kv8_layers(const air_hip_kv8_layout* kv, uint32_t layer, uint32_t layers) {
@@ -2364,6 +2369,10 @@ int air_hip_kv8_attention(air_hip_context* ctx, const air_hip_kv8_layout* kv, co
     if (m == 0) return AIR_HIP_OK;
     if (static_cast<uint64_t>(m) + runs > 65535u || q_heads > 65535u) {
         return fail(AIR_HIP_UNSUPPORTED, "at most 65535 rows and runs together, and q heads, per call");
+    }
+    const uint64_t group = q_heads / kv->kv_heads;
+    if ((static_cast<uint64_t>(m) + runs) * kv->kv_heads * ((group + 15u) / 16u) > (1u << 22)) {
+        return fail(AIR_HIP_UNSUPPORTED, "at most 2^22 (row or run, 16 q heads of a KV head) pairs per call");
     }
     DeviceScope scope(ctx->device);
     if (scope.status() != hipSuccess) return hip_fail(scope.status(), "hipSetDevice");

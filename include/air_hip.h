@@ -611,10 +611,15 @@ int air_hip_attention_online(air_hip_context* ctx, const air_hip_kv_layout* kv, 
  * the token position.
  *
  * Values: scale = A * (1 / qmax) in f32 for values of largest magnitude A
- * (qmax 127 or 448, 1 / qmax rounded to f32), code = the nearest to the f32 quotient x / scale (ties to even),
- * value = code * scale.  A non-finite value makes its block's scale NaN: the
- * block reads as NaN, and so does what attends to it, until it is begun anew
- * at its first slot. */
+ * (qmax 127 or 448, 1 / qmax rounded to f32), code = the nearest to the f32
+ * quotient x / scale (ties to even), value = code * scale.  A non-finite value
+ * makes its block's scale NaN: the block reads as NaN, and so does what attends
+ * to it, until it is begun anew at its first slot.
+ *
+ * Larger calls than these are refused (AIR_HIP_UNSUPPORTED): max_tokens up to
+ * 2^27 and times kv_heads up to 2^31; attention over 65535 rows and runs
+ * together and 2^22 of them times KV heads (times each 16 q heads of one);
+ * read and eviction over 65535 (sequence, layer) and (layer, KV head) pairs. */
 enum {
     AIR_HIP_KV8_I8 = 1,      /* codes -127..127 */
     AIR_HIP_KV8_E4M3 = 2     /* OCP e4m3: 4 exponent, 3 mantissa bits, +-448 */

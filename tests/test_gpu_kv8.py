@@ -666,6 +666,250 @@ def test_captured_steps_replay(torch_cuda):
 
 
 @pytest.mark.gpu
+@KINDS
+def test_many_runs(torch_cuda, hip_ctx, kind):
+    """Seventy runs of one to nine rows (and empty ones), more than a wave
+    looks up at a time; forty q heads of one KV head, so two parts of a tile."""
+    rng = np.random.default_rng(61 + kind)
+    q_heads, kvh, d, page_tokens = 40, 1, 64, 16
+    rows_of = [int(n) for n in rng.integers(1, 10, 70)]
+    before = [int(n) for n in rng.integers(0, 30, 70)]
+    lengths = [a + b for a, b in zip(before, rows_of)]
+    cache, tables = _filled(kind, kvh, d, page_tokens, lengths, rng, layers=1, layer=0)
+    dev = Device(torch_cuda, hip_ctx, cache)
+    pos, tab, runs = [], [], []
+    for i, (a, b) in enumerate(zip(before, rows_of)):
+        runs.append((len(pos), len(pos) + b))
+        if i % 9 == 0:
+            runs.append((len(pos) + b, len(pos) + b))
+        pos += range(a, a + b)
+        tab += [tables[i]] * b
+    pos[runs[5][0]:runs[5][1]] = [-1] * (runs[5][1] - runs[5][0])     # a run that attends to nothing
+    tab = np.array(tab)
+    for mode, name in ((capi.KV8_WEIGHTS_NONE, None), (capi.KV8_WEIGHTS_SET, "set"), (capi.KV8_WEIGHTS_ADD, "add")):
+        x = rows(rng, len(pos), q_heads, kvh, d)
+        got = dev.attention(x, pos, tab, 0, q_heads, max(lengths), runs, weights=mode)
+        want, tol, far = cache.attention(x, pos, tab, 0, q_heads, max(lengths), runs, weights=name)
+        within(got, want, tol)
+        pool = dev.pool()
+        check_weights(cache, pool, far)
+        cache.pool[...] = pool
+
+
+@pytest.mark.gpu
+@KINDS
+@pytest.mark.parametrize("kvh,d", [(8, 128), (8, 64)])
+def test_tiles_past_a_full_card(torch_cuda, hip_ctx, kind, kvh, d):
+    """More tiles than run at a time: those that fill the card are not cut,
+    the ones left over are."""
+    rng = np.random.default_rng(71 + kind)
+    group, n = 16, 1090
+    q_heads, m = kvh * group, 131 if d == 128 else 201
+    cache, tables = _filled(kind, kvh, d, 16, [n, n + 7], rng, layers=1, layer=0)
+    dev = Device(torch_cuda, hip_ctx, cache)
+    cutoff = m // 2 + 3
+    runs = [(0, cutoff), (cutoff, m)]
+    tab = np.array([tables[0]] * cutoff + [tables[1]] * (m - cutoff))
+    pos = [n - 1 - 300 * (r % 3) for r in range(m)]
+    x = rows(rng, 6, q_heads, kvh, d)[np.arange(m) % 6]           # six rows over and over
+    got = dev.attention(x, pos, tab, 0, q_heads, n + 7, runs)
+    some = [r for start in (0, cutoff) for r in range(start, start + 6)]
+    want, tol, _ = cache.attention(x[some], [pos[r] for r in some], tab[some], 0, q_heads, n + 7)
+    like = [some.index(next(s for s in some if s % 6 == r % 6 and (s < cutoff) == (r < cutoff))) for r in range(m)]
+    within(got, want[like], tol[like])
+
+
+@pytest.mark.gpu
+@KINDS
+def test_runs_of_one_row_over_split_keys(torch_cuda, hip_ctx, kind):
+    """Runs of a row each, one empty, one shorter than a split, over keys long
+    enough to be cut, with weights: the launch that joins the splits takes the
+    runs' rows."""
+    rng = np.random.default_rng(81 + kind)
+    q_heads, kvh, d = 12, 2, 64
+    lengths = [2500, 30, 1200]
+    cache, tables = _filled(kind, kvh, d, 32, lengths, rng, layers=1, layer=0)
+    dev = Device(torch_cuda, hip_ctx, cache)
+    pos, runs = [n - 1 for n in lengths], [(0, 1), (1, 1), (1, 2), (2, 3)]
+    for mode, name in ((capi.KV8_WEIGHTS_ADD, "add"), (capi.KV8_WEIGHTS_SET, "set")):
+        x = rows(rng, 3, q_heads, kvh, d, pad=8)
+        got = dev.attention(x, pos, tables, 0, q_heads, 2500, runs, weights=mode)
+        want, tol, far = cache.attention(x, pos, tables, 0, q_heads, 2500, runs, weights=name)
+        within(got, want, tol)
+        pool = dev.pool()
+        check_weights(cache, pool, far)
+        cache.pool[...] = pool
+
+
+@pytest.mark.gpu
+def test_runs_that_share_pages_add_up(torch_cuda, hip_ctx):
+    """Two runs over one sequence's pages: what both add to a weight is
+    there, whichever comes first (each addition rounds once)."""
+    rng = np.random.default_rng(91)
+    q_heads, kvh, d, n = 8, 2, 64, 200
+    cache, tables = _filled(I8, kvh, d, 16, [n], rng, layers=1, layer=0)
+    dev = Device(torch_cuda, hip_ctx, cache)
+    pos = list(range(n - 8, n)) + list(range(n - 6, n))
+    tab = np.repeat(tables, len(pos), axis=0)
+    x = rows(rng, len(pos), q_heads, kvh, d)
+    dev.attention(x, pos, tab, 0, q_heads, n, [(0, 8), (8, 14)], weights=capi.KV8_WEIGHTS_ADD)
+    _, _, first = cache.attention(x[:8], pos[:8], tab[:8], 0, q_heads, n, [(0, 8)], weights="add")
+    _, _, both = cache.attention(x[8:], pos[8:], tab[8:], 0, q_heads, n, [(0, 6)], weights="add")
+    check_weights(cache, dev.pool(), [b[:4] + (a[4] + b[4],) for a, b in zip(first, both)])
+
+
+@pytest.mark.gpu
+@KINDS
+@pytest.mark.parametrize("kvh,d,budget", [(2, 128, 333), (1, 64, 400)])
+def test_evict_many_blocks_in_place(torch_cuda, hip_ctx, kind, kvh, d, budget):
+    """More blocks than a workgroup takes at a time, kept tokens crowded at
+    the end (every block's sources lie far ahead) or at the front (a block is
+    its own source)."""
+    rng = np.random.default_rng(budget + kind)
+    lengths = [900, 500, budget + 1]
+    cache, tables = _filled(kind, kvh, d, 16, lengths, rng, layers=1, layer=0)
+    for i, n in enumerate(lengths):
+        for t in range(n):
+            at = cache.slot(tables[i], 0, 0, t)
+            for g in range(kvh):
+                rec = cache.slot(tables[i], 0, g, t)[0]
+                cache.floats(rec)[16 + at[1]] = np.float32(t if i == 0 else -t if i == 1 else rng.random())
+    dev = Device(torch_cuda, hip_ctx, cache)
+    got = dev.evict(lengths, tables, tables, 0, 1, 1, 2, budget, 900)
+    want = cache.evict(lengths, tables, tables, 0, 1, 1, 2, budget, 900)
+    assert np.array_equal(got, want)
+    fill = 7.0
+    for a, b in zip(dev.read(None, [budget] * 3, tables, 0, 1, budget, fill),
+                    cache.read(None, [budget] * 3, tables, 0, 1, budget, fill)):
+        assert np.array_equal(a, b)
+
+
+@pytest.mark.gpu
+def test_two_contexts_at_once(torch_cuda):
+    """Two contexts on two streams, their calls in turn without waiting:
+    each result is that of its calls alone."""
+    torch = torch_cuda
+    rng = np.random.default_rng(101)
+    q_heads, kvh, d = 14, 2, 64
+    lengths = [700, 90]
+    cache, tables = _filled(E4M3, kvh, d, 16, lengths, rng, layers=1, layer=0, max_pages=60)
+    xs = [rows(rng, 2, q_heads, kvh, d) for _ in range(8)]
+
+    def calls(dev, ctx, x, pos, tab, out):
+        capi.check(dev.lib.air_hip_kv8_append(ctx.handle, ctypes.byref(dev.kv), x.data_ptr(), x.shape[1], q_heads * d,
+                                              2, pos.data_ptr(), tab.data_ptr(), 0))
+        capi.check(dev.lib.air_hip_kv8_attention(ctx.handle, ctypes.byref(dev.kv), x.data_ptr(), x.shape[1], 2,
+                                                 pos.data_ptr(), tab.data_ptr(), 0, q_heads, None, 0, 960,
+                                                 capi.KV8_WEIGHTS_ADD, out.data_ptr()))
+        pos.add_(1)
+
+    def run(together):
+        streams = [torch.cuda.Stream() for _ in range(2)]
+        ctxs = [capi.Context(0, s.cuda_stream) for s in streams]
+        devs = [Device(torch, c, cache) for c in ctxs]
+        sides = []
+        for i, dev in enumerate(devs):
+            sides.append((dev.up(np.array(lengths) + 3 * i, np.int32), dev.up(tables, np.int32),
+                          [dev.up(x) for x in xs[4 * i:4 * i + 4]],
+                          [torch.zeros((2, q_heads * d), device="cuda:0") for _ in range(4)]))
+        torch.cuda.synchronize()
+        order = [(i, j) for j in range(4) for i in range(2)] if together else [(i, j) for i in range(2) for j in range(4)]
+        for i, j in order:
+            pos, tab, x, out = sides[i]
+            with torch.cuda.stream(streams[i]):
+                calls(devs[i], ctxs[i], x[j], pos, tab, out[j])
+            if not together:
+                torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        result = [torch.stack(s[3]).cpu().numpy() for s in sides] + [dev.pool() for dev in devs]
+        for c in ctxs:
+            c.close()
+        return result
+
+    together, alone = run(True), run(False)
+    assert np.isfinite(together[0]).all()
+    for a, b in zip(together, alone):                 # side 1 counts three stale slots as held: NaN codes among them
+        assert np.array_equal(a, b, equal_nan=a.dtype == np.float32)
+
+
+@pytest.mark.gpu
+def test_captured_prompt_replays(torch_cuda):
+    """A prompt's runs appended and attended to with weights, then an eviction
+    to other pages, in one graph: replays over changed rows equal the eager
+    calls, with a larger eager call (which regrows the scratch) between."""
+    torch = torch_cuda
+    rng = np.random.default_rng(111)
+    q_heads, kvh, d, m = 14, 2, 64, 60
+    cache = Cache(I8, kvh, d, 1, 16, 80, 20, seed=6)
+    both = page_tables(rng, [300, 300, 48, 48], 16, 20, 80)
+    stream = torch.cuda.Stream()
+    with capi.Context(0, stream.cuda_stream) as ctx, torch.cuda.stream(stream):
+        dev, ref = Device(torch, ctx, cache), Device(torch, ctx, cache)
+        x = dev.up(rows(rng, m, q_heads, kvh, d))
+        pos = dev.up(list(range(40, 70)) + list(range(100, 130)), np.int32)
+        tab = dev.up(np.repeat(both[:2], 30, axis=0), np.int32)
+        old, new, starts = dev.up(both[:2], np.int32), dev.up(both[2:], np.int32), dev.up([0, 30, 60], np.int32)
+        lengths = dev.up([70, 130], np.int32)
+        outs = [torch.zeros((m, q_heads * d), device="cuda:0") for _ in range(2)]
+        kept = [torch.zeros(2 * kvh * 48, dtype=torch.int32, device="cuda:0") for _ in range(2)]
+
+        def step(side, i, bound=320):
+            lib, h, kv = side.lib, ctx.handle, ctypes.byref(side.kv)
+            capi.check(lib.air_hip_kv8_append(h, kv, x.data_ptr(), x.shape[1], q_heads * d, m, pos.data_ptr(),
+                                              tab.data_ptr(), 0))
+            capi.check(lib.air_hip_kv8_attention(h, kv, x.data_ptr(), x.shape[1], m, pos.data_ptr(), tab.data_ptr(), 0,
+                                                 q_heads, starts.data_ptr(), 2, bound, capi.KV8_WEIGHTS_ADD,
+                                                 outs[i].data_ptr()))
+            capi.check(lib.air_hip_kv8_evict(h, kv, 2, lengths.data_ptr(), old.data_ptr(), new.data_ptr(), 0, 1, 2, 8,
+                                             48, 320, kept[i].data_ptr()))
+        step(dev, 0)
+        step(ref, 1)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=stream):
+            step(dev, 0)
+        wide = torch.zeros((4 * m, x.shape[1]), device="cuda:0")
+        gone = torch.full((4 * m,), -1, dtype=torch.int32, device="cuda:0")
+        wide_tab, wide_out = tab.repeat(4, 1), torch.empty((4 * m, q_heads * d), device="cuda:0")
+        for i in range(4):
+            x.copy_(dev.up(rows(rng, m, q_heads, kvh, d)))
+            if i == 2:                                # rows that attend to nothing, more of them than before
+                capi.check(dev.lib.air_hip_kv8_attention(ctx.handle, ctypes.byref(dev.kv), wide.data_ptr(), wide.shape[1],
+                                                         4 * m, gone.data_ptr(), wide_tab.data_ptr(), 0, q_heads, None,
+                                                         0, 320, capi.KV8_WEIGHTS_ADD, wide_out.data_ptr()))
+            torch.cuda.synchronize()
+            g.replay()
+            step(ref, 1)
+            torch.cuda.synchronize()
+            assert torch.equal(outs[0], outs[1]) and torch.equal(kept[0], kept[1]), i
+            assert np.array_equal(dev.pool(), ref.pool()), i
+        assert not wide_out.any()
+    torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+def test_sizes_past_the_grids_are_refused(torch_cuda, hip_ctx):
+    torch = torch_cuda
+    lib, h = capi.lib(), hip_ctx.handle
+    buf = torch.zeros(1 << 12, device="cuda:0")
+    ints = torch.zeros(64, dtype=torch.int32, device="cuda:0")
+    p, i = buf.data_ptr(), ints.data_ptr()
+
+    def attend(kv_heads, heads, m, top):
+        kv = capi.Kv8Layout(p, 16, kv_heads, 64, 1, 1 << 24, 1, None, 0, I8)
+        return lib.air_hip_kv8_attention(h, ctypes.byref(kv), p, heads * 64, m, i, i, 0, heads, None, 0, top, 0, p)
+    assert attend(65, 65, 65535, 16) == 6 and b"2^22" in lib.air_hip_last_error()
+    assert attend(1, 1, 0, (1 << 27) + 1) == 6 and b"2^27" in lib.air_hip_last_error()
+    assert attend(32, 32, 0, 1 << 27) == 6
+    assert attend(16, 16, 0, 1 << 27) == 0
+    kv = capi.Kv8Layout(p, 16, 1, 64, 1, 1 << 24, 1, None, 0, I8)
+    assert lib.air_hip_kv8_read(h, ctypes.byref(kv), 0, None, i, i, 0, 1, (1 << 27) + 1, p, None, None) == 6
+    assert lib.air_hip_kv8_evict(h, ctypes.byref(kv), 0, i, i, i, 0, 1, 0, 0, 8, (1 << 27) + 1, i) == 6
+    torch.cuda.synchronize()
+    assert not buf.any() and not ints.any()
+
+
+@pytest.mark.gpu
 def test_refusals(torch_cuda, hip_ctx):
     """Every argument that the host can judge is refused with a message, and
     nothing runs."""
