@@ -9,8 +9,9 @@
 // products run on v_mfma_f32_16x16x32_f16 with two instructions where one
 // f16 operand would take one: q = hi + lo against K codes, p = hi + lo
 // against V codes, summed in f32.  The result differs from a float64
-// attention over the same codes by ~5e-7 relative, as an f32 computation
-// does; a single f16 p would leave 2e-4.
+// attention over the same codes by 3e-7 to 6e-7 relative (torch's f32 products
+// and softmax over the decoded values: 4e-7 to 2e-6); a single f16 p would
+// leave 2e-4.
 //
 // A wave walks chunks of 64 tokens (four blocks) of one KV head for 16 query
 // vectors, with nothing staged in LDS:
@@ -28,6 +29,14 @@
 // far (for the denominator) and M2 >= every s log2(e) + log2(scale of V) (for
 // the numerators, whose p carries V's scale: a block of large values does not
 // take the low bits of the others).  Rescaling by a power of two is exact.
+//
+// What bounds it.  Decode over a cache larger than the chip's: reading it (48
+// rows over 4000..16000 tokens, 32 q heads on 8 KV heads of 128 dims: 189 us,
+// 5.2 TB/s of the 985 MB, as a large copy).  Fewer tokens: the waits of one
+// walk (32 rows over 500..1200 tokens: 11.3 us, 2.3 TB/s).  Prompts: the issue
+// of vector operations, some 20 a score (602 rows over 3300..3801 tokens, 28 q
+// heads: 85 us, 345 TFLOP/s of the products' 29 GFLOP; the matrix cores, which
+// do twice that for the operands' two halves, are busy a third of the time).
 #include "air_hip_device.hpp"
 #include "air_hip_kernels.hpp"
 #include "air_hip_kv8.hpp"
@@ -300,9 +309,8 @@ __device__ __forceinline__ void soften(float4v (&s)[4], float unit, float2 scale
     l += __builtin_amdgcn_ldexpf(sum, base - ref);
 }
 
-// The rows of a tile: with RUNS up to kRows rows of one run (kRows whole
-// groups of q heads fit its 16 NV vectors, at least one row), otherwise one
-// row.  A group of more than 16 NV q heads is cut into parts (grid x).
+// The rows of a tile: with RUNS up to tile_rows rows of one run (as many whole
+// groups of q heads as fit its 16 NV vectors, at least one), otherwise one row.  A group of more than 16 NV q heads is cut into parts.
 struct Tile {
     std::uint32_t row, rows;       // first row, rows (0: no tile)
     std::uint32_t head, heads;     // q heads of each row
@@ -354,10 +362,16 @@ __device__ __forceinline__ Kv8Work kv8_work(const Kv8Cut& cut, std::uint32_t blo
     return Kv8Work{cut.pairs / tile_heads - 1u - pair / tile_heads, pair % tile_heads, split, chunks};
 }
 
-// A tile of up to 16 NV query vectors of one KV head per workgroup; its waves
-// take the chunks of split blockIdx.z in turn, every wave for all vectors.
-// With NV > 1 the vectors' operands lie in LDS, and a chunk's codes are turned
-// into f16 once for all of them.
+// A tile of up to 16 NV query vectors of one KV head per workgroup; its W waves
+// take the chunks of its split in turn, every wave for all vectors, and meet
+// at the end.  With NV > 1 the vectors' operands lie in LDS, and a chunk's
+// codes are turned into f16 once for all of them: with 16 vectors a wave the
+// conversions alone are up to 16 operations a score (602 rows over 3300..3801
+// tokens: 208 us with 16 vectors and references moved in every chunk, 108 with
+// 32 and moved when passed, 85 with what followed).  Measured slower there: 128 vectors a workgroup whose waves share codes
+// converted in LDS (98 us where this took 94), and 32x32x16 products (92 where
+// this took 87): the waves wait longer between the phases, which they do not
+// overlap, than fewer instructions save.
 template <int TYPE, unsigned D, unsigned NV, bool RUNS, unsigned W>
 __global__ __launch_bounds__(64 * W, NV == 1u && W == kWaves ? 3 : 2) void kv8_attention_kernel(
     Kv8Geometry g, const float* __restrict__ qkv, std::uint64_t stride, std::uint32_t m,
@@ -634,7 +648,8 @@ __device__ __forceinline__ float4v join_splits(const float* __restrict__ base, s
     return y;
 }
 
-// Joins the splits of a tile's vectors.
+// Joins the splits of a tile's vectors.  A launch of its own costs 4 us here;
+// what it reads (a few MB) costs less.
 template <unsigned D, unsigned NV, bool RUNS>
 __global__ __launch_bounds__(kThreads) void kv8_merge_kernel(
     const std::int32_t* __restrict__ positions, std::uint32_t m, std::uint32_t q_heads, std::uint32_t kv_heads,

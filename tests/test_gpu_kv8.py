@@ -785,6 +785,26 @@ def test_evict_many_blocks_in_place(torch_cuda, hip_ctx, kind, kvh, d, budget):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("in_place", [True, False])
+def test_evict_of_a_long_sequence(torch_cuda, hip_ctx, in_place):
+    """More tokens than the selection holds in LDS, with equal weights on both
+    sides of that bound."""
+    rng = np.random.default_rng(121)
+    n, budget = 17001, 700
+    cache = Cache(I8, 1, 64, 1, 64, 290, 280, seed=8)
+    Cache.floats(cache.pool)[..., 16:32] = rng.integers(0, 40, cache.pool.shape[:-1] + (16,))
+    both = page_tables(rng, [n, budget], 64, 280, 290)
+    tables = both[:1]
+    new = tables if in_place else both[1:]
+    dev = Device(torch_cuda, hip_ctx, cache)
+    got = dev.evict([n], tables, new, 0, 1, 3, 30, budget, 280 * 64)
+    want = cache.evict([n], tables, new, 0, 1, 3, 30, budget, 280 * 64)
+    assert np.array_equal(got, want)
+    for a, b in zip(dev.read(None, [budget], new, 0, 1, budget, 7.0), cache.read(None, [budget], new, 0, 1, budget, 7.0)):
+        assert np.array_equal(a, b)
+
+
+@pytest.mark.gpu
 def test_two_contexts_at_once(torch_cuda):
     """Two contexts on two streams, their calls in turn without waiting:
     each result is that of its calls alone."""
