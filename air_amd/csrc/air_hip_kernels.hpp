@@ -432,11 +432,12 @@ struct Kv8Shape {
     Kv8Cut cut;
     std::uint32_t tile_rows;      // rows of one run a tile holds
     int kernel;                   // kKv8Rows ..
+    bool run_weights;             // weights by the kernel for runs of many vectors
 };
 Kv8Shape kv8_attention_shape(std::uint32_t m, std::uint32_t q_heads, std::uint32_t kv_heads, std::uint32_t head_dim,
-                             std::uint32_t runs, std::uint64_t max_tokens);
+                             std::uint32_t runs, std::uint64_t max_tokens, bool weights);
 // Bytes of scratch: the splits' partials and, with weights, the rows' softmax
-// statistics.
+// statistics and for run_weights their vectors' operands.
 std::uint64_t kv8_attention_scratch(const Kv8Shape& shape, std::uint32_t m, std::uint32_t q_heads,
                                     std::uint32_t head_dim, bool weights);
 // weights: 0 none, 1 add, 2 set.  run_starts may be null (every row its own run).

@@ -316,30 +316,66 @@ struct Tile {
     std::uint32_t head, heads;     // q heads of each row
 };
 
-__device__ __forceinline__ Tile find_tile(std::uint32_t index, const std::int32_t* __restrict__ run_starts,
+// x of this lane and those below it, summed: within rows of 16 lanes, then the
+// last lane of a row to the next, and of the lower half to the upper.
+__device__ __forceinline__ std::uint32_t wave_sums(std::uint32_t x) {
+    x += __builtin_amdgcn_update_dpp(0u, x, 0x111, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0u, x, 0x112, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0u, x, 0x114, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0u, x, 0x118, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0u, x, 0x142, 0xa, 0xf, false);
+    return x + __builtin_amdgcn_update_dpp(0u, x, 0x143, 0xc, 0xf, false);
+}
+
+// The tile that is `index`-th to start, of at most `tiles` tiles of the runs;
+// they count down, as the last rows of a run reach furthest.
+__device__ __forceinline__ Tile find_tile(std::uint32_t index, std::uint32_t tiles, const std::int32_t* __restrict__ run_starts,
                                           std::uint32_t runs, std::uint32_t m, std::uint32_t tile_rows) {
-    // Run i owns tiles run_starts[i] / tile_rows + i and on: at least as many
-    // as its rows need, and the count over all runs needs no prefix sum.  The
-    // wave looks 64 runs up at a time.
     const unsigned lane = threadIdx.x & 63u;
-    std::uint32_t lo = 0u, hi = runs;              // the run is in [lo, hi)
-    const auto first_tile = [&](std::uint32_t i) __attribute__((always_inline)) {
-        const std::int32_t s = run_starts[i];
-        return (s > 0 ? static_cast<std::uint32_t>(s) / tile_rows : 0u) + i;
-    };
-    while (hi - lo > 1u) {
-        const std::uint32_t step = (hi - lo + 63u) / 64u;
-        const std::uint32_t i = lo + lane * step;
-        const bool below = i < hi && first_tile(i) <= index;
-        const std::uint64_t mask = __ballot(below);
-        if (mask == 0u) return Tile{0u, 0u, 0u, 0u};
-        const std::uint32_t last = 63u - static_cast<std::uint32_t>(__builtin_clzll(mask));
-        lo += last * step;
-        hi = lo + step < hi ? lo + step : hi;
+    std::uint32_t run, first;                      // the tile's run, and that run's first tile
+    std::int64_t begin, end;
+    if (runs <= 64u) {
+        // The runs' tiles one after the other, so that the empty ones come last:
+        // spread between the others they leave some CUs two tiles and others
+        // none (24 runs of 4 rows of 28 q heads over 3000 tokens: 43 us, 30 so).
+        const std::int32_t b = lane < runs ? run_starts[lane] : 0, e = lane < runs ? run_starts[lane + 1u] : 0;
+        const bool held = b >= 0 && e > b && static_cast<std::uint32_t>(e) <= m;
+        const std::uint32_t mine = held ? (static_cast<std::uint32_t>(e - b) + tile_rows - 1u) / tile_rows : 0u;
+        const std::uint32_t upto = wave_sums(mine);
+        const std::uint32_t all = __builtin_amdgcn_readlane(upto, 63);
+        if (index >= all) return Tile{0u, 0u, 0u, 0u};
+        index = all - 1u - index;
+        run = static_cast<std::uint32_t>(__builtin_ctzll(__ballot(upto > index)));
+        first = __builtin_amdgcn_readlane(upto - mine, run);
+        begin = static_cast<std::int32_t>(__builtin_amdgcn_readlane(b, run));
+        end = static_cast<std::int32_t>(__builtin_amdgcn_readlane(e, run));
+    } else {
+        // Run i owns tiles run_starts[i] / tile_rows + i and on: at least as
+        // many as its rows need, and the count over all runs needs no prefix
+        // sum.  The wave looks 64 runs up at a time.
+        index = tiles - 1u - index;
+        std::uint32_t lo = 0u, hi = runs;          // the run is in [lo, hi)
+        const auto first_tile = [&](std::uint32_t i) __attribute__((always_inline)) {
+            const std::int32_t s = run_starts[i];
+            return (s > 0 ? static_cast<std::uint32_t>(s) / tile_rows : 0u) + i;
+        };
+        while (hi - lo > 1u) {
+            const std::uint32_t step = (hi - lo + 63u) / 64u;
+            const std::uint32_t i = lo + lane * step;
+            const bool below = i < hi && first_tile(i) <= index;
+            const std::uint64_t mask = __ballot(below);
+            if (mask == 0u) return Tile{0u, 0u, 0u, 0u};
+            const std::uint32_t last = 63u - static_cast<std::uint32_t>(__builtin_clzll(mask));
+            lo += last * step;
+            hi = lo + step < hi ? lo + step : hi;
+        }
+        run = lo;
+        first = first_tile(lo);
+        begin = run_starts[lo];
+        end = run_starts[lo + 1u];
+        if (begin < 0 || end > static_cast<std::int64_t>(m) || first > index) return Tile{0u, 0u, 0u, 0u};
     }
-    const std::int64_t begin = run_starts[lo], end = run_starts[lo + 1u];
-    if (begin < 0 || end > static_cast<std::int64_t>(m) || first_tile(lo) > index) return Tile{0u, 0u, 0u, 0u};
-    const std::int64_t row = begin + static_cast<std::int64_t>(index - first_tile(lo)) * tile_rows;
+    const std::int64_t row = begin + static_cast<std::int64_t>(index - first) * tile_rows;
     if (row >= end) return Tile{0u, 0u, 0u, 0u};
     const std::int64_t left = end - row;
     return Tile{static_cast<std::uint32_t>(row), static_cast<std::uint32_t>(left < tile_rows ? left : tile_rows), 0u, 0u};
@@ -347,9 +383,8 @@ __device__ __forceinline__ Tile find_tile(std::uint32_t index, const std::int32_
 
 // The (tile, heads) pairs of a launch, one workgroup for each of the first
 // `whole` ones and `splits` of split_chunks chunks for each of the others.
-// The tiles count down: the last rows of a run reach furthest and start first.
 struct Kv8Work {
-    std::uint32_t tile, tile_head, split, split_chunks;
+    std::uint32_t pair, tile, tile_head, split, split_chunks;
 };
 __device__ __forceinline__ Kv8Work kv8_work(const Kv8Cut& cut, std::uint32_t block, std::uint32_t tile_heads) {
     std::uint32_t pair = block, split = 0u, chunks = 0x7fffffffu / kChunkTokens;   // more than any tile has
@@ -359,7 +394,7 @@ __device__ __forceinline__ Kv8Work kv8_work(const Kv8Cut& cut, std::uint32_t blo
         split = (block - cut.whole) / pairs;
         chunks = cut.split_chunks;
     }
-    return Kv8Work{cut.pairs / tile_heads - 1u - pair / tile_heads, pair % tile_heads, split, chunks};
+    return Kv8Work{pair, pair / tile_heads, pair % tile_heads, split, chunks};
 }
 
 // A tile of up to 16 NV query vectors of one KV head per workgroup; its W waves
@@ -368,10 +403,11 @@ __device__ __forceinline__ Kv8Work kv8_work(const Kv8Cut& cut, std::uint32_t blo
 // codes are turned into f16 once for all of them: with 16 vectors a wave the
 // conversions alone are up to 16 operations a score (602 rows over 3300..3801
 // tokens: 208 us with 16 vectors and references moved in every chunk, 108 with
-// 32 and moved when passed, 85 with what followed).  Measured slower there: 128 vectors a workgroup whose waves share codes
-// converted in LDS (98 us where this took 94), and 32x32x16 products (92 where
-// this took 87): the waves wait longer between the phases, which they do not
-// overlap, than fewer instructions save.
+// 32 and moved when passed, 85 with what followed).  Measured slower there: 128
+// vectors a workgroup whose waves share codes converted in LDS (98 us where
+// this took 94), and 32x32x16 products (92 where this took 87): the waves wait
+// longer between the phases, which they do not overlap, than fewer instructions
+// save.
 template <int TYPE, unsigned D, unsigned NV, bool RUNS, unsigned W>
 __global__ __launch_bounds__(64 * W, NV == 1u && W == kWaves ? 3 : 2) void kv8_attention_kernel(
     Kv8Geometry g, const float* __restrict__ qkv, std::uint64_t stride, std::uint32_t m,
@@ -396,7 +432,7 @@ __global__ __launch_bounds__(64 * W, NV == 1u && W == kWaves ? 3 : 2) void kv8_a
     const std::uint32_t split = work.split, split_chunks = work.split_chunks;
     const std::uint32_t kvh = work.tile_head / parts, part = work.tile_head % parts;
     Tile tile{work.tile, 1u, 0u, 0u};
-    if constexpr (RUNS) tile = find_tile(work.tile, run_starts, runs, m, tile_rows);
+    if constexpr (RUNS) tile = find_tile(work.tile, cut.pairs / (g.kv_heads * parts), run_starts, runs, m, tile_rows);
     if (tile.rows == 0u) return;
     tile.head = kvh * group + part * kTile;
     tile.heads = group - part * kTile < kTile ? group - part * kTile : kTile;
@@ -594,7 +630,8 @@ __global__ __launch_bounds__(64 * W, NV == 1u && W == kWaves ? 3 : 2) void kv8_a
             *reinterpret_cast<float4v*>(out + vector * D + 4u * d4) = y;
             if (stats && d4 == 0u) stats[vector] = make_float2(static_cast<float>(mm), total == 0.0f ? 0.0f : 1.0f / total);
         } else {
-            float* const p = partials + (vector * cut.splits + split) * (D + kStat);
+            const std::uint64_t place = RUNS ? static_cast<std::uint64_t>(work.pair - cut.whole) * kTile + v : vector;
+            float* const p = partials + (place * cut.splits + split) * (D + kStat);
             if (d4 == 0u) *reinterpret_cast<float4v*>(p) = float4v{__int_as_float(mm), __int_as_float(mm2), total, 0.0f};
             *reinterpret_cast<float4v*>(p + kStat + 4u * d4) = acc;
         }
@@ -660,7 +697,7 @@ __global__ __launch_bounds__(kThreads) void kv8_merge_kernel(
     const Kv8Work work = kv8_work(cut, cut.whole + blockIdx.x, kv_heads * parts);
     const std::uint32_t kvh = work.tile_head / parts, part = work.tile_head % parts;
     Tile tile{work.tile, 1u, 0u, 0u};
-    if constexpr (RUNS) tile = find_tile(work.tile, run_starts, runs, m, tile_rows);
+    if constexpr (RUNS) tile = find_tile(work.tile, cut.pairs / (kv_heads * parts), run_starts, runs, m, tile_rows);
     if (tile.rows == 0u) return;
     tile.head = kvh * group + part * kTile;
     tile.heads = group - part * kTile < kTile ? group - part * kTile : kTile;
@@ -678,7 +715,8 @@ __global__ __launch_bounds__(kThreads) void kv8_merge_kernel(
             static_cast<std::uint64_t>(tile.row + v / tile.heads) * q_heads + tile.head + v % tile.heads;
         int ref;
         float total;
-        const float4v y = join_splits<D>(partials + vector * splits * (D + kStat), live, d4, ref, total);
+        const std::uint64_t place = RUNS ? static_cast<std::uint64_t>(blockIdx.x) * kTile + v : vector;
+        const float4v y = join_splits<D>(partials + place * splits * (D + kStat), live, d4, ref, total);
         *reinterpret_cast<float4v*>(out + vector * D + 4u * d4) = y;
         if (stats && d4 == 0u) stats[vector] = make_float2(static_cast<float>(ref), total == 0.0f ? 0.0f : 1.0f / total);
     }
@@ -971,13 +1009,32 @@ __global__ __launch_bounds__(kThreads, 2) void kv8_run_weights_kernel(
 } // namespace
 
 Kv8Shape kv8_attention_shape(std::uint32_t m, std::uint32_t q_heads, std::uint32_t kv_heads, std::uint32_t head_dim,
-                             std::uint32_t runs, std::uint64_t max_tokens) {
+                             std::uint32_t runs, std::uint64_t max_tokens, bool weights) {
     const std::uint32_t group = q_heads / kv_heads;
     const std::uint32_t chunks = static_cast<std::uint32_t>((max_tokens + kChunkTokens - 1u) / kChunkTokens);
-    // Two rows a run on average share their keys; below that a tile is a row.
-    if (runs != 0u && m >= 2u * runs) {
-        const std::uint32_t tile = kVectors * kRunTiles, parts = (group + tile - 1u) / tile;
-        const std::uint32_t tile_rows = group < tile ? tile / group : 1u;
+    const std::uint32_t row_parts = (group + kVectors - 1u) / kVectors;
+    const std::uint64_t row_pairs = static_cast<std::uint64_t>(m) * kv_heads * row_parts;
+    // Tiles of runs, as if all runs were of one length: a chunk of one costs
+    // as much as that of 1.6 single rows, and about 5 us more a call.  Over
+    // 660 calls (1..24 runs of 2..512 rows over up to 3000 tokens, 8 x 1, 8 x
+    // 2, 8 x 4, 4 x 7, 2 x 14 and 8 x 16 heads of 64 and 128 dims) this takes
+    // 0.7 % longer in the mean than the better of both, 30 % at most; runs'
+    // tiles always took 18 % longer, up to 1.8 times.
+    const std::uint32_t run_rows = runs != 0u ? (m + runs - 1u) / runs : 0u;
+    const std::uint32_t tile = kVectors * kRunTiles, parts = (group + tile - 1u) / tile;
+    const std::uint32_t tile_rows = group < tile ? tile / group : 1u;
+    const std::uint64_t run_pairs = static_cast<std::uint64_t>(runs) * ((run_rows + tile_rows - 1u) / tile_rows) * kv_heads * parts;
+    const bool by_work = 5u * row_pairs * (chunks + 2u) > 8u * run_pairs * (chunks + 2u) + 20000u;
+    // A run's weights: a wave a chunk takes its vectors one 16 after the other,
+    // which suits chunks for all SIMDs (24 runs of 24 rows over 3000 tokens, 8
+    // heads: 76 us against 105), and a workgroup a chunk does many vectors with
+    // few chunks (4 runs of 100 rows from the start: 26 against 19).  The second
+    // needs the vectors that runs' tiles leave, and is worth them from 80 on
+    // (a prompt of 512 rows, 4 x 7 heads: 397 us without, 65).
+    const std::uint64_t run_vectors = static_cast<std::uint64_t>(run_rows) * group;
+    const bool run_weights =
+        weights && 400u * ((run_vectors + kVectors - 1u) / kVectors) > static_cast<std::uint64_t>(runs) * kv_heads * chunks;
+    if (runs != 0u && (by_work || (weights && run_vectors >= 80u))) {
         const std::uint64_t pairs = (static_cast<std::uint64_t>(m / tile_rows) + runs) * kv_heads * parts;
         // Workgroups that run at a time: two a CU, with the registers of two
         // MFMA tiles of 128 dims, or three.  What fills them is not cut; the
@@ -987,9 +1044,7 @@ Kv8Shape kv8_attention_shape(std::uint32_t m, std::uint32_t q_heads, std::uint32
         const std::uint64_t whole = chunks >= 4u * kWaves ? pairs / slots * slots : pairs;
         std::uint64_t per = chunks;
         if (pairs > whole) {
-            const std::uint64_t run_rows = (m + runs - 1u) / runs;
-            const std::uint64_t held = static_cast<std::uint64_t>(runs) * ((run_rows + tile_rows - 1u) / tile_rows) * kv_heads * parts;
-            const std::uint64_t left = (pairs - whole) * (held < pairs ? held : pairs) / pairs;
+            const std::uint64_t left = (pairs - whole) * (run_pairs < pairs ? run_pairs : pairs) / pairs;
             const std::uint64_t splits = slots / (left > 0u ? left : 1u);
             per = (chunks + splits - 1u) / splits;
             per = (per + kWaves - 1u) / kWaves * kWaves;
@@ -999,23 +1054,21 @@ Kv8Shape kv8_attention_shape(std::uint32_t m, std::uint32_t q_heads, std::uint32
         const std::uint32_t splits = static_cast<std::uint32_t>((chunks + per - 1u) / per);
         return Kv8Shape{{static_cast<std::uint32_t>(pairs), static_cast<std::uint32_t>(splits > 1u ? whole : 0u), splits,
                          static_cast<std::uint32_t>(per)},
-                        tile_rows, kKv8Runs};
+                        tile_rows, kKv8Runs, run_weights};
     }
-    const std::uint32_t parts = (group + kVectors - 1u) / kVectors;
-    const std::uint64_t pairs = static_cast<std::uint64_t>(m) * kv_heads * parts;
     const auto shape = [&](std::uint64_t per, int kernel) {
-        return Kv8Shape{{static_cast<std::uint32_t>(pairs), 0u, static_cast<std::uint32_t>((chunks + per - 1u) / per),
+        return Kv8Shape{{static_cast<std::uint32_t>(row_pairs), 0u, static_cast<std::uint32_t>((chunks + per - 1u) / per),
                          static_cast<std::uint32_t>(per)},
-                        0u, kernel};
+                        0u, kernel, false};
     };
     // Few short rows: eight waves a workgroup walk a row's chunks in at most
     // four turns, without a second launch (32 rows over 500..1200 tokens: 11.2
     // us against 14; over 3000..4000 tokens 30 us against 19 with splits).
-    if (chunks <= 32u && pairs <= 256u) return shape(chunks, kKv8ShortRows);
+    if (chunks <= 32u && row_pairs <= 256u) return shape(chunks, kKv8ShortRows);
     // Splits of equal length, so that rows of unequal lengths make workgroups
     // of equal work: at least two chunks a wave, and at most about four
     // workgroups a CU if every row were max_tokens long.
-    std::uint64_t per = (pairs * chunks + 1023u) / 1024u;
+    std::uint64_t per = (row_pairs * chunks + 1023u) / 1024u;
     per = (per + kWaves - 1u) / kWaves * kWaves;
     if (per < 2u * kWaves) per = 2u * kWaves;
     return shape(per > chunks ? chunks : per, kKv8Rows);
@@ -1034,10 +1087,14 @@ Scratch scratch_of(const Kv8Shape& shape, std::uint32_t m, std::uint32_t q_heads
     const auto padded = [](std::uint64_t bytes) { return (bytes + 255u) / 256u * 256u; };
     Scratch s{};
     s.queries = weights ? padded(vectors * sizeof(float2)) : 0u;
-    const bool keep = weights && shape.kernel == kKv8Runs;
+    const bool keep = shape.run_weights;
     s.undos = s.queries + (keep ? vectors * head_dim * 2u * sizeof(_Float16) : 0u);
     s.partials = s.undos + (keep ? padded(vectors * sizeof(float)) : 0u);
-    s.bytes = s.partials + (shape.cut.splits > 1u ? vectors * shape.cut.splits * (head_dim + kStat) * sizeof(float) : 0u);
+    // Of runs the tiles that are cut have a place a vector, of rows all vectors.
+    const std::uint64_t places = shape.kernel == kKv8Runs
+                                     ? static_cast<std::uint64_t>(shape.cut.pairs - shape.cut.whole) * kVectors * kRunTiles
+                                     : vectors;
+    s.bytes = s.partials + (shape.cut.splits > 1u ? places * shape.cut.splits * (head_dim + kStat) * sizeof(float) : 0u);
     return s;
 }
 
@@ -1079,7 +1136,8 @@ void launch_typed(const Kv8Geometry& g, const float* qkv, std::uint64_t stride, 
     if (by_run) {
         AIR_KV8_ATTENTION(kRunTiles, true, kWaves);
         if (split) AIR_KV8_MERGE(kRunTiles, true);
-        if (weights) {
+        if (weights && !shape.run_weights) AIR_KV8_WEIGHTS(false, columns);
+        if (shape.run_weights) {
             hipLaunchKernelGGL((kv8_run_weights_kernel<TYPE, D>), dim3(chunks, g.kv_heads, runs), dim3(kThreads), 0, stream, g,
                                m, positions, tables, layer, q_heads, run_starts, max_tokens, scale, stats, queries, undos,
                                weights == 1);
@@ -1106,7 +1164,7 @@ hipError_t launch_kv8_attention(const Kv8Geometry& g, const float* qkv, std::uin
     const Scratch at = scratch_of(shape, m, q_heads, g.head_dim, weights != 0);
     unsigned char* const base = static_cast<unsigned char*>(scratch);
     float2* const stats = weights ? reinterpret_cast<float2*>(base) : nullptr;
-    const bool keep = weights && shape.kernel == kKv8Runs;
+    const bool keep = shape.run_weights;
     half8v* const queries = keep ? reinterpret_cast<half8v*>(base + at.queries) : nullptr;
     float* const undos = keep ? reinterpret_cast<float*>(base + at.undos) : nullptr;
     float* const partials = reinterpret_cast<float*>(base + at.partials);

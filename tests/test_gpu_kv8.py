@@ -667,6 +667,31 @@ def test_captured_steps_replay(torch_cuda):
 
 @pytest.mark.gpu
 @KINDS
+@pytest.mark.parametrize("q_heads,kvh,d,page_tokens,seqs", [
+    (14, 2, 128, 16, [(0, 400), (300, 101)]),
+    (6, 6, 64, 32, [(0, 331), (50, 90), (7, 1)]),
+])
+def test_large_prompts(torch_cuda, hip_ctx, kind, q_heads, kvh, d, page_tokens, seqs):
+    """Runs long enough for tiles of several rows without weights too; eight
+    rows at a time see the same tokens."""
+    rng = np.random.default_rng(131 + q_heads + kind)
+    lengths = [a + b + 8 for a, b in seqs]
+    cache, tables = _filled(kind, kvh, d, page_tokens, lengths, rng, layers=1, layer=0)
+    dev = Device(torch_cuda, hip_ctx, cache)
+    pos, tab, runs = [], [], []
+    for i, (a, b) in enumerate(seqs):
+        runs.append((len(pos), len(pos) + b))
+        pos += [a + r // 8 * 8 + 5 for r in range(b)]
+        tab += [tables[i]] * b
+    tab = np.array(tab)
+    x = rows(rng, len(pos), q_heads, kvh, d)
+    got = dev.attention(x, pos, tab, 0, q_heads, max(lengths), runs)
+    want, tol, _ = cache.attention(x, pos, tab, 0, q_heads, max(lengths), runs)
+    within(got, want, tol)
+
+
+@pytest.mark.gpu
+@KINDS
 def test_many_runs(torch_cuda, hip_ctx, kind):
     """Seventy runs of one to nine rows (and empty ones), more than a wave
     looks up at a time; forty q heads of one KV head, so two parts of a tile."""
