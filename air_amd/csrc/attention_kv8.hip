@@ -31,8 +31,8 @@
 // take the low bits of the others).  Rescaling by a power of two is exact.
 //
 // What bounds it.  Decode over a cache larger than the chip's: reading it (48
-// rows over 4000..16000 tokens, 32 q heads on 8 KV heads of 128 dims: 189 us,
-// 5.2 TB/s of the 985 MB, as a large copy).  Fewer tokens: the waits of one
+// rows over 4000..16000 tokens, 32 q heads on 8 KV heads of 128 dims: 193 us,
+// 5.1 TB/s of the 985 MB, as a large copy).  Fewer tokens: the waits of one
 // walk (32 rows over 500..1200 tokens: 11.3 us, 2.3 TB/s).  Prompts: the issue
 // of vector operations, some 20 a score (602 rows over 3300..3801 tokens, 28 q
 // heads: 85 us, 345 TFLOP/s of the products' 29 GFLOP; the matrix cores, which
@@ -1061,16 +1061,30 @@ Kv8Shape kv8_attention_shape(std::uint32_t m, std::uint32_t q_heads, std::uint32
                          static_cast<std::uint32_t>(per)},
                         0u, kernel, false};
     };
-    // Few short rows: eight waves a workgroup walk a row's chunks in at most
-    // four turns, without a second launch (32 rows over 500..1200 tokens: 11.2
-    // us against 14; over 3000..4000 tokens 30 us against 19 with splits).
-    if (chunks <= 32u && row_pairs <= 256u) return shape(chunks, kKv8ShortRows);
+    // Single rows, by the better of six ways over 510 calls of equal and 510 of
+    // unequal lengths (1..128 rows, up to 16000 tokens, 2 x 7, 4 x 7 and 8 x 4
+    // heads): this rule lies 2 % off it in the mean and 20 % at most.
+    //
+    // Eight waves a workgroup and one launch: up to two turns of the waves (32
+    // rows of 4 x 7 heads over 500..1200 tokens 11.8 us, 13.8 in splits), four
+    // with workgroups for half of the CUs, and any number where they fill
+    // them (64 such rows over 3000 tokens 33 us, 41 in splits).
+    const bool full = head_dim == 128u && row_pairs >= 160u;
+    if (row_pairs <= 256u && (chunks <= 16u || (chunks <= 32u && row_pairs >= 128u) || full)) {
+        return shape(chunks, kKv8ShortRows);
+    }
+    // More short rows than that: the splits' meeting would cost more than they
+    // even out (128 rows over 600 tokens 18 us, 24 in splits).
+    if (chunks <= 48u && row_pairs >= 320u) return shape(chunks, kKv8Rows);
     // Splits of equal length, so that rows of unequal lengths make workgroups
-    // of equal work: at least two chunks a wave, and at most about four
-    // workgroups a CU if every row were max_tokens long.
-    std::uint64_t per = (row_pairs * chunks + 1023u) / 1024u;
+    // of equal work, as many as run at a time if every row were max_tokens
+    // long: three a CU, or four with the registers of 64 dims.  At least a
+    // chunk a wave (one row over 2000 tokens 10.5 us, 15.3 unsplit), two where
+    // there are many.
+    const std::uint64_t slots = head_dim == 128u ? 768u : 1024u, least = chunks <= 32u ? kWaves : 2u * kWaves;
+    std::uint64_t per = (row_pairs * chunks + slots - 1u) / slots;
     per = (per + kWaves - 1u) / kWaves * kWaves;
-    if (per < 2u * kWaves) per = 2u * kWaves;
+    if (per < least) per = least;
     return shape(per > chunks ? chunks : per, kKv8Rows);
 }
 
