@@ -2307,7 +2307,7 @@ int air_hip_kv8_append(air_hip_context* ctx, const air_hip_kv8_layout* kv, const
     forget_loaded_source(ctx);
     if (int rc = check_kv8(kv); rc != AIR_HIP_OK) return rc;
     if (layer >= kv->layers) return fail(AIR_HIP_INVALID_ARGUMENT, "layer %u is out of range", layer);
-    if (row_stride < q_width + 2u * static_cast<uint64_t>(kv->kv_heads) * kv->head_dim) {
+    if (q_width > row_stride || row_stride - q_width < 2u * static_cast<uint64_t>(kv->kv_heads) * kv->head_dim) {
         return fail(AIR_HIP_INVALID_ARGUMENT, "row stride is shorter than q|k|v");
     }
     if (m == 0) return AIR_HIP_OK;

@@ -418,7 +418,7 @@ __global__ __launch_bounds__(kSelectThreads) void kv8_select_kernel(
         left = found_want;
     }
     // prefix is the want-th largest key, left how many keys equal to it stay.
-    std::uint32_t base_above = 0u, base_equal = 0u;   // larger and equal keys before this round
+    std::uint32_t base_above = 0u, base_equal = 0u;   // larger and equal keys before this pass
     for (std::uint32_t i0 = 0; i0 < count; i0 += kSelectThreads) {
         const std::uint32_t i = i0 + tid;
         const std::uint32_t key = i < count ? key_of(i) : 0u;

@@ -948,6 +948,8 @@ def test_sizes_past_the_grids_are_refused(torch_cuda, hip_ctx):
     assert attend(32, 32, 0, 1 << 27) == 6
     assert attend(16, 16, 0, 1 << 27) == 0
     kv = capi.Kv8Layout(p, 16, 1, 64, 1, 1 << 24, 1, None, 0, I8)
+    for width in (2 ** 64 - 128, 2 ** 64 - 1, 400):   # the first two pass 2^64 with k and v
+        assert lib.air_hip_kv8_append(h, ctypes.byref(kv), p, 512, width, 1, i, i, 0) == 1
     assert lib.air_hip_kv8_read(h, ctypes.byref(kv), 0, None, i, i, 0, 1, (1 << 27) + 1, p, None, None) == 6
     assert lib.air_hip_kv8_evict(h, ctypes.byref(kv), 0, i, i, i, 0, 1, 0, 0, 8, (1 << 27) + 1, i) == 6
     torch.cuda.synchronize()
