@@ -50,8 +50,9 @@ __device__ __forceinline__ float nan_f32() { return __builtin_nanf(""); }
 // decode step or a prompt stores in it (the next rows in the next slots) are
 // asked for before the other rows are looked through.  32 rows of 4 KV heads
 // of 128 dims take 7.4 us, two prompts of 509 rows 13.8 (1.4 and 4.4 more with
-// the loads one after the other), of which some 4 are the workgroups of the 15
-// of 16 rows that only find that their block has its writer.
+// the loads one after the other): 3.5 the launch with the 15 of 16 rows that
+// only find that their block has its writer (several rows a workgroup, in a
+// loop: 22), 1.4 the look at the other rows, the rest a writer's own waits.
 template <int TYPE, unsigned D>
 __global__ __launch_bounds__(2 * D) void kv8_append_kernel(Kv8Geometry g, const float* __restrict__ qkv,
                                                            std::uint64_t stride, std::uint64_t q_width,
@@ -458,8 +459,8 @@ __global__ __launch_bounds__(kSelectThreads) void kv8_select_kernel(
 // codes is touched: the old sequence is read whole (six layers of sequences
 // of 900..4100 tokens, 63 MB, and 25 MB written, in 33 us).  Measured slower:
 // four blocks a workgroup with their loads together (41 us), and 16 bytes a
-// dim and old block with the tokens picked from registers (52 us); fewer
-// workgroups a CU then cover each other's waits.
+// dim and old block with the tokens picked from registers (52 us) or from LDS
+// (36 us); fewer workgroups a CU then cover each other's waits.
 //
 // B > 1: in place.  One workgroup takes all blocks in ascending order, B at a
 // time.  Block b's tokens come from blocks >= b, so reading ahead is always
