@@ -41,6 +41,17 @@ __device__ __forceinline__ void kv8_store(Kv8Byte* p, T x) {
     *(__attribute__((address_space(1))) T*)p = x;
 }
 
+// x of this lane and those below it, summed: within rows of 16 lanes, then the
+// last lane of a row to the next, and of the lower half to the upper.
+__device__ __forceinline__ std::uint32_t wave_sums(std::uint32_t x) {
+    x += __builtin_amdgcn_update_dpp(0u, x, 0x111, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0u, x, 0x112, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0u, x, 0x114, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0u, x, 0x118, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0u, x, 0x142, 0xa, 0xf, false);
+    return x + __builtin_amdgcn_update_dpp(0u, x, 0x143, 0xc, 0xf, false);
+}
+
 // Entry of a page table that names block `block`'s page.
 __device__ __forceinline__ std::uint32_t kv8_slot(const Kv8Geometry& g, std::uint32_t block) {
     return g.page_magic == 0u ? block : __umulhi(block, g.page_magic);

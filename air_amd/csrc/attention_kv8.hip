@@ -316,17 +316,6 @@ struct Tile {
     std::uint32_t head, heads;     // q heads of each row
 };
 
-// x of this lane and those below it, summed: within rows of 16 lanes, then the
-// last lane of a row to the next, and of the lower half to the upper.
-__device__ __forceinline__ std::uint32_t wave_sums(std::uint32_t x) {
-    x += __builtin_amdgcn_update_dpp(0u, x, 0x111, 0xf, 0xf, true);
-    x += __builtin_amdgcn_update_dpp(0u, x, 0x112, 0xf, 0xf, true);
-    x += __builtin_amdgcn_update_dpp(0u, x, 0x114, 0xf, 0xf, true);
-    x += __builtin_amdgcn_update_dpp(0u, x, 0x118, 0xf, 0xf, true);
-    x += __builtin_amdgcn_update_dpp(0u, x, 0x142, 0xa, 0xf, false);
-    return x + __builtin_amdgcn_update_dpp(0u, x, 0x143, 0xc, 0xf, false);
-}
-
 // The tile that is `index`-th to start, of at most `tiles` tiles of the runs;
 // they count down, as the last rows of a run reach furthest.
 __device__ __forceinline__ Tile find_tile(std::uint32_t index, std::uint32_t tiles, const std::int32_t* __restrict__ run_starts,

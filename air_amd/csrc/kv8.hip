@@ -320,6 +320,7 @@ __global__ __launch_bounds__(256) void kv8_read_weights_kernel(Kv8Geometry g, st
 // ---- eviction ----------------------------------------------------------------
 
 constexpr unsigned kSelectThreads = 1024;
+constexpr unsigned kSelectBins = 2 * kSelectThreads;
 constexpr std::uint32_t kSelectKeys = 16384;   // keys held in LDS; longer sequences are read again each pass
 
 // Weights as unsigned integers of the same order; NaN (and a token whose page
@@ -338,20 +339,21 @@ __device__ __forceinline__ std::int64_t held_tokens(const Kv8Geometry& g, std::i
 }
 
 // The tokens a (sequence, layer, KV head) keeps, ascending, -1 behind them.
-// The want-th largest key of the middle tokens is found byte by byte from the
-// top (a histogram of the next byte over the keys that agree so far); then one
-// pass in token order writes the first keep_first, every larger key, as many
-// equal ones as are still wanted (the lowest tokens) and the last keep_last.
-// One workgroup has nothing to overlap its waits with, so the keys are read
-// once, into LDS, and a wave finds a byte's bin with a prefix sum: 1000 tokens
-// to 500 in 7 us, 4096 to 1024 in 16, the rounds' barriers and LDS additions.
+// The want-th largest key of the middle tokens is found from the top by 11, 11
+// and 10 bits (a histogram of the next digit over the keys that agree so far);
+// then one pass in token order writes the first keep_first, every larger key,
+// as many equal ones as are still wanted (the lowest tokens) and the last
+// keep_last.  One workgroup has nothing to overlap its waits with, so the keys
+// are read once, into LDS, and digits and places are found with prefix sums:
+// 1000 tokens to 500 in 7 us, 4096 to 1024 in 13 (16 by four bytes, whose
+// first has few values and many additions to one bin), the rounds' barriers.
 __global__ __launch_bounds__(kSelectThreads) void kv8_select_kernel(
     Kv8Geometry g, const std::int32_t* __restrict__ lengths, const std::int32_t* __restrict__ tables,
     std::uint32_t layer, std::uint32_t layers, std::uint32_t keep_first, std::uint32_t keep_last, std::uint32_t budget,
     std::uint64_t max_tokens, std::int32_t* __restrict__ kept) {
     constexpr unsigned kWaves = kSelectThreads / 64u;
     __shared__ std::uint32_t keys[kSelectKeys];
-    __shared__ std::uint32_t bins[256];
+    __shared__ std::uint32_t bins[kSelectBins];
     __shared__ std::uint32_t found_prefix, found_want;
     __shared__ std::uint32_t wave_above[kWaves], wave_equal[kWaves];
     const std::uint32_t head = blockIdx.x, l = blockIdx.y, seq = blockIdx.z;
@@ -384,68 +386,71 @@ __global__ __launch_bounds__(kSelectThreads) void kv8_select_kernel(
         return i < kSelectKeys ? keys[i] : read_key(lo + i);
     };
     std::uint32_t prefix = 0u, left = want;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        if (tid < 256u) bins[tid] = 0u;
+    for (int shift = 21;; shift = shift == 21 ? 10 : 0) {   // 11, 11 and 10 bits
+        bins[2u * tid] = bins[2u * tid + 1u] = 0u;
         __syncthreads();
         for (std::uint32_t i = tid; i < count; i += kSelectThreads) {
             const std::uint32_t key = key_of(i);
             // Shifts of 32 are undefined: the first round takes every key.
-            if (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&bins[(key >> shift) & 255u], 1u);
+            const bool agrees = shift == 21 || (shift == 10 ? key >> 21 == prefix >> 21 : key >> 10 == prefix >> 10);
+            if (agrees) atomicAdd(&bins[(key >> shift) & (shift == 0 ? 1023u : 2047u)], 1u);
         }
         __syncthreads();
-        if (wave == 0u) {
-            // Lane i holds bins 255 - 4 i and down; sums from the top.
-            std::uint32_t b[4], sum = 0u;
+        // Thread t holds two bins from the top; sums of those above.
+        const std::uint32_t at = kSelectBins - 1u - 2u * tid, high = bins[at], low = bins[at - 1u];
+        const std::uint32_t upto = wave_sums(high + low);
+        if (lane == 63u) wave_above[wave] = upto;
+        __syncthreads();
+        std::uint32_t before = upto - high - low;
 #pragma unroll
-            for (unsigned j = 0; j < 4u; ++j) sum += b[j] = bins[255u - 4u * lane - j];
-            std::uint32_t upto = sum;
-#pragma unroll
-            for (unsigned off = 1; off < 64u; off <<= 1) {
-                const std::uint32_t o = static_cast<std::uint32_t>(__shfl_up(static_cast<int>(upto), off));
-                if (lane >= off) upto += o;
-            }
-            std::uint32_t before = upto - sum;
-#pragma unroll
-            for (unsigned j = 0; j < 4u; ++j) {
-                if (before < left && before + b[j] >= left) {   // one bin of one lane: the left-th key is in it
-                    found_prefix = prefix | (255u - 4u * lane - j) << shift;
-                    found_want = left - before;
-                }
-                before += b[j];
-            }
+        for (unsigned w = 0; w < kWaves; ++w) before += w < wave ? wave_above[w] : 0u;
+        if (before < left && before + high + low >= left) {   // one thread: the left-th key is in one of its bins
+            const bool upper = before + high >= left;
+            found_prefix = prefix | (upper ? at : at - 1u) << shift;
+            found_want = left - before - (upper ? 0u : high);
         }
         __syncthreads();
         prefix = found_prefix;
         left = found_want;
+        if (shift == 0) break;
     }
     // prefix is the want-th largest key, left how many keys equal to it stay.
-    std::uint32_t base_above = 0u, base_equal = 0u;   // larger and equal keys before this pass
-    for (std::uint32_t i0 = 0; i0 < count; i0 += kSelectThreads) {
-        const std::uint32_t i = i0 + tid;
-        const std::uint32_t key = i < count ? key_of(i) : 0u;
-        const bool above = i < count && key > prefix, equal = i < count && key == prefix;
-        const std::uint64_t above_mask = __ballot(above), equal_mask = __ballot(equal);
-        if (lane == 0u) {
-            wave_above[wave] = static_cast<std::uint32_t>(__popcll(above_mask));
-            wave_equal[wave] = static_cast<std::uint32_t>(__popcll(equal_mask));
+    // A thread's tokens lie together, so one prefix sum over the threads places
+    // them (16384 tokens at a time: 16 a thread, whose weights are one line).
+    std::uint32_t base_above = 0u, base_equal = 0u;   // larger and equal keys before these tokens
+    for (std::uint32_t from = 0u; from < count; from += kSelectKeys) {
+        const std::uint32_t here = count - from < kSelectKeys ? count - from : kSelectKeys;
+        const std::uint32_t each = (here + kSelectThreads - 1u) / kSelectThreads;
+        const std::uint32_t begin = from + (tid * each < here ? tid * each : here);
+        const std::uint32_t end = from + here - begin < each ? from + here : begin + each;
+        std::uint32_t above = 0u, equal = 0u;
+        for (std::uint32_t i = begin; i < end; ++i) {
+            const std::uint32_t key = key_of(i);
+            above += key > prefix ? 1u : 0u;
+            equal += key == prefix ? 1u : 0u;
+        }
+        const std::uint32_t above_upto = wave_sums(above), equal_upto = wave_sums(equal);
+        if (lane == 63u) {
+            wave_above[wave] = above_upto;
+            wave_equal[wave] = equal_upto;
         }
         __syncthreads();
-        std::uint32_t a = base_above, e = base_equal, all_above = 0u, all_equal = 0u;
+        std::uint32_t a = base_above + above_upto - above, e = base_equal + equal_upto - equal;
 #pragma unroll
         for (unsigned w = 0; w < kWaves; ++w) {
             a += w < wave ? wave_above[w] : 0u;
             e += w < wave ? wave_equal[w] : 0u;
-            all_above += wave_above[w];
-            all_equal += wave_equal[w];
+            base_above += wave_above[w];
+            base_equal += wave_equal[w];
         }
-        const std::uint64_t below = (1ull << lane) - 1u;
-        a += static_cast<std::uint32_t>(__popcll(above_mask & below));
-        e += static_cast<std::uint32_t>(__popcll(equal_mask & below));
-        if (above || (equal && e < left)) {
-            out[keep_first + a + (e < left ? e : left)] = static_cast<std::int32_t>(lo + i);
+        for (std::uint32_t i = begin; i < end; ++i) {
+            const std::uint32_t key = key_of(i);
+            if (key > prefix || (key == prefix && e < left)) {
+                out[keep_first + a + (e < left ? e : left)] = static_cast<std::int32_t>(lo + i);
+            }
+            a += key > prefix ? 1u : 0u;
+            e += key == prefix ? 1u : 0u;
         }
-        base_above += all_above;
-        base_equal += all_equal;
         __syncthreads();
     }
 }
@@ -467,7 +472,7 @@ __global__ __launch_bounds__(kSelectThreads) void kv8_select_kernel(
 // safe, and a block may be written once every block up to it has been read:
 // all B are read, with the sources of the next B looked up meanwhile, then
 // written (24 sequences and layers of 4096 tokens to 1024, four KV heads, the
-// whole call: 203 us with one block at a time and no reading ahead, 80 so; 41
+// whole call: 203 us with one block at a time and no reading ahead, 78 so; 38
 // to another table).
 template <int TYPE, unsigned D, unsigned B>
 __global__ __launch_bounds__(2 * D * B) void kv8_compact_kernel(Kv8Geometry g, const std::int32_t* tables,
