@@ -774,10 +774,10 @@ __device__ __forceinline__ ChunkRecords chunk_records(const Kv8Geometry& g, std:
 // token takes one atomic addition: a page that two runs share loses nothing,
 // and elsewhere a single addition leaves one order.
 //
-// For tiles of single rows: a chunk of a (run, KV head) is one wave's.  MERGE,
-// where they were split: the grid's first column joins the splits of a run's
-// rows, and the others take the statistics from the partials themselves, so
-// that one launch follows the attention.
+// A chunk of a (run, KV head) is one wave's, which takes the run's vectors 16
+// at a time.  MERGE, where single rows were split: the grid's first column
+// joins the splits of a run's rows, and the others take the statistics from
+// the partials themselves, so that one launch follows the attention.
 template <int TYPE, unsigned D, bool MERGE>
 __global__ __launch_bounds__(kThreads, 3) void kv8_weights_kernel(
     Kv8Geometry g, const float* __restrict__ qkv, std::uint64_t stride, std::uint32_t m,
@@ -889,7 +889,7 @@ __global__ __launch_bounds__(kThreads, 3) void kv8_weights_kernel(
     put_weight(vrec, first, last, col, sum[0], add);
 }
 
-// The same for runs of several rows: a chunk is a workgroup's, whose waves take
+// The same for runs of many vectors: a chunk is a workgroup's, whose waves take
 // the vectors 16 at a time in turn and add up in LDS.  The attention left the
 // vectors' operands, and a wave reads 16 vectors ahead (four runs of 32 rows
 // over 2900..4100 tokens, 28 q heads on 4 KV heads of 128 dims: 30 us where
