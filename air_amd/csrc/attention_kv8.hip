@@ -635,53 +635,68 @@ __device__ __forceinline__ std::uint32_t live_splits(int reach, std::uint64_t ma
     return (chunks + split_chunks - 1u) / split_chunks;
 }
 
-// Dims 4 d4 .. + 3 of a vector from its splits' partials, eight loads in flight.
-template <unsigned D>
-__device__ __forceinline__ float4v join_splits(const float* __restrict__ base, std::uint32_t live, unsigned d4, int& ref,
-                                               float& total) {
-    constexpr unsigned kBatch = 8;
-    ref = kNone;
-    total = 0.0f;
-    int ref2 = kNone;
+// Dims 4 d4 .. + 3 of a vector over splits of it: references, denominator and
+// sums so far.
+struct Joined {
+    int ref = kNone, ref2 = kNone;
+    float total = 0.0f;
     float4v acc = {0.f, 0.f, 0.f, 0.f};
-    for (std::uint32_t s0 = 0; s0 < live; s0 += kBatch) {
+};
+
+__device__ __forceinline__ void join(Joined& x, int ref, int ref2, float total, const float4v& acc) {
+    const int next = ref > x.ref ? ref : x.ref, next2 = ref2 > x.ref2 ? ref2 : x.ref2;
+    x.total = __builtin_amdgcn_ldexpf(x.total, x.ref - next) + __builtin_amdgcn_ldexpf(total, ref - next);
+#pragma unroll
+    for (unsigned r = 0; r < 4u; ++r) {
+        x.acc[r] = __builtin_amdgcn_ldexpf(x.acc[r], x.ref2 - next2) + __builtin_amdgcn_ldexpf(acc[r], ref2 - next2);
+    }
+    x.ref = next;
+    x.ref2 = next2;
+}
+
+// Splits begin .. end - 1 of a vector's partials, eight loads in flight.
+template <unsigned D>
+__device__ __forceinline__ Joined join_splits(const float* __restrict__ base, std::uint32_t begin, std::uint32_t end,
+                                              unsigned d4) {
+    constexpr unsigned kBatch = 8;
+    Joined x;
+    for (std::uint32_t s0 = begin; s0 < end; s0 += kBatch) {
         float4v head[kBatch], sums[kBatch];
 #pragma unroll
         for (unsigned j = 0; j < kBatch; ++j) {
-            const std::uint32_t at = (s0 + j < live ? s0 + j : live - 1u) * (D + kStat);
+            const std::uint32_t at = (s0 + j < end ? s0 + j : end - 1u) * (D + kStat);
             head[j] = *reinterpret_cast<const float4v*>(base + at);
             sums[j] = *reinterpret_cast<const float4v*>(base + at + kStat + 4u * d4);
         }
 #pragma unroll
         for (unsigned j = 0; j < kBatch; ++j) {
-            if (s0 + j >= live) continue;
-            const int a = __float_as_int(head[j][0]), a2 = __float_as_int(head[j][1]);
-            const int next = a > ref ? a : ref, next2 = a2 > ref2 ? a2 : ref2;
-            total = __builtin_amdgcn_ldexpf(total, ref - next) + __builtin_amdgcn_ldexpf(head[j][2], a - next);
-#pragma unroll
-            for (unsigned r = 0; r < 4u; ++r) {
-                acc[r] = __builtin_amdgcn_ldexpf(acc[r], ref2 - next2) + __builtin_amdgcn_ldexpf(sums[j][r], a2 - next2);
-            }
-            ref = next;
-            ref2 = next2;
+            if (s0 + j < end) join(x, __float_as_int(head[j][0]), __float_as_int(head[j][1]), head[j][2], sums[j]);
         }
     }
+    return x;
+}
+
+__device__ __forceinline__ float4v normalised(const Joined& x) {
     float4v y;
 #pragma unroll
     for (unsigned r = 0; r < 4u; ++r) {
-        y[r] = total == 0.0f ? 0.0f : __builtin_amdgcn_ldexpf(acc[r] / total, ref2 - kPBits - ref);
+        y[r] = x.total == 0.0f ? 0.0f : __builtin_amdgcn_ldexpf(x.acc[r] / x.total, x.ref2 - kPBits - x.ref);
     }
     return y;
 }
 
 // Joins the splits of a tile's vectors.  A launch of its own costs 4 us here;
-// what it reads (a few MB) costs less.
-template <unsigned D, unsigned NV, bool RUNS>
+// what it reads (a few MB) costs less.  WIDE, for more than 16 splits: a
+// workgroup a vector, whose threads take a slice of the splits each and meet
+// in LDS (one row of 2 x 7 heads over 131072 tokens, 256 splits: 24 us with the
+// attention, 70 where a thread joins all of them).
+template <unsigned D, unsigned NV, bool RUNS, bool WIDE>
 __global__ __launch_bounds__(kThreads) void kv8_merge_kernel(
     const std::int32_t* __restrict__ positions, std::uint32_t m, std::uint32_t q_heads, std::uint32_t kv_heads,
     const std::int32_t* __restrict__ run_starts, std::uint32_t runs, std::uint32_t tile_rows, std::uint64_t max_tokens,
     Kv8Cut cut, const float* __restrict__ partials, float2* __restrict__ stats, float* __restrict__ out) {
     constexpr unsigned kTile = kVectors * NV;
+    constexpr unsigned kPieces = D / 4u, kSlices = WIDE ? kThreads / kPieces : 1u;
     const std::uint32_t group = q_heads / kv_heads, parts = (group + kTile - 1u) / kTile;
     const Kv8Work work = kv8_work(cut, cut.whole + blockIdx.x, kv_heads * parts);
     const std::uint32_t kvh = work.tile_head / parts, part = work.tile_head % parts;
@@ -697,17 +712,36 @@ __global__ __launch_bounds__(kThreads) void kv8_merge_kernel(
     }
     const std::uint32_t live = live_splits(reach, max_tokens, cut.split_chunks), splits = cut.splits;
     if (live <= 1u) return;   // the attention kernel wrote this tile
-    for (unsigned idx = blockIdx.y * kThreads + threadIdx.x; idx < tile.rows * tile.heads * (D / 4u);
-         idx += gridDim.y * kThreads) {
-        const unsigned v = idx / (D / 4u), d4 = idx % (D / 4u);
+    const unsigned d4 = threadIdx.x % kPieces, slice = WIDE ? threadIdx.x / kPieces : 0u;
+    const unsigned step = WIDE ? 1u : kThreads / kPieces;   // vectors at a time
+    for (unsigned v = blockIdx.y * step + (WIDE ? 0u : threadIdx.x / kPieces); v < tile.rows * tile.heads;
+         v += gridDim.y * step) {
         const std::uint64_t vector =
             static_cast<std::uint64_t>(tile.row + v / tile.heads) * q_heads + tile.head + v % tile.heads;
-        int ref;
-        float total;
         const std::uint64_t place = RUNS ? static_cast<std::uint64_t>(blockIdx.x) * kTile + v : vector;
-        const float4v y = join_splits<D>(partials + place * splits * (D + kStat), live, d4, ref, total);
-        *reinterpret_cast<float4v*>(out + vector * D + 4u * d4) = y;
-        if (stats && d4 == 0u) stats[vector] = make_float2(static_cast<float>(ref), total == 0.0f ? 0.0f : 1.0f / total);
+        const float* const base = partials + place * splits * (D + kStat);
+        const std::uint32_t each = (live + kSlices - 1u) / kSlices, from = slice * each < live ? slice * each : live;
+        Joined x = join_splits<D>(base, from, live - from < each ? live : from + each, d4);
+        if constexpr (WIDE) {
+            __shared__ float4v sums[kSlices][kPieces];
+            __shared__ int refs[kSlices], refs2[kSlices];
+            __shared__ float totals[kSlices];
+            __syncthreads();   // the vector before is out
+            sums[slice][d4] = x.acc;
+            if (d4 == 0u) {
+                refs[slice] = x.ref;
+                refs2[slice] = x.ref2;
+                totals[slice] = x.total;
+            }
+            __syncthreads();
+            if (slice != 0u) continue;
+#pragma unroll
+            for (unsigned w = 1; w < kSlices; ++w) join(x, refs[w], refs2[w], totals[w], sums[w][d4]);
+        }
+        *reinterpret_cast<float4v*>(out + vector * D + 4u * d4) = normalised(x);
+        if (stats && d4 == 0u) {
+            stats[vector] = make_float2(static_cast<float>(x.ref), x.total == 0.0f ? 0.0f : 1.0f / x.total);
+        }
     }
 }
 
@@ -775,9 +809,10 @@ __device__ __forceinline__ ChunkRecords chunk_records(const Kv8Geometry& g, std:
 // and elsewhere a single addition leaves one order.
 //
 // A chunk of a (run, KV head) is one wave's, which takes the run's vectors 16
-// at a time.  MERGE, where single rows were split: the grid's first column
-// joins the splits of a run's rows, and the others take the statistics from
-// the partials themselves, so that one launch follows the attention.
+// at a time.  MERGE, where single rows were split up to 16 times: the grid's
+// first column joins the splits of a run's rows, and the others take the
+// statistics from the partials themselves, so that one launch follows the
+// attention.
 template <int TYPE, unsigned D, bool MERGE>
 __global__ __launch_bounds__(kThreads, 3) void kv8_weights_kernel(
     Kv8Geometry g, const float* __restrict__ qkv, std::uint64_t stride, std::uint32_t m,
@@ -805,10 +840,8 @@ __global__ __launch_bounds__(kThreads, 3) void kv8_weights_kernel(
             const std::uint64_t vector = static_cast<std::uint64_t>(r) * q_heads + head0 + v % group;
             const std::uint32_t live = live_splits(positions[r], max_tokens, split_chunks);
             if (live <= 1u) continue;   // the attention kernel wrote this row
-            int ref;
-            float total;
             *reinterpret_cast<float4v*>(out + vector * D + 4u * d4) =
-                join_splits<D>(partials + vector * splits * (D + kStat), live, d4, ref, total);
+                normalised(join_splits<D>(partials + vector * splits * (D + kStat), 0u, live, d4));
         }
         return;
     }
@@ -1121,15 +1154,22 @@ void launch_typed(const Kv8Geometry& g, const float* qkv, std::uint64_t stride, 
     const Kv8Cut& cut = shape.cut;
     const bool split = cut.splits > 1u, by_run = shape.kernel == kKv8Runs;
     const dim3 grid(cut.whole + (cut.pairs - cut.whole) * cut.splits);
-    // A tile of several MFMA tiles is joined by several workgroups.
-    const dim3 merge_grid(cut.pairs - cut.whole, by_run ? 4u : 1u);
+    // A tile of several MFMA tiles is joined by several workgroups, and one of
+    // many splits by one a vector.
+    const bool wide = cut.splits > 16u;
+    const dim3 merge_grid(cut.pairs - cut.whole, wide ? kVectors : by_run ? 4u : 1u);
 #define AIR_KV8_ATTENTION(NV, RUNS, W)                                                                               \
     hipLaunchKernelGGL((kv8_attention_kernel<TYPE, D, NV, RUNS, W>), grid, dim3(64 * W), 0, stream, g, qkv, stride, m, \
                        positions, tables, layer, q_heads, run_starts, runs, shape.tile_rows, max_tokens, cut, scale, \
                        partials, stats, queries, undos, out)
-#define AIR_KV8_MERGE(NV, RUNS)                                                                                      \
-    hipLaunchKernelGGL((kv8_merge_kernel<D, NV, RUNS>), merge_grid, dim3(kThreads), 0, stream, positions, m, q_heads, \
+#define AIR_KV8_MERGE_KERNEL(NV, RUNS, WIDE)                                                                         \
+    hipLaunchKernelGGL((kv8_merge_kernel<D, NV, RUNS, WIDE>), merge_grid, dim3(kThreads), 0, stream, positions, m, q_heads, \
                        g.kv_heads, run_starts, runs, shape.tile_rows, max_tokens, cut, partials, stats, out)
+#define AIR_KV8_MERGE(NV, RUNS)                         \
+    do {                                                \
+        if (wide) AIR_KV8_MERGE_KERNEL(NV, RUNS, true); \
+        else AIR_KV8_MERGE_KERNEL(NV, RUNS, false);     \
+    } while (false)
 #define AIR_KV8_WEIGHTS(MERGE, COLUMNS)                                                                              \
     hipLaunchKernelGGL((kv8_weights_kernel<TYPE, D, MERGE>), dim3(COLUMNS, g.kv_heads, run_starts ? runs : m), \
                        dim3(kThreads), 0, stream, g, qkv, stride, m, positions, tables, layer, q_heads, run_starts,  \
@@ -1148,12 +1188,14 @@ void launch_typed(const Kv8Geometry& g, const float* qkv, std::uint64_t stride, 
     } else {
         if (shape.kernel == kKv8ShortRows) AIR_KV8_ATTENTION(1u, false, kShortWaves);
         else AIR_KV8_ATTENTION(1u, false, kWaves);
-        if (weights && split) AIR_KV8_WEIGHTS(true, columns + 1u);
-        else if (weights) AIR_KV8_WEIGHTS(false, columns);
-        else if (split) AIR_KV8_MERGE(1u, false);
+        const bool together = weights && split && !wide;   // splits and weights in one launch
+        if (together) AIR_KV8_WEIGHTS(true, columns + 1u);
+        if (split && !together) AIR_KV8_MERGE(1u, false);
+        if (weights && !together) AIR_KV8_WEIGHTS(false, columns);
     }
 #undef AIR_KV8_ATTENTION
 #undef AIR_KV8_MERGE
+#undef AIR_KV8_MERGE_KERNEL
 #undef AIR_KV8_WEIGHTS
 }
 

@@ -767,6 +767,29 @@ def test_runs_of_one_row_over_split_keys(torch_cuda, hip_ctx, kind):
 
 
 @pytest.mark.gpu
+@KINDS
+@pytest.mark.parametrize("d", [64, 128])
+def test_many_splits(torch_cuda, hip_ctx, kind, d):
+    """Keys cut into more splits than one thread joins: single rows, one of
+    them short, and a run, without weights and with."""
+    rng = np.random.default_rng(141 + d + kind)
+    q_heads, kvh, n = 3, 1, 9100
+    cache, tables = _filled(kind, kvh, d, 64, [n, 100], rng, layers=1, layer=0)
+    dev = Device(torch_cuda, hip_ctx, cache)
+    single = ([n - 1, 99], tables, None)
+    run = ([n - 1 - 290 * (r % 3) for r in range(30)], np.repeat(tables[:1], 30, axis=0), [(0, 30)])
+    for pos, tab, runs in (single, run):
+        for mode, name in ((capi.KV8_WEIGHTS_NONE, None), (capi.KV8_WEIGHTS_SET, "set")):
+            x = rows(rng, len(pos), q_heads, kvh, d)
+            got = dev.attention(x, pos, tab, 0, q_heads, n, runs, weights=mode)
+            want, tol, far = cache.attention(x, pos, tab, 0, q_heads, n, runs, weights=name)
+            within(got, want, tol)
+            pool = dev.pool()
+            check_weights(cache, pool, far)
+            cache.pool[...] = pool
+
+
+@pytest.mark.gpu
 def test_runs_that_share_pages_add_up(torch_cuda, hip_ctx):
     """Two runs over one sequence's pages: what both add to a weight is
     there, whichever comes first (each addition rounds once)."""
