@@ -179,11 +179,14 @@ __device__ __forceinline__ void load_keys(const Kv8Byte* rec, unsigned lane, Key
     }
 }
 
-// What a block's scores are multiplied by.  A block without a scale has codes
-// of zero; any factor will do, and one makes its masked scores -inf.
+// What a block's scores are multiplied by.  Scores are whole numbers below
+// 2^27, so a factor below f32's normal range leaves nothing of them (nor does
+// a scale of zero, whose codes are zero): the smallest normal number stands
+// for it, which keeps masked scores at -inf where zero would make them NaN.
+// A NaN scale passes.
 __device__ __forceinline__ float score_factor(float unit, float k_scale) {
     const float f = unit * k_scale;
-    return f == 0.0f ? 1.0f : f;
+    return f < 0x1p-126f ? 0x1p-126f : f;
 }
 // 2^(score * factor - base), one rounding
 __device__ __forceinline__ float score_power(float score, float factor, float base) {

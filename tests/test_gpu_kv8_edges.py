@@ -1,0 +1,72 @@
+"""The 8-bit KV cache at the ends of f32's range, captured calls that cut their
+keys, and the kernels and branches that only particular sizes reach.
+
+gpu: each against the model of kv8_model.py in 64 bits, or, replayed from a
+     graph, against the eager calls.
+"""
+import ctypes
+import math
+
+import numpy as np
+import pytest
+
+from air_amd import capi
+from tests.kv8_model import Cache, page_tables
+from tests.test_gpu_kv8 import Device, check_weights, rows, same, within
+
+I8, E4M3 = capi.KV8_I8, capi.KV8_E4M3
+KINDS = pytest.mark.parametrize("kind", [I8, E4M3], ids=["i8", "e4m3"])
+MODES = {None: capi.KV8_WEIGHTS_NONE, "add": capi.KV8_WEIGHTS_ADD, "set": capi.KV8_WEIGHTS_SET}
+
+
+def filled(kind, kvh, d, lengths, rng, max_pages=None, k_scale=None, page_tokens=16):
+    """A cache of one layer whose K of token t is k_scale(sequence, t) times
+    an ordinary one, stored by the model's append."""
+    pages = max(-(-n // page_tokens) for n in lengths)
+    cache = Cache(kind, kvh, d, 1, page_tokens, pages * len(lengths) + 3, max_pages or pages + 2, seed=kind)
+    tables = page_tables(rng, lengths, page_tokens, cache.max_pages, cache.pool_pages)
+    for i, n in enumerate(lengths):
+        x = rows(rng, n, 0, kvh, d, spread=0.5)
+        if k_scale is not None:
+            x[:, :kvh * d] *= np.array([[k_scale(i, t)] for t in range(n)], dtype=np.float32)
+        for a in range(0, n, 2048):
+            b = min(n, a + 2048)
+            cache.append(x[a:b], 0, list(range(a, b)), np.repeat(tables[i:i + 1], b - a, axis=0), 0)
+    return cache, tables
+
+
+def attend(dev, x, pos, tab, q_heads, max_tokens, runs=None, mode=None):
+    """One call checked against the model, output and weights."""
+    got = dev.attention(x, pos, tab, 0, q_heads, max_tokens, runs, weights=MODES[mode])
+    want, tol, far = dev.cache.attention(x, pos, tab, 0, q_heads, max_tokens, runs, weights=mode)
+    print("rows", len(pos), "runs", runs and len(runs), mode, flush=True)
+    within(got, want, tol)
+    if mode:
+        pool = dev.pool()
+        check_weights(dev.cache, pool, far)
+        dev.cache.pool[...] = pool
+
+
+@pytest.mark.gpu
+@KINDS
+@pytest.mark.parametrize("q_scale,k_scale", [(1.0, 1e-42), (1e-25, 1e-25), (1e-18, 1e-22), (1e-32, 1e-12)])
+def test_products_below_f32(torch_cuda, hip_ctx, kind, q_scale, k_scale):
+    """q and K whose products lie below f32's range, K of stored scales above
+    zero: scores of nothing, so every token weighs the same.  An ordinary block
+    lies between such blocks, and one row of ordinary q between such rows."""
+    rng = np.random.default_rng(kind + int(-math.log10(q_scale * k_scale)))
+    q_heads, kvh, d, n = 14, 2, 128, 600
+    cache, tables = filled(kind, kvh, d, [n, 101, 95], rng, k_scale=lambda i, t: 1.0 if t // 16 == 3 else k_scale)
+    k_scales = Cache.floats(cache.pool[tables[0, 4], 0, :, 0])[:, 0]
+    assert (k_scales > 0).all()
+    dev = Device(torch_cuda, hip_ctx, cache)
+
+    def query(m):
+        x = rows(rng, m, q_heads, kvh, d)
+        x[np.arange(m) != 1] *= np.float32(q_scale)
+        return x
+    for mode in (None, "set"):
+        attend(dev, query(3), [n - 1, 100, 94], tables, q_heads, 110, None, mode)
+        attend(dev, query(2), [n - 1, 70], tables[:2], q_heads, n, None, mode)        # cut
+        attend(dev, query(40), [60 + t for t in range(40)], np.repeat(tables[:1], 40, axis=0), q_heads, 110, [(0, 40)],
+               mode)
