@@ -127,7 +127,7 @@ __device__ __forceinline__ void load_query(const float* q, unsigned grp, QueryFr
     top = fmaxf(top, __shfl_xor(top, 16));
     top = fmaxf(top, __shfl_xor(top, 32));
     int e = static_cast<int>(__float_as_uint(top) >> 23) - 127;   // -127: zero or subnormal; 128: not finite
-    e = e < -110 ? -110 : e > 120 ? 120 : e;
+    e = e < -110 ? -110 : e > 127 ? 127 : e;   // both scales stay normal numbers
     const float scale = __uint_as_float(static_cast<std::uint32_t>(127 + 10 - e) << 23);
     f.undo = __uint_as_float(static_cast<std::uint32_t>(127 - 10 + e) << 23);
 #pragma unroll

@@ -70,3 +70,20 @@ def test_products_below_f32(torch_cuda, hip_ctx, kind, q_scale, k_scale):
         attend(dev, query(2), [n - 1, 70], tables[:2], q_heads, n, None, mode)        # cut
         attend(dev, query(40), [60 + t for t in range(40)], np.repeat(tables[:1], 40, axis=0), q_heads, 110, [(0, 40)],
                mode)
+
+
+@pytest.mark.gpu
+@KINDS
+def test_queries_up_to_f32s_largest(torch_cuda, hip_ctx, kind):
+    """q of 2^126 and more over K as small: ordinary scores."""
+    rng = np.random.default_rng(7 + kind)
+    q_heads, kvh, d, n = 14, 2, 128, 200
+    cache, tables = filled(kind, kvh, d, [n, n], rng, k_scale=lambda i, t: 2.0 ** -126)
+    dev = Device(torch_cuda, hip_ctx, cache)
+    for m, runs in ((2, None), (40, [(0, 40)])):
+        x = rows(rng, m, q_heads, kvh, d)
+        x[:, :q_heads * d] = np.clip(x[:, :q_heads * d], -3.9, 3.9) * np.float32(2.0 ** 126)
+        assert np.isfinite(x).all() and np.abs(x).max() > 2.0 ** 126
+        for mode in (None, "set"):
+            tab = np.repeat(tables[:1], m, axis=0) if runs else tables
+            attend(dev, x, [n - 1 - r for r in range(m)], tab, q_heads, n, runs, mode)
