@@ -210,7 +210,8 @@ def prepare(case, seed):
     if case["kind"] == "append":
         starts = _spread(case, case["start_min"], case["start_max"])
         lens = [s + run for s in starts]
-        back = -(-run // BLOCK) * BLOCK + BLOCK       # tokens read back of each sequence, at most
+        # Tokens read back of each sequence, at most: no more than a table names.
+        back = min(-(-run // BLOCK) * BLOCK + BLOCK, _max_pages(case, max(lens)) * case["page_tokens"])
         lo = [s // BLOCK * BLOCK for s in starts]
         state.update(back=back, lo=torch.tensor(lo, dtype=torch.int32, device="cuda"),
                      count=torch.tensor([n - b for n, b in zip(lens, lo)], dtype=torch.int32, device="cuda"),
