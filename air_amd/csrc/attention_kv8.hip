@@ -25,10 +25,12 @@
 // vector's statistics stay in its lanes (lane % 16), and an output lane holds
 // four consecutive dims of one vector.
 //
-// Running references are integers, in powers of two: M >= every s log2(e) so
-// far (for the denominator) and M2 >= every s log2(e) + log2(scale of V) (for
+// Running references are whole numbers, in powers of two: M >= every s log2(e)
+// so far (for the denominator) and M2 >= every s log2(e) + log2(scale of V) (for
 // the numerators, whose p carries V's scale: a block of large values does not
-// take the low bits of the others).  Rescaling by a power of two is exact.
+// take the low bits of the others).  Rescaling by a power of two is exact.  M
+// is an f32, so that scores of any size up to f32's largest do; M2 is held as
+// its lead over M.
 //
 // What bounds it.  Decode over a cache larger than the chip's: reading it (48
 // rows over 4000..16000 tokens, 32 q heads on 8 KV heads of 128 dims: 193 us,
@@ -51,7 +53,8 @@ constexpr unsigned kVectors = 16;          // query vectors of an MFMA tile
 constexpr unsigned kRunTiles = 2;          // MFMA tiles of a workgroup where runs have several rows
 constexpr unsigned kChunkBlocks = 4;       // blocks of a chunk, one per lane group
 constexpr unsigned kChunkTokens = kChunkBlocks * kKv8Block;
-constexpr int kNone = -(1 << 30);          // a reference that no score has set
+constexpr float kNone = -0x1.fffffep127f;  // a reference that no score has set: below all others
+constexpr int kNone2 = -(1 << 29);         // the same of M2
 constexpr int kPBits = 15;                 // p' < 2^15 in f16: the largest p' keeps 2^-38 of itself
 constexpr unsigned kStat = 4;              // floats before a partial's D sums
 
@@ -184,9 +187,29 @@ __device__ __forceinline__ void load_keys(const Kv8Byte* rec, unsigned lane, Key
 // a scale of zero, whose codes are zero): the smallest normal number stands
 // for it, which keeps masked scores at -inf where zero would make them NaN.
 // A NaN scale passes.
+constexpr float kLeastFactor = 0x1p-126f;
 __device__ __forceinline__ float score_factor(float unit, float k_scale) {
     const float f = unit * k_scale;
-    return f < 0x1p-126f ? 0x1p-126f : f;
+    return f < kLeastFactor ? kLeastFactor : f;
+}
+
+// Scores that may pass 2^23 are multiplied by their factor first, rounded to
+// f32, whose neighbours are one and more apart there: only so is the largest of
+// them its own reference, and its 2^(s - M) 1.  Below, the product is exact
+// until M is taken off it.  Every kernel decides by the factor alone, so all of
+// them take the same scores.  Returns whether a lane's block was one.
+template <int TYPE, unsigned D>
+__device__ __forceinline__ bool round_large(float4v (&s)[4], float& factor) {
+    constexpr float kLargest = static_cast<float>(D) * (TYPE == kKv8I8 ? 127.0f : 448.0f) * 0x1p11f;
+    const bool large = factor >= 0x1p23f / kLargest;
+    if (__builtin_expect(!__any(large), 1)) return false;
+#pragma unroll
+    for (unsigned b = 0; b < 4u; ++b) {
+#pragma unroll
+        for (unsigned r = 0; r < 4u; ++r) s[b][r] = large ? s[b][r] * factor : s[b][r];
+    }
+    factor = large ? 1.0f : factor;
+    return true;
 }
 // 2^(score * factor - base), one rounding
 __device__ __forceinline__ float score_power(float score, float factor, float base) {
@@ -227,22 +250,32 @@ __device__ __forceinline__ void chunk_scores(const KeyCodes<D>& k, const QueryFr
 }
 
 // max over the four lane groups of a vector, in every lane of it.
-__device__ __forceinline__ int groups_max(int x) {
-    const auto h = __builtin_amdgcn_permlane32_swap(x, x, false, false);
-    const int a = static_cast<int>(h[0]), b = static_cast<int>(h[1]);
-    const int m = a > b ? a : b;
-    const auto q = __builtin_amdgcn_permlane16_swap(m, m, false, false);
-    const int c = static_cast<int>(q[0]), d = static_cast<int>(q[1]);
+template <typename T>
+__device__ __forceinline__ T groups_max(T x) {
+    const auto swapped = [](const auto& pair, unsigned i) { return __builtin_bit_cast(T, static_cast<std::uint32_t>(pair[i])); };
+    const std::uint32_t bits = __builtin_bit_cast(std::uint32_t, x);
+    const auto h = __builtin_amdgcn_permlane32_swap(bits, bits, false, false);
+    const T a = swapped(h, 0u), b = swapped(h, 1u), m = a > b ? a : b;
+    const std::uint32_t half = __builtin_bit_cast(std::uint32_t, m);
+    const auto q = __builtin_amdgcn_permlane16_swap(half, half, false, false);
+    const T c = swapped(q, 0u), d = swapped(q, 1u);
     return c > d ? c : d;
+}
+
+// The difference of two references as an exponent: what is past 2^28 either
+// way leaves nothing of an f32, and sums of a few such stay in 32 bits.
+__device__ __forceinline__ int powers(float difference) {
+    return static_cast<int>(__builtin_amdgcn_fmed3f(difference, -0x1p28f, 0x1p28f));
 }
 
 // The scores of a chunk into p' = hi + lo, the B operands of the products
 // with V, and into the denominator.  `ahead`: how far this lane's vector lies
 // behind the block's first token (it sees tokens 0..ahead); `here`: the block
-// has a page; scale: of K and V.
-template <unsigned D>
-__device__ __forceinline__ void soften(float4v (&s)[4], float unit, float2 scale, bool here, int ahead, int& ref, int& ref2,
-                                       float& l, float4v (&o)[D / 16], half8v (&p_hi)[2], half8v (&p_lo)[2]) {
+// has a page; scale: of K and V; `far`: whether a chunk of the wave's had
+// scores that may pass 2^23.
+template <int TYPE, unsigned D>
+__device__ __forceinline__ void soften(float4v (&s)[4], float unit, float2 scale, bool here, int ahead, float& ref, int& ref2,
+                                       bool& far, float& l, float4v (&o)[D / 16], half8v (&p_hi)[2], half8v (&p_lo)[2]) {
     float factor = score_factor(unit, scale.x);
     float v_scale = scale.y;
     const int exponent = __builtin_amdgcn_frexp_expf(v_scale);   // scale of V < 2^exponent
@@ -250,7 +283,7 @@ __device__ __forceinline__ void soften(float4v (&s)[4], float unit, float2 scale
         // What a vector does not see scores -inf; a block that it sees
         // nothing of has no scales either (they may be NaN).
         const int limit = here ? ahead : -1;
-        factor = limit < 0 ? 1.0f : factor;
+        factor = limit < 0 ? kLeastFactor : factor;
         v_scale = limit < 0 ? 0.0f : v_scale;
 #pragma unroll
         for (unsigned b = 0; b < 4u; ++b) {
@@ -260,6 +293,7 @@ __device__ __forceinline__ void soften(float4v (&s)[4], float unit, float2 scale
             }
         }
     }
+    far |= round_large<TYPE, D>(s, factor);
     float top = s[0][0];
 #pragma unroll
     for (unsigned b = 0; b < 4u; ++b) {
@@ -268,18 +302,30 @@ __device__ __forceinline__ void soften(float4v (&s)[4], float unit, float2 scale
     }
     // The block's own references; the vector's only move when one of its
     // blocks passes them.
-    const float bound = fminf(ceilf(top * factor), 0x1p28f);
-    const int block_m = bound < -0x1p28f ? kNone : static_cast<int>(bound);   // differences stay in 32 bits
-    const int block_m2 = block_m == kNone || v_scale == 0.0f ? kNone : block_m + exponent;
+    const float block_m = ceilf(top * factor);
+    const int held_m = powers(ref);
+    int block_m2 = powers(far ? block_m - ref : block_m) + exponent;
+    if (__builtin_expect(far, 0)) block_m2 += held_m;
+    block_m2 = v_scale == 0.0f ? kNone2 : block_m2;
     if (__any(block_m > ref || block_m2 > ref2)) {
-        const int next = groups_max(block_m > ref ? block_m : ref);
-        const int next2 = groups_max(block_m2 > ref2 ? block_m2 : ref2);
-        l = __builtin_amdgcn_ldexpf(l, ref - next);
-        const int down = ref2 - next2;
+        const float next = groups_max(block_m > ref ? block_m : ref);
+        const int down = powers(ref - next);
+        int next2, down2;
+        if (__builtin_expect(far, 0)) {            // by way of the leads, whatever M is
+            const int held = ref2 - held_m + down > kNone2 ? ref2 - held_m + down : kNone2;
+            const int mine = v_scale == 0.0f ? kNone2 : powers(block_m - next) + exponent;
+            const int lead = groups_max(mine > held ? mine : held);
+            down2 = held - lead;
+            next2 = powers(next) + lead;
+        } else {
+            next2 = groups_max(block_m2 > ref2 ? block_m2 : ref2);
+            down2 = ref2 - next2;
+        }
+        l = __builtin_amdgcn_ldexpf(l, down);
 #pragma unroll
         for (unsigned t = 0; t < D / 16u; ++t) {
 #pragma unroll
-            for (unsigned r = 0; r < 4u; ++r) o[t][r] = __builtin_amdgcn_ldexpf(o[t][r], down);
+            for (unsigned r = 0; r < 4u; ++r) o[t][r] = __builtin_amdgcn_ldexpf(o[t][r], down2);
         }
         ref = next;
         ref2 = next2;
@@ -287,18 +333,27 @@ __device__ __forceinline__ void soften(float4v (&s)[4], float unit, float2 scale
     // p' = 2^(s - base) * share, below 2^kPBits; a scale of V far below the
     // others' (or zero) keeps base near M, so the same powers also sum up the
     // denominator.  s - base is small where p is large, and rounded once.
-    int e = ref2 - ref - 40;
+    const int lead = ref2 - powers(ref);
+    int e = lead - 40;
     e = v_scale == 0.0f || exponent < e ? e : exponent;
-    const int base = ref2 - e;
-    const float share = __builtin_amdgcn_ldexpf(v_scale, kPBits - e);
-    const float fbase = static_cast<float>(base);
+    int over = lead - e, up = kPBits - e;          // base - M, and the exponent of share / (scale of V)
+    const float base = ref + static_cast<float>(over);
+    if (__builtin_expect(far, 0)) {
+        // Past 2^24 the sum was rounded, so the exponents follow from what it
+        // became; p' is as large as before, so where share would overflow the
+        // power is zero.
+        over = powers(base - ref);
+        up = kPBits - lead + over;
+        up = up < 100 - exponent ? up : 100 - exponent;
+    }
+    const float share = __builtin_amdgcn_ldexpf(v_scale, up);
     float sum = 0.0f;
 #pragma unroll
     for (unsigned b = 0; b < 4u; ++b) {
 #pragma unroll
         for (unsigned r = 0; r < 4u; r += 2u) {
-            const float x0 = score_power(s[b][r], factor, fbase);
-            const float x1 = score_power(s[b][r + 1u], factor, fbase);
+            const float x0 = score_power(s[b][r], factor, base);
+            const float x1 = score_power(s[b][r + 1u], factor, base);
             sum += x0;
             sum += x1;
             half2v hi, lo;
@@ -309,7 +364,7 @@ __device__ __forceinline__ void soften(float4v (&s)[4], float unit, float2 scale
             p_lo[b >> 1][4u * (b & 1u) + r + 1u] = lo[1];
         }
     }
-    l += __builtin_amdgcn_ldexpf(sum, base - ref);
+    l += __builtin_amdgcn_ldexpf(sum, over);
 }
 
 // The rows of a tile: with RUNS up to tile_rows rows of one run (as many whole
@@ -416,8 +471,8 @@ __global__ __launch_bounds__(64 * W, NV == 1u && W == kWaves ? 3 : 2) void kv8_a
     };
     __shared__ Shared sh;
     __shared__ float undo_of[kTile];
-    __shared__ int wave_m[W][kTile], wave_m2[W][kTile];
-    __shared__ float wave_l[W][kTile];
+    __shared__ float wave_m[W][kTile], wave_l[W][kTile];
+    __shared__ int wave_power[W][kTile], wave_m2[W][kTile];
     const unsigned tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, grp = lane >> 4, col = lane & 15u;
     const std::uint32_t group = q_heads / g.kv_heads, parts = (group + kTile - 1u) / kTile;
     const Kv8Work work = kv8_work(cut, blockIdx.x, g.kv_heads * parts);
@@ -484,12 +539,14 @@ __global__ __launch_bounds__(64 * W, NV == 1u && W == kWaves ? 3 : 2) void kv8_a
         for (unsigned n = 0; n < NV; ++n) undo[n] = undo_of[n * kVectors + col];
     }
 
-    int ref[NV], ref2[NV];                         // M and M2
-    float l[NV];
+    float ref[NV], l[NV];                          // M and the denominator
+    int ref2[NV];                                  // M2, as powers(M) and its lead
+    bool far = false;
     float4v o[NV][D / 16];
 #pragma unroll
     for (unsigned n = 0; n < NV; ++n) {
-        ref[n] = ref2[n] = kNone;
+        ref[n] = kNone;
+        ref2[n] = kNone2;
         l[n] = 0.0f;
 #pragma unroll
         for (unsigned t = 0; t < D / 16u; ++t) o[n][t] = float4v{0.f, 0.f, 0.f, 0.f};
@@ -545,7 +602,8 @@ __global__ __launch_bounds__(64 * W, NV == 1u && W == kWaves ? 3 : 2) void kv8_a
         half8v p_hi[NV][2], p_lo[NV][2];
 #pragma unroll
         for (unsigned n = 0; n < NV; ++n) {
-            soften<D>(s[n], undo[n] * score_scale, now, here, pos[n] - first, ref[n], ref2[n], l[n], o[n], p_hi[n], p_lo[n]);
+            soften<TYPE, D>(s[n], undo[n] * score_scale, now, here, pos[n] - first, ref[n], ref2[n], far, l[n], o[n], p_hi[n],
+                            p_lo[n]);
         }
         if constexpr (TYPE == kKv8E4M3) {
             // Slots behind the tile's last token may hold NaN codes, which a
@@ -578,7 +636,7 @@ __global__ __launch_bounds__(64 * W, NV == 1u && W == kWaves ? 3 : 2) void kv8_a
         }
     }
 
-    // The waves meet: sums in units of 2^(M2 - kPBits), l of 2^M.
+    // The waves meet: sums in units of 2^(M + lead - kPBits), l of 2^M.
     if constexpr (NV > 1u) __syncthreads();        // the query operands make room
 #pragma unroll
     for (unsigned n = 0; n < NV; ++n) {
@@ -587,6 +645,7 @@ __global__ __launch_bounds__(64 * W, NV == 1u && W == kWaves ? 3 : 2) void kv8_a
         l[n] += __shfl_xor(l[n], 32);
         if (grp == 0u) {
             wave_m[wave][v] = ref[n];
+            wave_power[wave][v] = powers(ref[n]);
             wave_m2[wave][v] = ref2[n];
             wave_l[wave][v] = l[n];
         }
@@ -596,20 +655,46 @@ __global__ __launch_bounds__(64 * W, NV == 1u && W == kWaves ? 3 : 2) void kv8_a
     __syncthreads();
     for (unsigned idx = tid; idx < nq * (D / 4u); idx += 64u * W) {
         const unsigned v = idx / (D / 4u), d4 = idx % (D / 4u);
-        int mm = kNone, mm2 = kNone;
+        float4v sums[W];
+        float denominators[W];
+        int power[W], m2[W], most_m = -(1 << 28), most_m2 = kNone2;
 #pragma unroll
         for (unsigned w = 0; w < W; ++w) {
-            mm = wave_m[w][v] > mm ? wave_m[w][v] : mm;
-            mm2 = wave_m2[w][v] > mm2 ? wave_m2[w][v] : mm2;
+            power[w] = wave_power[w][v];
+            m2[w] = wave_m2[w][v];
+            denominators[w] = wave_l[w][v];
+            sums[w] = *reinterpret_cast<const float4v*>(&sh.sums[w][v][4u * d4]);
+        }
+#pragma unroll
+        for (unsigned w = 0; w < W; ++w) {
+            most_m = power[w] > most_m ? power[w] : most_m;
+            most_m2 = m2[w] > most_m2 ? m2[w] : most_m2;
+        }
+        float mm = static_cast<float>(most_m);
+        int lead = most_m2 - most_m;
+        if (__builtin_expect(most_m <= -(1 << 27) || most_m == 1 << 28, 0)) {
+            // References too large for differences of their powers: the leads
+            // stay, and M goes by its own differences.
+            mm = kNone;
+            for (unsigned w = 0; w < W; ++w) mm = wave_m[w][v] > mm ? wave_m[w][v] : mm;
+            most_m = 0;
+            most_m2 = kNone2;
+#pragma unroll
+            for (unsigned w = 0; w < W; ++w) {
+                m2[w] -= power[w];
+                power[w] = powers(wave_m[w][v] - mm);
+                m2[w] += power[w];
+                most_m2 = m2[w] > most_m2 ? m2[w] : most_m2;
+            }
+            lead = most_m2;
         }
         float total = 0.0f;
         float4v acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (unsigned w = 0; w < W; ++w) {
-            total += __builtin_amdgcn_ldexpf(wave_l[w][v], wave_m[w][v] - mm);
-            const float4v a = *reinterpret_cast<const float4v*>(&sh.sums[w][v][4u * d4]);
+            total += __builtin_amdgcn_ldexpf(denominators[w], power[w] - most_m);
 #pragma unroll
-            for (unsigned r = 0; r < 4u; ++r) acc[r] += __builtin_amdgcn_ldexpf(a[r], wave_m2[w][v] - mm2);
+            for (unsigned r = 0; r < 4u; ++r) acc[r] += __builtin_amdgcn_ldexpf(sums[w][r], m2[w] - most_m2);
         }
         const std::uint64_t vector =
             static_cast<std::uint64_t>(tile.row + v / tile.heads) * q_heads + tile.head + v % tile.heads;
@@ -617,14 +702,14 @@ __global__ __launch_bounds__(64 * W, NV == 1u && W == kWaves ? 3 : 2) void kv8_a
             float4v y;
 #pragma unroll
             for (unsigned r = 0; r < 4u; ++r) {
-                y[r] = total == 0.0f ? 0.0f : __builtin_amdgcn_ldexpf(acc[r] / total, mm2 - kPBits - mm);
+                y[r] = total == 0.0f ? 0.0f : __builtin_amdgcn_ldexpf(acc[r] / total, lead - kPBits);
             }
             *reinterpret_cast<float4v*>(out + vector * D + 4u * d4) = y;
-            if (stats && d4 == 0u) stats[vector] = make_float2(static_cast<float>(mm), total == 0.0f ? 0.0f : 1.0f / total);
+            if (stats && d4 == 0u) stats[vector] = make_float2(mm, total == 0.0f ? 0.0f : 1.0f / total);
         } else {
             const std::uint64_t place = RUNS ? static_cast<std::uint64_t>(work.pair - cut.whole) * kTile + v : vector;
             float* const p = partials + (place * cut.splits + split) * (D + kStat);
-            if (d4 == 0u) *reinterpret_cast<float4v*>(p) = float4v{__int_as_float(mm), __int_as_float(mm2), total, 0.0f};
+            if (d4 == 0u) *reinterpret_cast<float4v*>(p) = float4v{mm, __int_as_float(lead), total, 0.0f};
             *reinterpret_cast<float4v*>(p + kStat + 4u * d4) = acc;
         }
     }
@@ -641,20 +726,24 @@ __device__ __forceinline__ std::uint32_t live_splits(int reach, std::uint64_t ma
 // Dims 4 d4 .. + 3 of a vector over splits of it: references, denominator and
 // sums so far.
 struct Joined {
-    int ref = kNone, ref2 = kNone;
+    float ref = kNone;
+    int lead = kNone2;
     float total = 0.0f;
     float4v acc = {0.f, 0.f, 0.f, 0.f};
 };
 
-__device__ __forceinline__ void join(Joined& x, int ref, int ref2, float total, const float4v& acc) {
-    const int next = ref > x.ref ? ref : x.ref, next2 = ref2 > x.ref2 ? ref2 : x.ref2;
-    x.total = __builtin_amdgcn_ldexpf(x.total, x.ref - next) + __builtin_amdgcn_ldexpf(total, ref - next);
+__device__ __forceinline__ void join(Joined& x, float ref, int lead, float total, const float4v& acc) {
+    const float next = ref > x.ref ? ref : x.ref;
+    const int mine_down = powers(x.ref - next), down = powers(ref - next);
+    const int mine = x.lead + mine_down > kNone2 ? x.lead + mine_down : kNone2, theirs = lead + down;
+    const int next_lead = theirs > mine ? theirs : mine;
+    x.total = __builtin_amdgcn_ldexpf(x.total, mine_down) + __builtin_amdgcn_ldexpf(total, down);
 #pragma unroll
     for (unsigned r = 0; r < 4u; ++r) {
-        x.acc[r] = __builtin_amdgcn_ldexpf(x.acc[r], x.ref2 - next2) + __builtin_amdgcn_ldexpf(acc[r], ref2 - next2);
+        x.acc[r] = __builtin_amdgcn_ldexpf(x.acc[r], mine - next_lead) + __builtin_amdgcn_ldexpf(acc[r], theirs - next_lead);
     }
     x.ref = next;
-    x.ref2 = next2;
+    x.lead = next_lead;
 }
 
 // Splits begin .. end - 1 of a vector's partials, eight loads in flight.
@@ -673,7 +762,7 @@ __device__ __forceinline__ Joined join_splits(const float* __restrict__ base, st
         }
 #pragma unroll
         for (unsigned j = 0; j < kBatch; ++j) {
-            if (s0 + j < end) join(x, __float_as_int(head[j][0]), __float_as_int(head[j][1]), head[j][2], sums[j]);
+            if (s0 + j < end) join(x, head[j][0], __float_as_int(head[j][1]), head[j][2], sums[j]);
         }
     }
     return x;
@@ -683,7 +772,7 @@ __device__ __forceinline__ float4v normalised(const Joined& x) {
     float4v y;
 #pragma unroll
     for (unsigned r = 0; r < 4u; ++r) {
-        y[r] = x.total == 0.0f ? 0.0f : __builtin_amdgcn_ldexpf(x.acc[r] / x.total, x.ref2 - kPBits - x.ref);
+        y[r] = x.total == 0.0f ? 0.0f : __builtin_amdgcn_ldexpf(x.acc[r] / x.total, x.lead - kPBits);
     }
     return y;
 }
@@ -727,23 +816,23 @@ __global__ __launch_bounds__(kThreads) void kv8_merge_kernel(
         Joined x = join_splits<D>(base, from, live - from < each ? live : from + each, d4);
         if constexpr (WIDE) {
             __shared__ float4v sums[kSlices][kPieces];
-            __shared__ int refs[kSlices], refs2[kSlices];
-            __shared__ float totals[kSlices];
+            __shared__ float refs[kSlices], totals[kSlices];
+            __shared__ int leads[kSlices];
             __syncthreads();   // the vector before is out
             sums[slice][d4] = x.acc;
             if (d4 == 0u) {
                 refs[slice] = x.ref;
-                refs2[slice] = x.ref2;
+                leads[slice] = x.lead;
                 totals[slice] = x.total;
             }
             __syncthreads();
             if (slice != 0u) continue;
 #pragma unroll
-            for (unsigned w = 1; w < kSlices; ++w) join(x, refs[w], refs2[w], totals[w], sums[w][d4]);
+            for (unsigned w = 1; w < kSlices; ++w) join(x, refs[w], leads[w], totals[w], sums[w][d4]);
         }
         *reinterpret_cast<float4v*>(out + vector * D + 4u * d4) = normalised(x);
         if (stats && d4 == 0u) {
-            stats[vector] = make_float2(static_cast<float>(x.ref), x.total == 0.0f ? 0.0f : 1.0f / x.total);
+            stats[vector] = make_float2(x.ref, x.total == 0.0f ? 0.0f : 1.0f / x.total);
         }
     }
 }
@@ -884,19 +973,17 @@ __global__ __launch_bounds__(kThreads, 3) void kv8_weights_kernel(
         const std::uint32_t live = MERGE ? live_splits(position, max_tokens, split_chunks) : 1u;
         if (MERGE && __any(live > 1u)) {
             // Lane group grp takes splits grp, grp + 4, ...; then they meet.
-            int ref = kNone;
-            float total = 0.0f;
+            float ref = kNone, total = 0.0f;
             for (std::uint32_t s = grp; s < live && live > 1u; s += 4u) {
                 const float4v head = *reinterpret_cast<const float4v*>(partials + (vector * splits + s) * (D + kStat));
-                const int a = __float_as_int(head[0]), next = a > ref ? a : ref;
-                total = __builtin_amdgcn_ldexpf(total, ref - next) + __builtin_amdgcn_ldexpf(head[2], a - next);
+                const float next = head[0] > ref ? head[0] : ref;
+                total = __builtin_amdgcn_ldexpf(total, powers(ref - next)) + __builtin_amdgcn_ldexpf(head[2], powers(head[0] - next));
                 ref = next;
             }
-            const int all = groups_max(ref);
-            total = __builtin_amdgcn_ldexpf(total, ref - all);
+            base = groups_max(ref);
+            total = __builtin_amdgcn_ldexpf(total, powers(ref - base));
             total += __shfl_xor(total, 16);
             total += __shfl_xor(total, 32);
-            base = static_cast<float>(all);
             share = total == 0.0f ? 0.0f : 1.0f / total;
             if (live <= 1u) {   // the attention kernel left this row's
                 const float2 st = stats[vector];
@@ -910,7 +997,8 @@ __global__ __launch_bounds__(kThreads, 3) void kv8_weights_kernel(
         }
         float4v s[4];
         chunk_scores<TYPE, D>(keys, q, s);
-        const float factor = score_factor(q.undo * score_scale, k_scale);
+        float factor = score_factor(q.undo * score_scale, k_scale);
+        round_large<TYPE, D>(s, factor);
         const int limit = vrec == nullptr ? -1 : upto - first;
 #pragma unroll
         for (unsigned t = 0; t < 16u; ++t) {
@@ -1002,7 +1090,8 @@ __global__ __launch_bounds__(kThreads, 2) void kv8_run_weights_kernel(
                                                                   s[b], 0, 0, 0);
                 }
             }
-            const float factor = score_factor(now.q.undo * score_scale, k_scale);
+            float factor = score_factor(now.q.undo * score_scale, k_scale);
+            round_large<TYPE, D>(s, factor);
             if (__all(limit >= 15)) {
 #pragma unroll
                 for (unsigned t = 0; t < 16u; ++t) {

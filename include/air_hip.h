@@ -679,7 +679,9 @@ int air_hip_kv8_read(air_hip_context* ctx, const air_hip_kv8_layout* kv, uint32_
 /* Attention of every row's q heads over slots 0..positions[r] of its sequence
  * (below max_tokens, which bounds the work and sizes the context's scratch):
  * out [m][q_heads * head_dim], f32 accurate over the stored values (both
- * products carry their f32 operand as two f16 parts, sums in f32).  Tokens
+ * products carry their f32 operand as two f16 parts, sums in f32): q to 2^-22
+ * of its vector's largest magnitude (or to 2^-133, if that is more), scores of
+ * any size that f32 holds; scores past f32's range are infinities.  Tokens
  * without a page take no part; a row that attends to nothing (a negative
  * position) gets zeros.
  *   run_starts  int32 [runs + 1], device, ascending: run i is rows

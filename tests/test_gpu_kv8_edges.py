@@ -87,3 +87,58 @@ def test_queries_up_to_f32s_largest(torch_cuda, hip_ctx, kind):
         for mode in (None, "set"):
             tab = np.repeat(tables[:1], m, axis=0) if runs else tables
             attend(dev, x, [n - 1 - r for r in range(m)], tab, q_heads, n, runs, mode)
+
+
+@pytest.mark.gpu
+@KINDS
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("size", [2e6, 3e7, 1e8, 4e8, 1e12, 1e30], ids=lambda s: f"{s:.0e}")
+def test_scores_far_past_f32s_whole_numbers(torch_cuda, hip_ctx, kind, d, size):
+    """Scores of +-1, 1/2 and 1/4 times `size`.  Tokens of one such score have
+    the same codes under the same scale, so whatever a kernel makes of them is
+    equal, and the others lie so far below that their part is zero: the tokens
+    of the largest score share the weight equally, to the accuracy of p and the
+    sums (2^-21 and 6 sqrt(tokens) 2^-24, as the model derives them for scores
+    without an error).  Rows of ordinary q between them; cut and uncut keys, a
+    run's tiles, weights by every kernel."""
+    rng = np.random.default_rng(d + kind + int(math.log10(size)))
+    q_heads, kvh, n = 14, 2, 1300
+    cache, tables = filled(kind, kvh, d, [n, n, 100], rng)
+    sign = np.where(rng.random((kvh, d)) < 0.5, -1.0, 1.0).astype(np.float32)
+    part = rng.choice([1.0, 0.5, 0.25], n).astype(np.float32)
+    part[::16] = 1.0                                  # every block's scale is that of 1
+    part[rng.integers(1, 16)] = 0.25
+    x = np.concatenate([(part[:, None, None] * sign).reshape(n, -1),
+                        rng.standard_normal((n, kvh * d)).astype(np.float32)], axis=1)
+    for i, b in enumerate((n, n, 100)):
+        cache.append(x[:b], 0, list(range(b)), np.repeat(tables[i:i + 1], b, axis=0), 0)
+    dev = Device(torch_cuda, hip_ctx, cache)
+    exact = {"on": False}
+    usual = cache.rounding
+
+    def rounding(q, k, tokens):
+        ds, rel = usual(q, k, tokens)
+        s = np.sort(k @ q / math.sqrt(d))
+        if s[-1] - s[0] < 1e5:
+            return ds, rel
+        exact["on"] = True
+        gaps = np.diff(s)
+        assert ((gaps == 0) | (gaps > 100 + 2 * ds)).all()
+        return 0.0, 2.0 ** -21 + 6 * math.sqrt(tokens) * 2.0 ** -24
+    cache.rounding = rounding
+
+    def query(m):
+        q = rng.standard_normal((m, kvh, q_heads // kvh, d)).astype(np.float32)
+        # Eight bits, so that float64 sums the 128 products without a rounding.
+        a = rng.integers(180, 256, q.shape[:3]) * 2.0 ** (math.floor(math.log2(size / math.sqrt(d))) - 8)
+        a *= np.where(rng.random(q.shape[:3]) < 0.5, -1, 1)
+        far = rng.random(q.shape[:3]) < 0.8
+        far[0] = True
+        q[far] = (a[..., None] * sign[None, :, None, :]).astype(np.float32)[far]
+        return q.reshape(m, -1)
+    for mode in (None, "set"):
+        attend(dev, query(3), [90, -1, 33], tables, q_heads, 100, None, mode)       # one launch
+        attend(dev, query(2), [n - 1, 740], tables[:2], q_heads, n, None, mode)     # cut, joined
+        attend(dev, query(24), [n - 3 - 200 * (r % 4) for r in range(24)], np.repeat(tables[:1], 24, axis=0), q_heads, n,
+               [(0, 24)], mode)
+    assert exact["on"]
