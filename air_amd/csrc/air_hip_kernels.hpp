@@ -436,10 +436,11 @@ struct Kv8Shape {
 };
 Kv8Shape kv8_attention_shape(std::uint32_t m, std::uint32_t q_heads, std::uint32_t kv_heads, std::uint32_t head_dim,
                              std::uint32_t runs, std::uint64_t max_tokens, bool weights);
-// Bytes of scratch: the splits' partials and, with weights, the rows' softmax
-// statistics and for run_weights their vectors' operands.
-std::uint64_t kv8_attention_scratch(const Kv8Shape& shape, std::uint32_t m, std::uint32_t q_heads,
-                                    std::uint32_t head_dim, bool weights);
+// Bytes of scratch that suffice: for the splits' partials and, with weights, the
+// rows' softmax statistics and of runs their vectors' operands.  They grow with
+// m, runs, max_tokens and weights.
+std::uint64_t kv8_attention_scratch(std::uint32_t m, std::uint32_t q_heads, std::uint32_t kv_heads, std::uint32_t head_dim,
+                                    std::uint32_t runs, std::uint64_t max_tokens, bool weights);
 // weights: 0 none, 1 add, 2 set.  run_starts may be null (every row its own run).
 hipError_t launch_kv8_attention(const Kv8Geometry& g, const float* qkv, std::uint64_t stride, std::uint32_t m,
                                 const std::int32_t* positions, const std::int32_t* tables, std::uint32_t layer,

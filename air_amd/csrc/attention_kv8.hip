@@ -1210,27 +1210,53 @@ struct Scratch {
     std::uint64_t queries, undos, partials, bytes;
 };
 
-Scratch scratch_of(const Kv8Shape& shape, std::uint32_t m, std::uint32_t q_heads, std::uint32_t head_dim, bool weights) {
-    const std::uint64_t vectors = static_cast<std::uint64_t>(m) * q_heads;
+// places: vectors' splits.
+Scratch scratch_parts(std::uint64_t vectors, std::uint32_t head_dim, bool weights, bool keep, std::uint64_t places) {
     const auto padded = [](std::uint64_t bytes) { return (bytes + 255u) / 256u * 256u; };
     Scratch s{};
     s.queries = weights ? padded(vectors * sizeof(float2)) : 0u;
-    const bool keep = shape.run_weights;
     s.undos = s.queries + (keep ? vectors * head_dim * 2u * sizeof(_Float16) : 0u);
     s.partials = s.undos + (keep ? padded(vectors * sizeof(float)) : 0u);
-    // Of runs the tiles that are cut have a place a vector, of rows all vectors.
-    const std::uint64_t places = shape.kernel == kKv8Runs
-                                     ? static_cast<std::uint64_t>(shape.cut.pairs - shape.cut.whole) * kVectors * kRunTiles
-                                     : vectors;
-    s.bytes = s.partials + (shape.cut.splits > 1u ? places * shape.cut.splits * (head_dim + kStat) * sizeof(float) : 0u);
+    s.bytes = s.partials + places * (head_dim + kStat) * sizeof(float);
     return s;
+}
+
+Scratch scratch_of(const Kv8Shape& shape, std::uint32_t m, std::uint32_t q_heads, std::uint32_t head_dim, bool weights) {
+    const std::uint64_t vectors = static_cast<std::uint64_t>(m) * q_heads;
+    // Of runs the tiles that are cut have a place a vector, of rows all vectors.
+    const std::uint64_t cut = shape.kernel == kKv8Runs
+                                  ? static_cast<std::uint64_t>(shape.cut.pairs - shape.cut.whole) * kVectors * kRunTiles
+                                  : vectors;
+    return scratch_parts(vectors, head_dim, weights, shape.run_weights, shape.cut.splits > 1u ? cut * shape.cut.splits : 0u);
 }
 
 } // namespace
 
-std::uint64_t kv8_attention_scratch(const Kv8Shape& shape, std::uint32_t m, std::uint32_t q_heads,
-                                    std::uint32_t head_dim, bool weights) {
-    return scratch_of(shape, m, q_heads, head_dim, weights).bytes;
+// What a call asks for is not what its shape takes, which falls where more rows
+// need fewer splits, but a bound that grows with m, runs, max_tokens and
+// weights: a call with the largest of each leaves room for all others, so that
+// none of them allocates while it is captured.
+//
+// Splits of single rows hold at least kWaves chunks, and there is more than one
+// only of less pairs than slots, when pairs * splits < slots + pairs.  Tiles are
+// cut from 4 kWaves chunks on, less of them than slots, into splits of at least
+// 2 kWaves chunks; run_pairs is at least half of pairs, so with the rounding
+// of `left` tiles * splits is at most 3 slots.
+std::uint64_t kv8_attention_scratch(std::uint32_t m, std::uint32_t q_heads, std::uint32_t kv_heads, std::uint32_t head_dim,
+                                    std::uint32_t runs, std::uint64_t max_tokens, bool weights) {
+    const auto least = [](std::uint64_t a, std::uint64_t b) { return a < b ? a : b; };
+    const std::uint64_t chunks = (max_tokens + kChunkTokens - 1u) / kChunkTokens, group = q_heads / kv_heads;
+    const std::uint64_t row_parts = (group + kVectors - 1u) / kVectors, row_slots = head_dim == 128u ? 768u : 1024u;
+    const std::uint64_t row_splits = least(m * kv_heads * row_parts * ((chunks + kWaves - 1u) / kWaves), 2u * row_slots);
+    std::uint64_t places = chunks > kWaves ? row_splits * ((group + row_parts - 1u) / row_parts) : 0u;
+    if (runs != 0u && chunks >= 4u * kWaves) {
+        const std::uint64_t tile = kVectors * kRunTiles, parts = (group + tile - 1u) / tile;
+        const std::uint64_t tiles = (m / (group < tile ? tile / group : 1u) + runs) * kv_heads * parts;
+        const std::uint64_t slots = head_dim == 128u ? 512u : 768u;
+        const std::uint64_t splits = least(least(tiles, slots) * ((chunks + 2u * kWaves - 1u) / (2u * kWaves)), 3u * slots);
+        places = places > splits * tile ? places : splits * tile;
+    }
+    return scratch_parts(static_cast<std::uint64_t>(m) * q_heads, head_dim, weights, weights && runs != 0u, places).bytes;
 }
 
 namespace {

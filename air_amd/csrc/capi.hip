@@ -2377,7 +2377,8 @@ int air_hip_kv8_attention(air_hip_context* ctx, const air_hip_kv8_layout* kv, co
     DeviceScope scope(ctx->device);
     if (scope.status() != hipSuccess) return hip_fail(scope.status(), "hipSetDevice");
     const Kv8Shape shape = kv8_attention_shape(m, q_heads, kv->kv_heads, kv->head_dim, runs, max_tokens, weights != 0);
-    if (int rc = ensure_attention_scratch(ctx, kv8_attention_scratch(shape, m, q_heads, kv->head_dim, weights != 0));
+    if (int rc = ensure_attention_scratch(ctx, kv8_attention_scratch(m, q_heads, kv->kv_heads, kv->head_dim, runs, max_tokens,
+                                                                     weights != 0));
         rc != AIR_HIP_OK) {
         return rc;
     }

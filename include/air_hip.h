@@ -696,7 +696,10 @@ int air_hip_kv8_read(air_hip_context* ctx, const air_hip_kv8_layout* kv, uint32_
  *               the weight of every slot 0..the run's last position; _SET
  *               stores that sum.  Deterministic where no page belongs to two
  *               runs of the call.
- * q|k|v rows and out 16-byte aligned, row_stride a multiple of 4. */
+ * q|k|v rows and out 16-byte aligned, row_stride a multiple of 4.  The scratch
+ * (26 MB at most beside what the rows' statistics and operands take) grows with
+ * m, runs, max_tokens and whether weights are gathered: after a call with the
+ * largest of each, other calls over the same heads allocate nothing. */
 enum {
     AIR_HIP_KV8_WEIGHTS_NONE = 0,
     AIR_HIP_KV8_WEIGHTS_ADD = 1,

@@ -142,3 +142,53 @@ def test_scores_far_past_f32s_whole_numbers(torch_cuda, hip_ctx, kind, d, size):
         attend(dev, query(24), [n - 3 - 200 * (r % 4) for r in range(24)], np.repeat(tables[:1], 24, axis=0), q_heads, n,
                [(0, 24)], mode)
     assert exact["on"]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("q_heads,kvh,d", [(28, 4, 128), (14, 2, 64), (40, 1, 64), (8, 8, 128)])
+def test_the_largest_call_sizes_the_scratch(torch_cuda, q_heads, kvh, d):
+    """After a call of the most rows, runs and tokens with weights, no call of
+    fewer grows the scratch: a capture of any of them allocates nothing."""
+    torch = torch_cuda
+    rng = np.random.default_rng(q_heads + d)
+    page_tokens, m, top = 1024, 300, 131072
+    stream = torch.cuda.Stream()
+    with capi.Context(0, stream.cuda_stream) as ctx, torch.cuda.stream(stream):
+        pool = torch.zeros(16, device="cuda:0")
+        kv = capi.Kv8Layout(pool.data_ptr(), page_tokens, kvh, d, 1, top // page_tokens, 1, None, 0, I8)
+        x = torch.zeros((m, q_heads * d), device="cuda:0")
+        out = torch.empty_like(x)
+        gone = torch.full((m,), -1, dtype=torch.int32, device="cuda:0")
+        tables = torch.full((m, top // page_tokens), -1, dtype=torch.int32, device="cuda:0")
+
+        def call(rows_, runs, tokens, mode):
+            starts = None
+            if runs:
+                cuts = np.sort(rng.integers(0, rows_ + 1, runs - 1))
+                starts = torch.tensor([0, *cuts.tolist(), rows_], dtype=torch.int32, device="cuda:0")
+            capi.check(capi.lib().air_hip_kv8_attention(
+                ctx.handle, ctypes.byref(kv), x.data_ptr(), q_heads * d, rows_, gone.data_ptr(), tables.data_ptr(), 0,
+                q_heads, starts.data_ptr() if runs else None, runs, tokens, mode, out.data_ptr()))
+            torch.cuda.synchronize()
+        call(m, m, top, capi.KV8_WEIGHTS_ADD)
+        before = ctx.stats()["workspace_generation"]
+        sizes = [(64, 0, 4000), (48, 0, 4000), (32, 0, 4000), (16, 0, 4000), (1, 0, top), (2, 1, top), (m, 1, top),
+                 (m, 2, 4000), (60, 2, 320), (33, 33, 70000)]
+        for _ in range(150):
+            rows_ = int(math.exp(rng.uniform(0, math.log(m + 0.99))))
+            runs = int(rng.integers(0, 3)) * int(math.exp(rng.uniform(0, math.log(rows_ + 0.99))))
+            sizes.append((rows_, min(runs, m), int(math.exp(rng.uniform(0, math.log(top))))))
+        for rows_, runs, tokens in sizes:
+            for mode in (capi.KV8_WEIGHTS_NONE, capi.KV8_WEIGHTS_SET):
+                call(rows_, runs, tokens, mode)
+                assert ctx.stats()["workspace_generation"] == before, (rows_, runs, tokens, mode)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=stream):
+            capi.check(capi.lib().air_hip_kv8_attention(
+                ctx.handle, ctypes.byref(kv), x.data_ptr(), q_heads * d, 16, gone.data_ptr(), tables.data_ptr(), 0,
+                q_heads, None, 0, 4000, capi.KV8_WEIGHTS_SET, out.data_ptr()))
+        out.fill_(1.0)
+        g.replay()
+        torch.cuda.synchronize()
+        assert not out[:16].any() and (out[16:] == 1.0).all()
+    torch.cuda.synchronize()
