@@ -192,3 +192,79 @@ def test_the_largest_call_sizes_the_scratch(torch_cuda, q_heads, kvh, d):
         torch.cuda.synchronize()
         assert not out[:16].any() and (out[16:] == 1.0).all()
     torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("q_heads,kvh,d", [(14, 2, 64), (28, 4, 128)])
+def test_captured_calls_that_cut_their_keys(torch_cuda, q_heads, kvh, d):
+    """Calls whose keys are cut, each in a graph of its own on one context:
+    rows joined in a launch of their own, by a workgroup a vector, and in that
+    of the weights; a prompt's tiles with their weights.  Every replay equals
+    the eager calls on a copy of the cache, also after an eager call that needed
+    a larger scratch, so that the graphs use the one they were captured with."""
+    torch = torch_cuda
+    rng = np.random.default_rng(151 + d)
+    lengths = [5000, 40, 900]
+    cache, tables = filled(E4M3, kvh, d, lengths, rng, max_pages=600)
+    stream = torch.cuda.Stream()
+    with capi.Context(0, stream.cuda_stream) as ctx, torch.cuda.stream(stream):
+        dev, ref = Device(torch, ctx, cache), Device(torch, ctx, cache)
+        m = 40
+        x = dev.up(rows(rng, m, q_heads, kvh, d))
+        pos = dev.up([n - 1 for n in lengths], np.int32)
+        tab = dev.up(tables, np.int32)
+        run_pos = dev.up([4900 + r for r in range(20)] + [850 + r for r in range(20)], np.int32)
+        run_tab = dev.up(np.repeat(tables[[0, 2]], 20, axis=0), np.int32)
+        starts = dev.up([0, 20, 40], np.int32)
+        out = [torch.zeros((m, q_heads * d), device="cuda:0") for _ in range(2)]
+
+        def rows_call(side, y, bound, mode):
+            capi.check(side.lib.air_hip_kv8_attention(
+                ctx.handle, ctypes.byref(side.kv), x.data_ptr(), x.shape[1], 3, pos.data_ptr(), tab.data_ptr(), 0,
+                q_heads, None, 0, bound, mode, y.data_ptr()))
+
+        def runs_call(side, y, bound, mode):
+            capi.check(side.lib.air_hip_kv8_attention(
+                ctx.handle, ctypes.byref(side.kv), x.data_ptr(), x.shape[1], m, run_pos.data_ptr(), run_tab.data_ptr(),
+                0, q_heads, starts.data_ptr(), 2, bound, mode, y.data_ptr()))
+        kinds = [(rows_call, 1500, capi.KV8_WEIGHTS_NONE), (rows_call, 1500, capi.KV8_WEIGHTS_ADD),
+                 (rows_call, 9600, capi.KV8_WEIGHTS_NONE), (rows_call, 9600, capi.KV8_WEIGHTS_ADD),
+                 (runs_call, 5000, capi.KV8_WEIGHTS_SET), (runs_call, 5000, capi.KV8_WEIGHTS_ADD)]
+        for call, bound, mode in kinds:
+            for side in (dev, ref):
+                call(side, out[0], bound, mode)       # sizes the scratch
+        torch.cuda.synchronize()
+        before = ctx.stats()["workspace_generation"]
+        graphs = []
+        for call, bound, mode in kinds:
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=stream):
+                call(dev, out[0], bound, mode)
+            graphs.append(g)
+        assert ctx.stats()["workspace_generation"] == before
+
+        def grow():
+            many = 1000
+            wide = torch.zeros((many, q_heads * d), device="cuda:0")
+            gone = torch.full((many,), -1, dtype=torch.int32, device="cuda:0")
+            none = torch.full((many, cache.max_pages), -1, dtype=torch.int32, device="cuda:0")
+            ends = dev.up([0, many], np.int32)
+            capi.check(dev.lib.air_hip_kv8_attention(
+                ctx.handle, ctypes.byref(dev.kv), wide.data_ptr(), q_heads * d, many, gone.data_ptr(), none.data_ptr(),
+                0, q_heads, ends.data_ptr(), 1, 5000, capi.KV8_WEIGHTS_ADD, wide.data_ptr()))
+            torch.cuda.synchronize()
+            assert ctx.stats()["workspace_generation"] > before
+        for turn in range(3):
+            if turn == 1:
+                grow()
+            for g, (call, bound, mode) in zip(graphs, kinds):
+                x.copy_(dev.up(rows(rng, m, q_heads, kvh, d)))
+                for y in out:
+                    y.zero_()
+                torch.cuda.synchronize()
+                g.replay()
+                call(ref, out[1], bound, mode)
+                torch.cuda.synchronize()
+                assert out[0].any() and torch.equal(out[0], out[1]), (turn, call.__name__, bound, mode)
+                assert same(dev.pool(), ref.pool()), (turn, call.__name__, bound, mode)
+    torch.cuda.synchronize()
