@@ -268,3 +268,29 @@ def test_captured_calls_that_cut_their_keys(torch_cuda, q_heads, kvh, d):
                 assert out[0].any() and torch.equal(out[0], out[1]), (turn, call.__name__, bound, mode)
                 assert same(dev.pool(), ref.pool()), (turn, call.__name__, bound, mode)
     torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+@KINDS
+@pytest.mark.parametrize("kvh,d,page_tokens", [(4, 128, 16), (3, 64, 32)])
+def test_read_of_the_weights_alone(torch_cuda, hip_ctx, kind, kvh, d, page_tokens):
+    """No k and no v asked for: from the start and from inside a block, past
+    max_tokens, without a page, of no tokens; the rest of the buffer stays."""
+    torch = torch_cuda
+    rng = np.random.default_rng(17 + kind)
+    lengths = [150, 1, 77, 33]
+    cache = Cache(kind, kvh, d, 3, page_tokens, 40, 12, seed=3)
+    tables = page_tables(rng, lengths, page_tokens, 12, 40)
+    tables[2, 1] = -1
+    dev = Device(torch, hip_ctx, cache)
+    for starts, counts, layer, layers, top in ((None, lengths, 1, 2, 150), ([5, 0, 30, 33], [90, 1, 40, 0], 0, 3, 64),
+                                               ([-1, 0, 16, 31], [9, 0, 48, 2], 2, 1, 48)):
+        w = torch.full((layers, 4, top, kvh), 7.0, device="cuda:0")
+        s = dev.up(starts, np.int32) if starts else None
+        n, t = dev.up(counts, np.int32), dev.up(tables, np.int32)
+        capi.check(dev.lib.air_hip_kv8_read(hip_ctx.handle, ctypes.byref(dev.kv), 4, s.data_ptr() if starts else None,
+                                            n.data_ptr(), t.data_ptr(), layer, layers, top, None, None, w.data_ptr()))
+        torch.cuda.synchronize()
+        counts = [0 if starts and a < 0 else c for a, c in zip(starts or lengths, counts)]
+        want = cache.read(starts, counts, tables, layer, layers, top, 7.0)[2]
+        assert np.array_equal(w.cpu().numpy(), want)
