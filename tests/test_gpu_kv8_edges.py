@@ -294,3 +294,40 @@ def test_read_of_the_weights_alone(torch_cuda, hip_ctx, kind, kvh, d, page_token
         counts = [0 if starts and a < 0 else c for a, c in zip(starts or lengths, counts)]
         want = cache.read(starts, counts, tables, layer, layers, top, 7.0)[2]
         assert np.array_equal(w.cpu().numpy(), want)
+
+
+@pytest.mark.gpu
+@KINDS
+@pytest.mark.parametrize("kvh,d", [(4, 128), (2, 64)])
+def test_append_and_read_of_unaligned_rows(torch_cuda, hip_ctx, kind, kvh, d):
+    """Rows that begin 4 bytes past an alignment, of odd strides, with k behind
+    a q of odd width; values read to such buffers."""
+    torch = torch_cuda
+    rng = np.random.default_rng(27 + kind)
+    n, width = 53, 2 * kvh * d
+    for offset, pad, q_width in ((1, 0, 4), (0, 1, 4), (0, 0, 3), (3, 5, 7)):
+        cache = Cache(kind, kvh, d, 1, 16, 6, 5, seed=9)
+        table = page_tables(rng, [n], 16, 5, 6)
+        dev = Device(torch, hip_ctx, cache)
+        stride = q_width + width + pad
+        x = rng.standard_normal((n, stride)).astype(np.float32)
+        buf = torch.zeros(offset + n * stride, device="cuda:0")
+        buf[offset:] = dev.up(x).reshape(-1)
+        pos, tab = dev.up(list(range(n)), np.int32), dev.up(np.repeat(table, n, axis=0), np.int32)
+        capi.check(dev.lib.air_hip_kv8_append(hip_ctx.handle, ctypes.byref(dev.kv), buf.data_ptr() + 4 * offset, stride,
+                                              q_width, n, pos.data_ptr(), tab.data_ptr(), 0))
+        cache.append(x, q_width, list(range(n)), np.repeat(table, n, axis=0), 0)
+        assert same(dev.pool(), cache.pool), (offset, pad, q_width)
+        size = (n + 2) * kvh * d
+        for at_k, at_v in ((1, 0), (0, 3), (2, 1)):
+            k, v = (torch.full((at + size + 1,), 7.0, device="cuda:0") for at in (at_k, at_v))
+            count = dev.up([n], np.int32)
+            capi.check(dev.lib.air_hip_kv8_read(hip_ctx.handle, ctypes.byref(dev.kv), 1, None, count.data_ptr(),
+                                                tab.data_ptr(), 0, 1, n + 2, k.data_ptr() + 4 * at_k,
+                                                v.data_ptr() + 4 * at_v, None))
+            torch.cuda.synchronize()
+            want_k, want_v, _ = cache.read(None, [n], table, 0, 1, n + 2, 7.0)
+            for got, want, at in ((k, want_k, at_k), (v, want_v, at_v)):
+                got = got.cpu().numpy()
+                assert np.array_equal(got[at:at + size], want.reshape(-1))
+                assert (got[:at] == 7.0).all() and got[-1] == 7.0
