@@ -331,3 +331,32 @@ def test_append_and_read_of_unaligned_rows(torch_cuda, hip_ctx, kind, kvh, d):
                 got = got.cpu().numpy()
                 assert np.array_equal(got[at:at + size], want.reshape(-1))
                 assert (got[:at] == 7.0).all() and got[-1] == 7.0
+
+
+def runs_of(lengths, rows_of, tables, empty_every):
+    """Rows at the end of each sequence, as runs with empty ones between."""
+    pos, tab, runs = [], [], []
+    for i, (n, b) in enumerate(zip(lengths, rows_of)):
+        runs.append((len(pos), len(pos) + b))
+        if i % empty_every == 0:
+            runs.append((len(pos) + b, len(pos) + b))
+        pos += range(n - b, n)
+        tab += [tables[i]] * b
+    return pos, np.array(tab), runs
+
+
+@pytest.mark.gpu
+@KINDS
+@pytest.mark.parametrize("q_heads,kvh,d", [(14, 2, 64), (6, 2, 128)])
+def test_many_ragged_runs_in_tiles_of_rows(torch_cuda, hip_ctx, kind, q_heads, kvh, d):
+    """More runs than a wave looks up at a time, of one to nineteen rows, in
+    tiles of four and of ten rows; empty runs among them and at both ends."""
+    rng = np.random.default_rng(161 + kind + d)
+    rows_of = [int(b) for b in rng.integers(1, 20, 75)]
+    lengths = [int(a) + b for a, b in zip(rng.integers(0, 40, 75), rows_of)]
+    cache, tables = filled(kind, kvh, d, lengths, rng, max_pages=30)
+    pos, tab, runs = runs_of(lengths, rows_of, tables, 8)
+    runs = [(0, 0)] + runs + [(len(pos), len(pos))] * 2
+    dev = Device(torch_cuda, hip_ctx, cache)
+    for mode in (None, "set", "add"):
+        attend(dev, rows(rng, len(pos), q_heads, kvh, d), pos, tab, q_heads, 480, runs, mode)
