@@ -360,3 +360,19 @@ def test_many_ragged_runs_in_tiles_of_rows(torch_cuda, hip_ctx, kind, q_heads, k
     dev = Device(torch_cuda, hip_ctx, cache)
     for mode in (None, "set", "add"):
         attend(dev, rows(rng, len(pos), q_heads, kvh, d), pos, tab, q_heads, 480, runs, mode)
+
+
+@pytest.mark.gpu
+@KINDS
+@pytest.mark.parametrize("d", [64, 128])
+def test_runs_tiles_with_a_wave_a_chunk_of_weights(torch_cuda, hip_ctx, kind, d):
+    """Runs of many vectors over keys that may be long: tiles, some of them
+    cut, whose weights a wave a chunk gathers."""
+    rng = np.random.default_rng(171 + kind + d)
+    q_heads, kvh, runs_n, b = 14, 2, 24, 12
+    lengths = [1450, 1300] + [int(n) for n in rng.integers(b, 60, runs_n - 2)]
+    cache, tables = filled(kind, kvh, d, lengths, rng, max_pages=208)
+    pos, tab, runs = runs_of(lengths, [b] * runs_n, tables, 100)
+    dev = Device(torch_cuda, hip_ctx, cache)
+    for mode in ("set", "add"):
+        attend(dev, rows(rng, len(pos), q_heads, kvh, d), pos, tab, q_heads, 208 * 16, runs, mode)
