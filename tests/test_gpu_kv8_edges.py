@@ -376,3 +376,17 @@ def test_runs_tiles_with_a_wave_a_chunk_of_weights(torch_cuda, hip_ctx, kind, d)
     dev = Device(torch_cuda, hip_ctx, cache)
     for mode in ("set", "add"):
         attend(dev, rows(rng, len(pos), q_heads, kvh, d), pos, tab, q_heads, 208 * 16, runs, mode)
+
+
+@pytest.mark.gpu
+@KINDS
+def test_rows_for_most_of_the_card_are_not_cut(torch_cuda, hip_ctx, kind):
+    """Forty rows of four KV heads under a bound far above most of them: a
+    workgroup a (row, KV head) takes all chunks, without and with weights."""
+    rng = np.random.default_rng(181 + kind)
+    q_heads, kvh, d = 8, 4, 128
+    lengths = [2700] + [int(n) for n in rng.integers(1, 90, 39)]
+    cache, tables = filled(kind, kvh, d, lengths, rng)
+    dev = Device(torch_cuda, hip_ctx, cache)
+    for mode in (None, "add", "set"):
+        attend(dev, rows(rng, 40, q_heads, kvh, d), [n - 1 for n in lengths], tables, q_heads, 2720, None, mode)
