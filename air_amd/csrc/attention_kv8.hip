@@ -33,12 +33,14 @@
 // its lead over M.
 //
 // What bounds it.  Decode over a cache larger than the chip's: reading it (48
-// rows over 4000..16000 tokens, 32 q heads on 8 KV heads of 128 dims: 193 us,
-// 5.1 TB/s of the 985 MB, as a large copy).  Fewer tokens: the waits of one
-// walk (32 rows over 500..1200 tokens: 11.3 us, 2.3 TB/s).  Prompts: the issue
-// of vector operations, some 20 a score (602 rows over 3300..3801 tokens, 28 q
-// heads: 85 us, 345 TFLOP/s of the products' 29 GFLOP; the matrix cores, which
-// do twice that for the operands' two halves, are busy a third of the time).
+// rows over 4000..16000 tokens, 32 q heads on 8 KV heads of 128 dims: 191 us,
+// 5.2 TB/s of the 985 MB, as a large copy).  Fewer tokens: the waits of one
+// walk (32 rows over 500..1200 tokens: 11.5 us, 2.3 TB/s).  Prompts: the
+// alternation of products and softmax.  Vector operations, some 20 a score, take
+// a third of the wave time and so do the matrix cores, which multiply both
+// halves of an operand; the two waves of a SIMD do the one and the other in
+// phases that hardly overlap (602 rows over 3300..3801 tokens, 28 q heads: 85
+// us, 345 TFLOP/s of the products' 29 GFLOP).
 #include "air_hip_device.hpp"
 #include "air_hip_kernels.hpp"
 #include "air_hip_kv8.hpp"
@@ -1133,7 +1135,10 @@ Kv8Shape kv8_attention_shape(std::uint32_t m, std::uint32_t q_heads, std::uint32
     // 660 calls (1..24 runs of 2..512 rows over up to 3000 tokens, 8 x 1, 8 x
     // 2, 8 x 4, 4 x 7, 2 x 14 and 8 x 16 heads of 64 and 128 dims) this takes
     // 0.7 % longer in the mean than the better of both, 30 % at most; runs'
-    // tiles always took 18 % longer, up to 1.8 times.
+    // tiles always took 18 % longer, up to 1.8 times.  Runs of one call were
+    // of about one length there.  63 rows of a decode step and a prompt's 512 in
+    // one call, 4 x 7 heads over 4000 tokens, take 136 us (43 and 79 in calls of
+    // their own), with weights 565 (78 and 136).
     const std::uint32_t run_rows = runs != 0u ? (m + runs - 1u) / runs : 0u;
     const std::uint32_t tile = kVectors * kRunTiles, parts = (group + tile - 1u) / tile;
     const std::uint32_t tile_rows = group < tile ? tile / group : 1u;
@@ -1175,25 +1180,29 @@ Kv8Shape kv8_attention_shape(std::uint32_t m, std::uint32_t q_heads, std::uint32
                          static_cast<std::uint32_t>(per)},
                         0u, kernel, false};
     };
-    // Single rows, by the better of six ways over 510 calls of equal and 510 of
-    // unequal lengths (1..128 rows, up to 16000 tokens, 2 x 7, 4 x 7 and 8 x 4
-    // heads): this rule lies 2 % off it in the mean and 20 % at most.
+    // Single rows, by the best of seven ways over 510 calls of equal and 510 of
+    // unequal lengths (1..128 rows, up to 16000 tokens, lengths within a factor of
+    // four, 2 x 7, 4 x 7 and 8 x 4 heads): this rule lies 2.4 and 0.8 % off it in
+    // the mean and 20 % at most.
     //
     // Eight waves a workgroup and one launch: up to two turns of the waves (32
-    // rows of 4 x 7 heads over 500..1200 tokens 11.8 us, 13.8 in splits), four
+    // rows of 4 x 7 heads over 500..1200 tokens 11.5 us, 14.2 in splits), four
     // with workgroups for half of the CUs, and any number where they fill
-    // them (64 such rows over 3000 tokens 33 us, 41 in splits).
+    // them (64 such rows over 3000 tokens 34 us, 38 in splits; 40 over 60000
+    // 478, 516 in splits).  That is for lengths much alike: of 40 rows one over
+    // 131072 tokens and the others over 1000, the long one's four workgroups walk
+    // 747 us, where splits take 278 (one over 16000: 97, 47).
     const bool full = head_dim == 128u && row_pairs >= 160u;
     if (row_pairs <= 256u && (chunks <= 16u || (chunks <= 32u && row_pairs >= 128u) || full)) {
         return shape(chunks, kKv8ShortRows);
     }
     // More short rows than that: the splits' meeting would cost more than they
-    // even out (128 rows over 600 tokens 18 us, 24 in splits).
+    // even out (128 rows over 600 tokens 19 us, 25 in splits).
     if (chunks <= 48u && row_pairs >= 320u) return shape(chunks, kKv8Rows);
     // Splits of equal length, so that rows of unequal lengths make workgroups
     // of equal work, as many as run at a time if every row were max_tokens
     // long: three a CU, or four with the registers of 64 dims.  At least a
-    // chunk a wave (one row over 2000 tokens 10.5 us, 15.3 unsplit), two where
+    // chunk a wave (one row over 2000 tokens 11 us, 19 unsplit), two where
     // there are many.
     const std::uint64_t slots = head_dim == 128u ? 768u : 1024u, least = chunks <= 32u ? kWaves : 2u * kWaves;
     std::uint64_t per = (row_pairs * chunks + slots - 1u) / slots;

@@ -347,6 +347,8 @@ __device__ __forceinline__ std::int64_t held_tokens(const Kv8Geometry& g, std::i
 // are read once, into LDS, and digits and places are found with prefix sums:
 // 1000 tokens to 500 in 7 us, 4096 to 1024 in 13 (16 by four bytes, whose
 // first has few values and many additions to one bin), the rounds' barriers.
+// Past kSelectKeys every round reads the weights again, 64 bytes of each block
+// (131072 tokens to 2048, gathered too, in 404).
 __global__ __launch_bounds__(kSelectThreads) void kv8_select_kernel(
     Kv8Geometry g, const std::int32_t* __restrict__ lengths, const std::int32_t* __restrict__ tables,
     std::uint32_t layer, std::uint32_t layers, std::uint32_t keep_first, std::uint32_t keep_last, std::uint32_t budget,
@@ -462,7 +464,7 @@ __global__ __launch_bounds__(kSelectThreads) void kv8_select_kernel(
 // ratio its codes take are found once, by 16 threads for K and 16 for V.
 // With a quarter of the tokens kept nearly every 64-byte piece of the old
 // codes is touched: the old sequence is read whole (six layers of sequences
-// of 900..4100 tokens, 63 MB, and 25 MB written, in 33 us).  Measured slower:
+// of 900..4100 tokens, 63 MB, and 25 MB written, in 32 us).  Measured slower:
 // four blocks a workgroup with their loads together (41 us), and 16 bytes a
 // dim and old block with the tokens picked from registers (52 us) or from LDS
 // (36 us); fewer workgroups a CU then cover each other's waits.

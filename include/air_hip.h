@@ -666,8 +666,9 @@ int air_hip_kv8_append(air_hip_context* ctx, const air_hip_kv8_layout* kv, const
                        uint32_t layer);
 
 /* Tokens starts[i] .. starts[i] + lengths[i] - 1 (starts null: from 0; at
- * most max_tokens) of `sequences` sequences (page_tables: int32
- * [sequences][max_pages]) in layers [layer, layer + layers) as f32 values:
+ * most max_tokens, which is at most max_pages * page_tokens) of `sequences`
+ * sequences (page_tables: int32 [sequences][max_pages]) in layers [layer, layer
+ * + layers) as f32 values:
  *   k, v     [layers][sequences][max_tokens][kv_heads * head_dim]
  *   weights  [layers][sequences][max_tokens][kv_heads]
  * any of them null.  What lies behind a sequence's tokens, and tokens without
@@ -677,7 +678,8 @@ int air_hip_kv8_read(air_hip_context* ctx, const air_hip_kv8_layout* kv, uint32_
                      uint64_t max_tokens, float* k, float* v, float* weights);
 
 /* Attention of every row's q heads over slots 0..positions[r] of its sequence
- * (below max_tokens, which bounds the work and sizes the context's scratch):
+ * (below max_tokens <= max_pages * page_tokens, which bounds the work, sizes
+ * the context's scratch and, with m and runs, decides how the work is cut):
  * out [m][q_heads * head_dim], f32 accurate over the stored values (both
  * products carry their f32 operand as two f16 parts, sums in f32): q to 2^-22
  * of its vector's largest magnitude (or to 2^-133, if that is more), scores of
@@ -716,9 +718,10 @@ int air_hip_kv8_attention(air_hip_context* ctx, const air_hip_kv8_layout* kv, co
  * those between the ones of largest weight (equal weights: the lowest slots;
  * NaN ranks lowest), in their order, in slots 0..budget - 1 of the pages of
  * new_page_tables, with their weights.  Shorter sequences keep every token.
- * The caller's new length is min(lengths[i], budget).  A new block's scale is
- * the largest of its tokens' scales; codes are rounded again where it differs
- * (code * (old / new), f32).
+ * The caller's new length is the least of lengths[i], max_tokens (at most
+ * max_pages * page_tokens) and budget.  A new block's scale is the largest of
+ * its tokens' scales; codes are rounded again where it differs (code * (old /
+ * new), f32).
  *   new_page_tables  int32 [sequences][max_pages]: either page_tables itself
  *                    (the same pointer), which shortens in place, or tables
  *                    whose pages no page_tables of the call names; pages of
